@@ -68,6 +68,13 @@ typedef struct ttamd_view4 {
     int64_t stride[4];
 } ttamd_view4;
 
+/* A strided matrix (row and column stride). */
+typedef struct ttamd_view2 {
+    const void *data;
+    int64_t offset;
+    int64_t stride[2];
+} ttamd_view2;
+
 /* Epilogue fused into the GEMM's store phase.  All fields 0/NULL = plain C = A.B, which is
  * what BackendBase::batched_matmul computes.  The other modes serve the callers either side
  * of the GEMM: nn::Linear's `+ bias->expand()` (tinytensor/nn/linear.cpp:45-48), the ReLU
@@ -328,6 +335,66 @@ ttamd_status ttamd_linear_mse_head(int device, ttamd_dtype dtype, int64_t rows, 
                                    const void *input, const void *weight, const void *bias, const void *target,
                                    const void *relu_input, void *output, void *loss_out, void *grad_output_out,
                                    void *grad_input_out, void *grad_weight_out, void *grad_bias_out, void *stream);
+
+/* ---- operators of a language-model student: tokens in, a gated block, a teacher's logits as the target ----------------
+ * No counterpart in the reference; they stand beside nn::Linear (nn/linear.cpp:42-50) and nn::mse_loss
+ * (nn/loss.cpp:69-72).  f32 / f64.  Results are dense row-major and may not overlap an operand.  A `workspace` is device
+ * memory of the size that the matching _workspace call names (host arithmetic only), the caller's own for the call: calls
+ * that may run at the same time, and graphs that may be replayed at the same time, need one each.  Nothing is kept in it
+ * between calls.  Only kernels are enqueued (no memset or copy nodes).  Results are the same bits on every call. */
+
+/* Rows of a table by token: out[i, :] = scale * table[index[i], :] for i < count, out dense [count, dim].  index: dense,
+ * i32 or i64.  table: element (v, d) at table[v * row_stride + d * col_stride], strides >= 0 (a transposed weight is read
+ * in place).  An index below 0 or from vocab on names no row and gives a row of zeros: padding.
+ * vocab <= 2^28, dim <= 2^21, count < 2^31. */
+ttamd_status ttamd_embedding_forward(int device, ttamd_dtype dtype, ttamd_dtype index_dtype, int64_t count, int64_t vocab,
+                                     int64_t dim, const void *index, const void *table, int64_t row_stride,
+                                     int64_t col_stride, double scale, void *out, void *stream);
+/* Its gradient: grad_table[v, :] = scale * sum of grad_out[i, :] over the i with index[i] == v, for every v < vocab (zeros
+ * where there is none); accumulate != 0: grad_table += that, rows without a position are left alone.  grad_out
+ * [count, dim] and grad_table [vocab, dim] dense.  Sums run over the positions in groups whose order the indices fix, in
+ * 64 bits. */
+ttamd_status ttamd_embedding_backward_workspace(ttamd_dtype dtype, int64_t count, int64_t vocab, int64_t dim, size_t *bytes);
+ttamd_status ttamd_embedding_backward(int device, ttamd_dtype dtype, ttamd_dtype index_dtype, int64_t count, int64_t vocab,
+                                      int64_t dim, const void *grad_out, const void *index, double scale, int accumulate,
+                                      void *grad_table, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The gated pair of Linear layers of a feed-forward block: g = x . Wg + bg, u = x . Wu + bu, out = act(g) * u.
+ * input [rows, inner], gate_weight and up_weight [inner, hidden]: any non-negative strides, read in place.  gate_bias,
+ * up_bias: dense [hidden], each may be NULL.  out [rows, hidden].  gate_out / up_out: both or neither; they receive g and
+ * u, what the backward pass reads.  gelu is the exact (erf) form. */
+typedef enum ttamd_activation { TTAMD_ACT_SILU = 0, TTAMD_ACT_GELU = 1, TTAMD_ACT_RELU = 2, TTAMD_ACT_SIGMOID = 3 } ttamd_activation;
+ttamd_status ttamd_gated_linear_workspace(ttamd_dtype dtype, int64_t rows, int64_t inner, int64_t hidden, int backward,
+                                          size_t *bytes);
+ttamd_status ttamd_gated_linear_forward(int device, ttamd_dtype dtype, int activation, int64_t rows, int64_t inner,
+                                        int64_t hidden, const ttamd_view2 *input, const ttamd_view2 *gate_weight,
+                                        const ttamd_view2 *up_weight, const void *gate_bias, const void *up_bias, void *out,
+                                        void *gate_out, void *up_out, void *workspace, size_t workspace_bytes, void *stream);
+/* Its backward pass from grad_out = d loss / d out and the saved g and u (all dense [rows, hidden]):
+ * dg = grad_out * u * act'(g), du = grad_out * act(g); grad_input [rows, inner] = dg . Wg^T + du . Wu^T;
+ * grad_{gate,up}_weight [inner, hidden] = x^T . d{g,u}; grad_{gate,up}_bias [hidden] (each may be NULL) = column sums of
+ * d{g,u}.  relu's derivative is 1 at 0, as TensorRelu::backward has it (autograd/unary_ops.cpp:568-573).  rows = 0: the
+ * weights' and biases' gradients are zeros. */
+ttamd_status ttamd_gated_linear_backward(int device, ttamd_dtype dtype, int activation, int64_t rows, int64_t inner,
+                                         int64_t hidden, const void *grad_out, const ttamd_view2 *input,
+                                         const ttamd_view2 *gate_weight, const ttamd_view2 *up_weight, const void *gate,
+                                         const void *up, void *grad_input, void *grad_gate_weight, void *grad_up_weight,
+                                         void *grad_gate_bias, void *grad_up_bias, void *workspace, size_t workspace_bytes,
+                                         void *stream);
+
+/* Distillation from a teacher's top logits, loss and gradient in one call.  With T the temperature and, for every row,
+ *   p = softmax of teacher_logit / T over the row's valid slots,  q = softmax of input / T over all cols columns,
+ *   loss_out [1] = sum over rows of row_weight * T^2 * sum_j p_j (log p_j - log q[teacher_index_j]),
+ *   grad_input_out [rows, cols] = d loss / d input = row_weight * T * (q - p at the teacher's columns).
+ * input: rows of cols elements, input_row_stride >= cols apart; teacher_index (i32 / i64) and teacher_logit: dense
+ * [rows, top], 1 <= top <= 1024.  A slot whose index lies outside the columns is padding; one whose logit is -inf has
+ * p = 0; an index may come twice.  row_weight: dense [rows] or NULL (1 / rows each: the mean).  A row of weight 0, or
+ * without a slot that counts, adds nothing, has a gradient of zeros and is not read. */
+ttamd_status ttamd_distill_loss_workspace(ttamd_dtype dtype, int64_t rows, int64_t cols, int64_t top, size_t *bytes);
+ttamd_status ttamd_distill_loss(int device, ttamd_dtype dtype, ttamd_dtype index_dtype, int64_t rows, int64_t cols, int64_t top,
+                                const void *input, int64_t input_row_stride, const void *teacher_index,
+                                const void *teacher_logit, const void *row_weight, double temperature, void *loss_out,
+                                void *grad_input_out, void *workspace, size_t workspace_bytes, void *stream);
 
 /* BackendBase::uniform_real_ / normal_ (backend_base.h:96-103) for a dense float tensor with scalar parameters, as
  * nn::Linear's default initialisation calls them (nn/init.cpp:30-52,106-112).  dist 0 = uniform_real(low = p0,

@@ -1,0 +1,146 @@
+"""What the student operators (embedding, gated pair, distillation loss) refuse, answered on the host before any device is
+touched, and their workspace sizes.  No GPU needed."""
+import ctypes as C
+
+import pytest
+
+A = 1 << 20  # an address that looks like device memory; no call here gets as far as using it
+
+
+def view(capi, data=A, offset=0, stride=(8, 1)):
+    v = capi.View2()
+    v.data, v.offset = data, offset
+    v.stride[0], v.stride[1] = stride
+    return C.byref(v)
+
+
+def embed(tt, dtype=None, index_dtype=None, count=4, vocab=10, dim=8, index=A, table=2 * A, rs=8, cs=1, out=3 * A):
+    capi = tt._capi
+    return capi.lib.ttamd_embedding_forward(0, capi.F32 if dtype is None else dtype, capi.I32 if index_dtype is None else index_dtype, count,
+                                            vocab, dim, index, table, rs, cs, 1.0, out, None)
+
+
+def test_embedding_refusals(tt):
+    capi = tt._capi
+    assert embed(tt, dtype=capi.I32) == capi.ERR_UNSUPPORTED_DTYPE
+    assert embed(tt, dtype=42) == capi.ERR_UNSUPPORTED_DTYPE
+    for bad in (capi.F32, capi.U8, capi.BOOL, 42):
+        assert embed(tt, index_dtype=bad) == capi.ERR_UNSUPPORTED_DTYPE
+    for kw in (dict(count=-1), dict(vocab=0), dict(dim=0), dict(count=1 << 31), dict(vocab=(1 << 28) + 1), dict(dim=(1 << 21) + 1),
+               dict(rs=-1), dict(cs=-1), dict(index=None), dict(table=None), dict(out=None), dict(table=A + 2), dict(out=A + 1),
+               dict(index=A + 2)):
+        assert embed(tt, **kw) == capi.ERR_INVALID_ARGUMENT, kw
+        assert b"embedding" in capi.lib.ttamd_last_error_string()
+
+
+def test_embedding_backward_refusals(tt):
+    capi, lib = tt._capi, tt._capi.lib
+    n = C.c_size_t()
+    query = lib.ttamd_embedding_backward_workspace
+    assert query(capi.I32, 4, 10, 8, C.byref(n)) == capi.ERR_UNSUPPORTED_DTYPE
+    assert query(capi.F32, 4, 0, 8, C.byref(n)) == capi.ERR_INVALID_ARGUMENT
+    assert query(capi.F32, 4, 10, 8, None) == capi.ERR_INVALID_ARGUMENT
+    assert query(capi.F32, 4, 10, 8, C.byref(n)) == capi.OK and n.value > 0
+    need = n.value
+
+    def call(index_dtype=capi.I32, count=4, dy=A, index=2 * A, grad=3 * A, ws=4 * A, size=need):
+        return lib.ttamd_embedding_backward(0, capi.F32, index_dtype, count, 10, 8, dy, index, 1.0, 0, grad, ws, size, None)
+
+    assert call(index_dtype=capi.F32) == capi.ERR_UNSUPPORTED_DTYPE
+    for kw in (dict(count=-1), dict(dy=None), dict(index=None), dict(grad=None), dict(ws=None), dict(size=need - 1), dict(dy=A + 1),
+               dict(grad=A + 2), dict(ws=A + 4), dict(index=A + 1)):
+        assert call(**kw) == capi.ERR_INVALID_ARGUMENT, kw
+
+
+def test_gated_linear_refusals(tt):
+    capi, lib = tt._capi, tt._capi.lib
+    n = C.c_size_t()
+    assert lib.ttamd_gated_linear_workspace(capi.I64, 3, 8, 8, 0, C.byref(n)) == capi.ERR_UNSUPPORTED_DTYPE
+    assert lib.ttamd_gated_linear_workspace(capi.F32, 3, 0, 8, 0, C.byref(n)) == capi.ERR_INVALID_ARGUMENT
+    assert lib.ttamd_gated_linear_workspace(capi.F32, 3, 8, 8, 0, None) == capi.ERR_INVALID_ARGUMENT
+    assert lib.ttamd_gated_linear_workspace(capi.F32, 3, 8, 8, 1, C.byref(n)) == capi.OK
+
+    def forward(dtype=capi.F32, act=0, rows=3, x=view(capi), wg=view(capi), wu=view(capi), out=2 * A, gate=None, up=None, ws=3 * A, size=1 << 30):
+        return lib.ttamd_gated_linear_forward(0, dtype, act, rows, 8, 8, x, wg, wu, None, None, out, gate, up, ws, size, None)
+
+    assert forward(dtype=capi.I32) == capi.ERR_UNSUPPORTED_DTYPE
+    for kw in (dict(act=4), dict(act=-1), dict(rows=-1), dict(x=None), dict(wg=view(capi, data=None)), dict(wu=view(capi, offset=-1)),
+               dict(wu=view(capi, stride=(8, -1))), dict(x=view(capi, data=A + 2)), dict(out=None), dict(out=A + 1), dict(gate=4 * A),
+               dict(up=4 * A), dict(ws=3 * A + 4)):
+        assert forward(**kw) == capi.ERR_INVALID_ARGUMENT, kw
+
+    def backward(act=0, dh=A, gate=A, up=A, dx=2 * A, dwg=3 * A, dwu=4 * A, ws=5 * A, size=1 << 30, x=view(capi)):
+        return lib.ttamd_gated_linear_backward(0, capi.F32, act, 3, 8, 8, dh, x, view(capi), view(capi), gate, up, dx, dwg, dwu, None, None, ws, size, None)
+
+    for kw in (dict(act=9), dict(dh=None), dict(gate=None), dict(up=None), dict(dx=None), dict(dwg=None), dict(dwu=None), dict(ws=None),
+               dict(size=8), dict(dh=A + 2), dict(dwu=A + 3), dict(x=None)):
+        assert backward(**kw) == capi.ERR_INVALID_ARGUMENT, kw
+
+
+def test_distill_loss_refusals(tt):
+    capi, lib = tt._capi, tt._capi.lib
+    n = C.c_size_t()
+    query = lib.ttamd_distill_loss_workspace
+    assert query(capi.BOOL, 3, 8, 2, C.byref(n)) == capi.ERR_UNSUPPORTED_DTYPE
+    for rows, cols, top in ((-1, 8, 2), (3, 0, 2), (3, 8, 0), (3, 8, 1025), (3, 1 << 30, 2)):
+        assert query(capi.F32, rows, cols, top, C.byref(n)) == capi.ERR_INVALID_ARGUMENT
+    assert query(capi.F32, 3, 8, 2, C.byref(n)) == capi.OK
+    need = n.value
+
+    def call(index_dtype=capi.I64, z=A, stride=8, index=2 * A, logit=3 * A, weight=None, t=1.0, loss=4 * A, grad=5 * A, ws=6 * A, size=need):
+        return lib.ttamd_distill_loss(0, capi.F32, index_dtype, 3, 8, 2, z, stride, index, logit, weight, t, loss, grad, ws, size, None)
+
+    for bad in (capi.U8, capi.F32):
+        assert call(index_dtype=bad) == capi.ERR_UNSUPPORTED_DTYPE
+    for kw in (dict(stride=7), dict(t=0.0), dict(t=-1.0), dict(t=float("nan")), dict(t=float("inf")), dict(z=None), dict(index=None),
+               dict(logit=None), dict(loss=None), dict(grad=None), dict(ws=None), dict(size=need - 1), dict(z=A + 2), dict(index=A + 4),
+               dict(weight=A + 1), dict(ws=A + 4), dict(grad=A), dict(grad=A + 4 * 16)):
+        assert call(**kw) == capi.ERR_INVALID_ARGUMENT, kw
+    call(grad=A)
+    assert b"over the logits" in lib.ttamd_last_error_string()
+
+
+class _Memory:
+    """A storage without a device behind it."""
+
+    def __init__(self, device):
+        self.ptr, self.nbytes, self.device = A, 1 << 20, device
+
+
+def test_python_argument_checks(tt):
+    capi, Dev = tt._capi, tt.Device("amd", 1)
+
+    def t(shape, dtype=capi.F32, device=tt.kAMD, stride=None):
+        return tt.Tensor(_Memory(device), dtype, shape, stride)
+
+    ids, table = t((2, 3), capi.I64), t((10, 8))
+    for call in (
+        lambda: tt.embedding(ids, t((10, 8, 1))),
+        lambda: tt.embedding(t((2, 3)), table),
+        lambda: tt.embedding(t((2, 3), capi.BOOL), table),
+        lambda: tt.embedding(ids, t((10, 8), capi.I32)),
+        lambda: tt.embedding(t((2, 3), capi.I64, Dev), table),
+        lambda: tt.embedding(ids, table, out=t((2, 8))),
+        lambda: tt.embedding(ids, table, out=t((2, 3, 8), capi.F64)),
+        lambda: tt.embedding(ids, table, out=t((2, 3, 8), stride=(48, 16, 2))),
+        lambda: tt.embedding_backward(t((2, 4, 8)), ids, 10),
+        lambda: tt.embedding_backward(t((2, 3, 8)), ids, 10, accumulate=True),
+        lambda: tt.embedding_backward(t((2, 3, 8)), ids, 10, out=t((9, 8))),
+        lambda: tt.gated_linear(t((4, 8)), t((8, 6)), t((8, 5))),
+        lambda: tt.gated_linear(t((4, 7)), t((8, 6)), t((8, 6))),
+        lambda: tt.gated_linear(t((4, 8)), t((8, 6)), t((8, 6), capi.F64)),
+        lambda: tt.gated_linear(t((4, 8)), t((8, 6)), t((8, 6)), activation="tanh"),
+        lambda: tt.gated_linear(t((4, 8)), t((8, 6)), t((8, 6)), b_gate=t((5,))),
+        lambda: tt.gated_linear(t((4, 8)), t((8, 6)), t((8, 6)), out=t((4, 5))),
+        lambda: tt.gated_linear_backward(t((4, 6)), t((4, 8)), t((8, 6)), t((8, 6)), t((4, 6)), t((4, 5))),
+        lambda: tt.gated_linear_backward(t((4, 6)), t((2, 2, 8)), t((8, 6)), t((8, 6)), t((4, 6)), t((4, 6))),
+        lambda: tt.gated_linear_backward(t((4, 6)), t((4, 8)), t((8, 6)), t((8, 6)), t((4, 6)), t((4, 6)), out=(None,) * 3),
+        lambda: tt.distill_loss(t((4, 8)), t((4, 2), capi.I64), t((4, 3))),
+        lambda: tt.distill_loss(t((4, 8)), t((5, 2), capi.I64), t((5, 2))),
+        lambda: tt.distill_loss(t((4, 8)), t((4, 2)), t((4, 2))),
+        lambda: tt.distill_loss(t((4, 8)), t((4, 2), capi.I32), t((4, 2), capi.F64)),
+        lambda: tt.distill_loss(t((4, 8)), t((4, 2), capi.I32), t((4, 2)), row_weight=t((3,))),
+        lambda: tt.distill_loss(t((4, 8)), t((4, 2), capi.I32), t((4, 2)), out=(t((1,)), t((4, 9)))),
+    ):
+        with pytest.raises(tt.TTException):
+            call()

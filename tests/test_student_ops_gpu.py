@@ -1,0 +1,592 @@
+"""The operators of a language-model student on the GPU -- embedding, the gated pair of Linear layers, the distillation
+loss -- against their formulas in 64 bits, at the sizes, views and masks where they can go wrong.
+
+Tolerances count roundings: u is half a step of the type (2^-24, 2^-53)."""
+import zlib
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [np.float32, np.float64]
+U = {np.float32: 2.0 ** -24, np.float64: 2.0 ** -53}
+ACTS = ["silu", "gelu", "relu", "sigmoid"]
+
+
+def rng_of(*key):
+    return np.random.default_rng([zlib.crc32(k.encode()) if isinstance(k, str) else int(k) for k in key])
+
+
+def framed(tt, shape, dtype, margin=37):
+    """A result tensor inside a larger buffer of a known pattern, and a check that the pattern around it is intact."""
+    n = int(np.prod(shape))
+    host = np.full(n + 2 * margin, 77.0, dtype)
+    whole = tt.Tensor.from_numpy(host)
+    t = tt.Tensor(whole.storage, whole.dtype, shape, None, margin)
+
+    def intact():
+        back = whole.to_numpy()
+        return np.all(back[:margin] == 77.0) and np.all(back[margin + n:] == 77.0)
+
+    return t, intact
+
+
+# ---- embedding -----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("index", [np.int32, np.int64, np.uint8, np.int16])
+@pytest.mark.parametrize("shape, vocab, dim", [((1,), 1, 1), ((3,), 5, 1), ((2, 7), 11, 3), ((65,), 100, 4), ((1,), 100, 1024),
+                                               ((5, 3), 40, 333), ((300,), 17, 66), ((9,), 120, 2051), ((0,), 7, 5)])
+def test_embedding_rows(tt, dtype, index, shape, vocab, dim):
+    r = rng_of(vocab, dim, 1)
+    table = r.normal(0, 1, (vocab, dim)).astype(dtype)
+    ids = r.integers(0, vocab, shape).astype(index)
+    scale = 3.3
+    out, intact = framed(tt, shape + (dim,), dtype)
+    got = tt.embedding(tt.Tensor.from_numpy(ids), tt.Tensor.from_numpy(table), scale=scale, out=out)
+    assert got is out
+    assert np.array_equal(out.to_numpy(), table[ids.astype(np.int64)] * dtype(scale))  # one product, rounded once: exact
+    assert intact()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_embedding_views_and_padding(tt, dtype):
+    r = rng_of(3)
+    base = r.normal(0, 1, (64, 50)).astype(dtype)
+    ids = np.array([[0, 49, 7], [-1, 50, 3]], np.int64)
+    t = tt.Tensor.from_numpy(base)
+    tied = t.permute(1, 0)  # a Linear weight [in, out] as a table of `out` rows, read in place
+    got = tt.embedding(tt.Tensor.from_numpy(ids), tied, scale=0.5).to_numpy()
+    want = np.where(((ids >= 0) & (ids < 50))[..., None], base.T[np.clip(ids, 0, 49)] * dtype(0.5), dtype(0))
+    assert np.array_equal(got, want)
+    # rows further apart than they are long, a first element off every boundary
+    part = tt.Tensor(t.storage, t.dtype, (40, 31), (50, 1), 53)
+    ids2 = r.integers(-3, 43, (70,)).astype(np.int32)
+    rows = base.reshape(-1)[53:][np.arange(40)[:, None] * 50 + np.arange(31)]
+    want = np.where(((ids2 >= 0) & (ids2 < 40))[:, None], rows[np.clip(ids2, 0, 39)], dtype(0))
+    assert np.array_equal(tt.embedding(tt.Tensor.from_numpy(ids2), part).to_numpy(), want)
+    # one row for every token, and indices that are a strided view themselves
+    one = tt.Tensor(t.storage, t.dtype, (9, 50), (0, 1), 100)
+    idv = tt.Tensor.from_numpy(np.arange(12, dtype=np.int32).reshape(3, 4)).permute(1, 0)
+    got = tt.embedding(idv, one).to_numpy()
+    assert got.shape == (4, 3, 50)
+    want = np.where((np.arange(12).reshape(3, 4).T < 9)[..., None], base[2], dtype(0))
+    assert np.array_equal(got, want)
+
+
+def embedding_gradient(dy, ids, vocab, scale):
+    """(gradient, sum of magnitudes, rows a token) in 64 bits."""
+    g, m, n = np.zeros((vocab, dy.shape[-1])), np.zeros((vocab, dy.shape[-1])), np.zeros(vocab)
+    ok = (ids >= 0) & (ids < vocab)
+    np.add.at(g, ids[ok], dy[ok].astype(np.float64))
+    np.add.at(m, ids[ok], np.abs(dy[ok]).astype(np.float64))
+    np.add.at(n, ids[ok], 1)
+    return g * scale, m * abs(scale), n
+
+
+def check_embedding_gradient(got, dy, ids, vocab, scale, dtype, before=None):
+    want, mag, n = embedding_gradient(dy, ids, vocab, scale)
+    if before is not None:
+        want = want + before
+    # sums in 64 bits (n + 2 roundings of 2^-53 of the magnitudes, and the comparison's own sum as many), rounded once
+    tol = U[dtype] * np.abs(want) + 2 * (n[:, None] + 3) * 2.0 ** -53 * (mag + (0 if before is None else np.abs(before)))
+    assert np.all(np.abs(got.astype(np.float64) - want) <= tol)
+    return n
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("index", [np.int32, np.int64])
+@pytest.mark.parametrize("count, vocab, dim", [(1, 1, 1), (1, 300, 8), (5, 3, 7), (16, 1, 4), (17, 1, 5), (257, 2, 3), (100, 1000, 333), (1000, 37, 130),
+                                               (4096, 600, 64), (3000, 140000, 12), (700, 513, 1028), (0, 9, 6), (5000, 1, 260)])
+def test_embedding_gradient(tt, dtype, index, count, vocab, dim):
+    r = rng_of(count, vocab, dim)
+    dy = r.normal(0, 1, (count, dim)).astype(dtype)
+    ids = (r.random(count) ** 3 * (vocab + 2)).astype(index) - 1  # a few tokens often; -1 and vocab: padding
+    out, intact = framed(tt, (vocab, dim), dtype)
+    tt.embedding_backward(tt.Tensor.from_numpy(dy), tt.Tensor.from_numpy(ids), vocab, scale=1.7, out=out)
+    got = out.to_numpy()
+    n = check_embedding_gradient(got, dy, ids, vocab, 1.7, dtype)
+    assert np.all(got[n == 0] == 0)
+    assert intact()
+    # the same bits again, and added to what is there
+    again = tt.embedding_backward(tt.Tensor.from_numpy(dy), tt.Tensor.from_numpy(ids), vocab, scale=1.7).to_numpy()
+    assert np.array_equal(got, again)
+    before = r.normal(0, 1, (vocab, dim)).astype(dtype)
+    acc = tt.Tensor.from_numpy(before)
+    tt.embedding_backward(tt.Tensor.from_numpy(dy), tt.Tensor.from_numpy(ids), vocab, scale=1.7, out=acc, accumulate=True)
+    check_embedding_gradient(acc.to_numpy(), dy, ids, vocab, 1.7, dtype, before.astype(np.float64))
+    assert np.array_equal(acc.to_numpy()[n == 0], before[n == 0])
+
+
+@pytest.mark.parametrize("pattern", ["one", "blocks", "bucket", "borders"])
+def test_embedding_gradient_runs(tt, pattern):
+    """Runs of equal tokens that fill, end at, cross and span the groups that are added up together."""
+    count, vocab, dim = 2048, 1024, 20
+    i = np.arange(count)
+    ids = {"one": np.full(count, 5), "blocks": i // 16, "bucket": (i * 7 % 4) * 256 + 3, "borders": np.where(i < 15, 1, np.where(i < 33, 2, np.where(i < 48, 3, 4 + i // 100)))}[pattern]
+    r = rng_of(7)
+    ids = ids[r.permutation(count)].astype(np.int32)
+    dy = r.integers(-8, 9, (count, dim)).astype(np.float32)  # whole numbers: the sums are exact
+    got = tt.embedding_backward(tt.Tensor.from_numpy(dy), tt.Tensor.from_numpy(ids), vocab).to_numpy()
+    assert np.array_equal(got.astype(np.float64), embedding_gradient(dy, ids, vocab, 1.0)[0])
+
+
+# ---- the gated pair ------------------------------------------------------------------------------------------------------
+
+
+def erf(x):
+    from scipy.special import erf as f
+    return f(x)
+
+
+def act_of(g, act):
+    if act == "relu":
+        return np.maximum(g, 0), np.where(g < 0, 0.0, 1.0)
+    if act == "gelu":
+        cdf = 0.5 * (1 + erf(g * 0.5 ** 0.5))
+        return g * cdf, cdf + g * np.exp(-0.5 * g * g) / (2 * np.pi) ** 0.5
+    with np.errstate(over="ignore"):
+        s = 1 / (1 + np.exp(-g))
+    return (s, s * (1 - s)) if act == "sigmoid" else (g * s, s * (1 + g * (1 - s)))
+
+
+def act_error(g, act, u):
+    """Bounds of |act(g)|'s and |act'(g)|'s errors.  s = 1 / (1 + exp(-g)): exp within 2 steps (4 u), a sum, a quotient: 6 u
+    of s, and 7 u absolute in 1 - s; the products add a few u each.  erf within 2 steps of a value up to 1 (4 u), its
+    argument's rounding 1 u more, halved: 3 u absolute in the distribution function, 8 u with the products."""
+    if act == "relu":
+        return 0 * g, 0 * g
+    value = 8 * u * (np.ones_like(g) if act == "sigmoid" else np.abs(g))
+    return value, 20 * u * (1 + np.abs(g))
+
+
+def gated_reference(x, wg, wu, bg, bu, act):
+    x, wg, wu = (a.astype(np.float64) for a in (x, wg, wu))
+    g, u = x @ wg, x @ wu
+    if bg is not None:
+        g = g + bg.astype(np.float64)
+    if bu is not None:
+        u = u + bu.astype(np.float64)
+    return g, u
+
+
+def product_error(a, b, u, extra=0.0):
+    """(terms + 2) roundings of the magnitudes: an inner product of any order of summation, and a bias."""
+    return (a.shape[1] + 2 + extra) * u * (np.abs(a).astype(np.float64) @ np.abs(b).astype(np.float64))
+
+
+def check_gated(tt, dtype, act, x, wg, wu, bg, bu, tx, twg, twu, dh=None, save=True):
+    u_ = U[dtype]
+    put = lambda a: tt.Tensor.from_numpy(a) if a is not None else None  # noqa: E731
+    hidden = wg.shape[1]
+    g, u = gated_reference(x, wg, wu, bg, bu, act)
+    eg = product_error(x, wg, u_) + (u_ * np.abs(bg) if bg is not None else 0)
+    eu = product_error(x, wu, u_) + (u_ * np.abs(bu) if bu is not None else 0)
+    value, slope = act_of(g, act)
+    ev, _ = act_error(g, act, u_)
+    th = framed(tt, (x.shape[0], hidden), dtype)
+    plain = tt.gated_linear(tx, twg, twu, put(bg), put(bu), activation=act, out=th[0])
+    assert plain is th[0] and th[1]()
+    h, sg, su = tt.gated_linear(tx, twg, twu, put(bg), put(bu), activation=act, save=True)
+    # act' is at most 1.13 in magnitude for these, so an error of g reaches act(g) 1.2 times at most
+    tol = (ev + 1.2 * eg) * (np.abs(u) + eu) + np.abs(value) * eu + 2 * u_ * np.abs(value * u)
+    for got in (plain.to_numpy(), h.to_numpy()):
+        assert np.all(np.abs(got - value * u) <= tol + 1e-300)
+    assert np.all(np.abs(sg.to_numpy() - g) <= eg) and np.all(np.abs(su.to_numpy() - u) <= eu)
+    if dh is None:
+        return
+    # backward from the saved g and u as they are
+    g, u = sg.to_numpy().astype(np.float64), su.to_numpy().astype(np.float64)
+    value, slope = act_of(g, act)
+    ev, es = act_error(g, act, u_)
+    d = dh.astype(np.float64)
+    dg, du = d * u * slope, d * value
+    edg, edu = np.abs(d * u) * es + 3 * u_ * np.abs(dg), np.abs(d) * ev + 2 * u_ * np.abs(du)
+    want = (dg @ wg.T.astype(np.float64) + du @ wu.T.astype(np.float64), x.T.astype(np.float64) @ dg, x.T.astype(np.float64) @ du,
+            dg.sum(0), du.sum(0))
+    tol = (edg @ np.abs(wg.T) + edu @ np.abs(wu.T) + product_error(np.concatenate([dg, du], 1), np.concatenate([wg.T, wu.T], 0), u_, 2),
+           np.abs(x.T) @ edg + product_error(x.T, dg, u_), np.abs(x.T) @ edu + product_error(x.T, du, u_),
+           edg.sum(0) + (len(dg) + 2) * u_ * np.abs(dg).sum(0), edu.sum(0) + (len(du) + 2) * u_ * np.abs(du).sum(0))
+    frames = [framed(tt, w.shape, dtype) for w in want]
+    got = tt.gated_linear_backward(put(dh), tx, twg, twu, sg, su, activation=act, out=tuple(f[0] for f in frames))
+    for name, a, w, t, f in zip(("dx", "dwg", "dwu", "dbg", "dbu"), got, want, tol, frames):
+        assert np.all(np.abs(a.to_numpy() - w) <= t + 1e-300), name
+        assert f[1](), name
+    none = tt.gated_linear_backward(put(dh), tx, twg, twu, sg, su, activation=act, bias_grad=False)
+    assert none[3] is None and none[4] is None
+    for a, b in zip(got[:3], none[:3]):
+        assert np.array_equal(a.to_numpy(), b.to_numpy())
+
+
+def gated_data(r, dtype, rows, inner, hidden):
+    n = lambda *s: r.normal(0, 1, s).astype(dtype)  # noqa: E731
+    return n(rows, inner), (n(inner, hidden) * inner ** -0.5).astype(dtype), (n(inner, hidden) * inner ** -0.5).astype(dtype), n(hidden), n(hidden), n(rows, hidden)
+
+
+SIZES = [(1, 1, 1), (1, 5, 3), (1, 64, 128), (2, 333, 70), (3, 1024, 260), (5, 48, 1000), (8, 200, 516), (9, 128, 256), (16, 96, 33), (17, 64, 64), (33, 100, 77),
+         (64, 64, 128), (65, 40, 132), (130, 260, 192), (128, 256, 1024), (300, 17, 130), (257, 512, 384)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("rows, inner, hidden", SIZES)
+def test_gated_linear(tt, dtype, act, rows, inner, hidden):
+    r = rng_of(rows, inner, hidden, act)
+    x, wg, wu, bg, bu, dh = gated_data(r, dtype, rows, inner, hidden)
+    both = (rows + hidden) % 3
+    bg, bu = (bg, bu) if both == 0 else (bg, None) if both == 1 else (None, None)
+    check_gated(tt, dtype, act, x, wg, wu, bg, bu, *(tt.Tensor.from_numpy(a) for a in (x, wg, wu)), dh=dh)
+
+
+@pytest.mark.parametrize("rows, inner, hidden", [(1024, 784, 1024), (1024, 1024, 516), (2048, 512, 1536), (512, 2048, 256), (16, 1024, 4096), (130, 4096, 512)])
+def test_gated_linear_large(tt, rows, inner, hidden):
+    r = rng_of(rows, inner, hidden)
+    x, wg, wu, bg, bu, dh = gated_data(r, np.float32, rows, inner, hidden)
+    check_gated(tt, np.float32, "silu", x, wg, wu, bg, bu, *(tt.Tensor.from_numpy(a) for a in (x, wg, wu)), dh=dh)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 4, 11, 70, 256])
+@pytest.mark.parametrize("form", ["transposed", "packed", "padded", "offset", "strided", "tied", "expanded"])
+def test_gated_linear_views(tt, dtype, rows, form):
+    inner, hidden = 96, 160
+    r = rng_of(rows, form)
+    x, wg, wu, bg, bu, dh = gated_data(r, dtype, rows, inner, hidden)
+    T = tt.Tensor
+    tx, twg, twu = (T.from_numpy(a) for a in (x, wg, wu))
+    if form == "transposed":
+        tx, twg, twu = (T.from_numpy(np.ascontiguousarray(a.T)).permute(1, 0) for a in (x, wg, wu))
+    elif form == "packed":    # gate and up side by side in one weight
+        w = T.from_numpy(np.concatenate([wg, wu], 1))
+        twg, twu = (T(w.storage, w.dtype, (inner, hidden), (2 * hidden, 1), o) for o in (0, hidden))
+    elif form == "padded":
+        def padded(a, extra):
+            t = T.from_numpy(np.concatenate([a, np.full((a.shape[0], extra), np.nan, dtype)], 1))
+            return T(t.storage, t.dtype, a.shape, (a.shape[1] + extra, 1), 0)
+        tx, twg, twu = padded(x, 4), padded(wg, 3), padded(wu, 8)
+    elif form == "offset":
+        def moved(a):
+            t = T.from_numpy(np.concatenate([np.full(3, np.nan, dtype), a.reshape(-1)]))
+            return T(t.storage, t.dtype, a.shape, (a.shape[1], 1), 3)
+        tx, twg, twu = moved(x), moved(wg), moved(wu)
+    elif form == "strided":
+        def spread(a):
+            b = np.full((a.shape[0], a.shape[1], 2), np.nan, dtype)
+            b[..., 0] = a
+            t = T.from_numpy(b)
+            return T(t.storage, t.dtype, a.shape, (2 * a.shape[1], 2), 0)
+        tx, twg, twu = spread(x), spread(wg), spread(wu)
+    elif form == "tied":      # one weight for both
+        wu, twu = wg, twg
+    else:                     # the same row for every position
+        x = np.repeat(x[:1], rows, 0)
+        tx = T(tx.storage, tx.dtype, (rows, inner), (0, 1), 0)
+    check_gated(tt, dtype, "silu", x, wg, wu, bg, None, tx, twg, twu, dh=dh)
+
+
+def test_gated_linear_shapes(tt):
+    r = rng_of(11)
+    x, wg, wu, bg, bu, _ = gated_data(r, np.float32, 24, 40, 36)
+    T = tt.Tensor.from_numpy
+    flat = tt.gated_linear(T(x), T(wg), T(wu), T(bg), T(bu)).to_numpy()
+    three = tt.gated_linear(T(x.reshape(2, 12, 40)), T(wg), T(wu), T(bg), T(bu))
+    assert three.shape == (2, 12, 36) and np.array_equal(three.to_numpy().reshape(24, 36), flat)
+    one = tt.gated_linear(T(x[0]), T(wg), T(wu), T(bg), T(bu))
+    assert one.shape == (36,)
+    g, u = gated_reference(x[:1], wg, wu, bg, bu, "silu")
+    assert np.allclose(one.to_numpy(), (act_of(g, "silu")[0] * u)[0], rtol=1e-5, atol=1e-6)
+    none = tt.gated_linear(T(x[:0]), T(wg), T(wu))
+    assert none.shape == (0, 36)
+    e = T(np.zeros((0, 36), np.float32))
+    grads = tt.gated_linear_backward(e, T(x[:0]), T(wg), T(wu), e, e)
+    assert grads[0].shape == (0, 40) and all(np.all(t.to_numpy() == 0) for t in grads[1:])
+
+
+@pytest.mark.parametrize("rows", [1, 6, 40, 200])
+def test_gated_linear_whole_numbers_and_infinities(tt, rows):
+    """relu on whole numbers is exact (no term of the sums is lost or taken twice); an infinity reaches its row alone."""
+    r = rng_of(rows, 5)
+    x, wg, wu = (r.integers(-3, 4, s).astype(np.float32) for s in ((rows, 72), (72, 132), (72, 132)))
+    dh = r.integers(-2, 3, (rows, 132)).astype(np.float32)
+    T = tt.Tensor.from_numpy
+    h, g, u = tt.gated_linear(T(x), T(wg), T(wu), activation="relu", save=True)
+    wantg, wantu = x @ wg, x @ wu
+    assert np.array_equal(g.to_numpy(), wantg) and np.array_equal(u.to_numpy(), wantu)
+    assert np.array_equal(h.to_numpy(), np.maximum(wantg, 0) * wantu)
+    got = tt.gated_linear_backward(T(dh), T(x), T(wg), T(wu), g, u, activation="relu")
+    dg, du = (dh * wantu * (wantg >= 0)).astype(np.float64), (dh * np.maximum(wantg, 0)).astype(np.float64)
+    want = (dg @ wg.T + du @ wu.T, x.T @ dg, x.T @ du, dg.sum(0), du.sum(0))
+    assert max(np.abs(w).max() for w in want) < 2 ** 24
+    for a, w in zip(got, want):
+        assert np.array_equal(a.to_numpy().astype(np.float64), w)
+    bad = x.copy()
+    bad[rows // 2, 3] = np.inf
+    h2 = tt.gated_linear(T(bad), T(wg), T(wu), activation="relu").to_numpy()
+    keep = np.arange(rows) != rows // 2
+    assert np.array_equal(h2[keep], h.to_numpy()[keep]) and not np.isfinite(h2[rows // 2]).all()
+
+
+# ---- the distillation loss -----------------------------------------------------------------------------------------------
+
+
+def distill_reference(z, ids, t_logit, temp, w):
+    """loss, gradient, and what their tolerances need, in 64 bits."""
+    z, t_logit = z.astype(np.float64), t_logit.astype(np.float64)
+    rows, cols = z.shape
+    loss, grad, rel = np.zeros(rows), np.zeros((rows, cols)), np.zeros((rows, cols))
+    lt = np.zeros(rows)
+    for r in range(rows):
+        ok = (ids[r] >= 0) & (ids[r] < cols)
+        t = np.where(ok, t_logit[r], -np.inf)
+        if w[r] == 0 or not (np.any(t > -np.inf) or np.any(np.isnan(t))):
+            continue
+        with np.errstate(invalid="ignore", divide="ignore"):
+            xt, xz = (t - t.max()) / temp, (z[r] - z[r].max()) / temp
+            p, q = np.exp(xt), np.exp(xz)
+            p, lq = p / p.sum(), xz - np.log(q.sum())
+            q = q / q.sum()
+            some = p != 0
+            terms = p[some] * (np.log(p[some]) - lq[ids[r][some]])
+            loss[r] = w[r] * temp ** 2 * terms.sum()
+            share = np.zeros(cols)
+            np.add.at(share, ids[r][ok], p[ok])
+            grad[r] = w[r] * temp * (q - share)
+            # relative errors, in u: of an exponential 4 |x| + 4 (the difference, the factor, the product; two of the
+            # function), of a sum the mean of its terms' and a rounding a level
+            eq, ep = np.where(q > 0, 4 * np.abs(xz) + 4, 0), np.where(p > 0, 4 * np.abs(np.where(np.isfinite(xt), xt, 0)) + 4, 0)
+            sq, sp = (q * eq).sum() + cols / 64 + 24, (p * ep).sum() + 28
+            share_err = np.zeros(cols)
+            np.add.at(share_err, ids[r][ok], (p * (ep + sp + 4 + len(p)))[ok])
+            rel[r] = w[r] * temp * (q * (eq + sq + 4) + share_err)
+            fin = np.isfinite(terms)
+            lt[r] = w[r] * temp ** 2 * ((np.abs(np.log(p[some]) - lq[ids[r][some]]) + 1) * p[some] * (ep[some] + sp + 4))[fin].sum() + w[r] * temp ** 2 * sq
+    return loss.sum(), grad, rel, lt.sum() + np.abs(loss[np.isfinite(loss)]).sum() * 4
+
+
+def check_distill(tt, z, ids, t_logit, temp, w, dtype, tz=None, index=np.int64):
+    u = U[dtype]
+    rows, cols = z.shape
+    weight = np.full(rows, 1 / max(rows, 1)) if w is None else w.astype(np.float64)
+    loss, grad, rel, lt = distill_reference(z, ids, t_logit, temp, weight)
+    T = tt.Tensor.from_numpy
+    out = framed(tt, (1,), dtype), framed(tt, (rows, cols), dtype)
+    args = (tz if tz is not None else T(z), T(ids.astype(index)), T(t_logit))
+    kw = dict(temperature=temp, row_weight=T(w) if w is not None else None)
+    got = tt.distill_loss(*args, out=(out[0][0], out[1][0]), **kw)
+    a, g = got[0].to_numpy()[0], got[1].to_numpy().astype(np.float64)
+    assert out[0][1]() and out[1][1]()
+    fin = np.isfinite(grad)
+    assert np.array_equal(np.isnan(g), np.isnan(grad))
+    assert np.all(np.abs(g[fin] - grad[fin]) <= u * rel[fin] + 4 * np.finfo(dtype).tiny), np.max(np.abs(g[fin] - grad[fin]) - u * rel[fin])
+    if np.isfinite(loss):
+        assert abs(a - loss) <= u * lt + u * abs(loss) + np.finfo(dtype).tiny, (a, loss, u * lt)
+    else:
+        assert (np.isnan(a) and np.isnan(loss)) or a == loss
+    again = tt.distill_loss(*args, **kw)
+    assert np.array_equal(again[0].to_numpy(), got[0].to_numpy(), equal_nan=True) and np.array_equal(again[1].to_numpy(), got[1].to_numpy(), equal_nan=True)
+    return g
+
+
+def distill_data(r, rows, cols, top, dtype):
+    z = (r.normal(0, 2, (rows, cols))).astype(dtype)
+    ids = np.stack([r.permutation(cols)[:top] if top <= cols else r.integers(0, cols, top) for _ in range(rows)]) if rows else np.zeros((0, top), np.int64)
+    return z, ids, r.normal(2, 2, (rows, top)).astype(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, cols, top", [(1, 1, 1), (3, 2, 2), (5, 3, 1), (4, 10, 4), (130, 10, 10), (7, 17, 5), (3, 64, 8), (9, 65, 33), (2, 257, 64),
+                                             (5, 1000, 100), (3, 1024, 7), (3, 1025, 64), (2, 2051, 300), (6, 4096, 64), (3, 8191, 1), (2, 8200, 1024),
+                                             (2, 16390, 16), (1, 33001, 128), (3, 65537, 70), (2, 98305, 33), (1, 131073, 64), (140, 5000, 12), (2, 200003, 9),
+                                             (300, 2000, 3), (0, 8, 2)])
+def test_distill_loss(tt, dtype, rows, cols, top):
+    r = rng_of(rows, cols, top)
+    z, ids, t = distill_data(r, rows, cols, top, dtype)
+    check_distill(tt, z, ids, t, 1.0 if cols % 2 else 2.5, None, dtype, index=np.int32 if top % 2 else np.int64)
+
+
+# sizes of every way through the operator: tiny rows, a wave, workgroups of several sizes, rows cut into parts
+MASK_SIZES = [(6, 12), (6, 300), (6, 3001), (6, 20000), (150, 9000), (130, 70001)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, cols", MASK_SIZES)
+def test_distill_masks(tt, dtype, rows, cols):
+    r = rng_of(rows, cols, 2)
+    top = 7
+    z, ids, t = distill_data(r, rows, cols, top, dtype)
+    w = r.random(rows).astype(dtype)
+    w[1] = 0
+    z[1] = np.nan                                       # weighs nothing: never looked at
+    ids[2] = [-1, cols, -5, cols + 7, 1 << 30, -(1 << 31), cols]  # no slot counts
+    t[3] = -np.inf                                      # nothing left of the teacher
+    ids[4, :3] = ids[4, 3]                              # one column several times
+    ids[0, 2], t[0, 3] = -1, -np.inf                    # padding and an impossible column among others
+    z[5] = np.finfo(dtype).min                          # the lowest value everywhere but at a few columns
+    z[5, ids[5]] = r.normal(0, 1, top)
+    z[0, 5:9] = -np.inf                                 # words the student may not say
+    ids[0, :] = np.where((ids[0] >= 5) & (ids[0] < 9), 0, ids[0])
+    g = check_distill(tt, z, ids, t, 2.0, w, dtype, index=np.int32)
+    assert np.all(g[1] == 0) and np.all(g[2] == 0) and np.all(g[3] == 0) and np.all(g[0, 5:9] == 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, cols", MASK_SIZES)
+def test_distill_infinities(tt, dtype, rows, cols):
+    r = rng_of(rows, cols, 3)
+    z, ids, t = distill_data(r, rows, cols, 4, dtype)
+    z[0] = -np.inf                                      # no column is possible: not a number, in this row alone
+    z[1, cols // 2] = np.inf
+    z[2, cols - 1] = np.nan
+    z[3, : cols - 2] = -np.inf                          # all but the last two columns impossible
+    ids[3] = cols - 1
+    g = check_distill(tt, z, ids, t, 1.0, None, dtype)
+    assert np.isnan(g[:3]).all() and np.isfinite(g[3:]).all()
+    # the teacher wants a word that the student may not say: an infinite loss, a finite gradient
+    z, ids, t = distill_data(r, rows, cols, 4, dtype)
+    z[1, ids[1, 0]] = -np.inf
+    check_distill(tt, z, ids, t, 1.0, None, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, cols", [(5, 10), (5, 1003), (4, 6001), (3, 40002)])
+def test_distill_rows_apart(tt, dtype, rows, cols):
+    """Logits that are part of a wider matrix, beginning off every boundary."""
+    r = rng_of(rows, cols, 4)
+    z, ids, t = distill_data(r, rows, cols, 5, dtype)
+    wide = np.full((rows, cols + 5), np.nan, dtype)
+    wide[:, 3:3 + cols] = z
+    whole = tt.Tensor.from_numpy(wide)
+    check_distill(tt, z, ids, t, 1.5, None, dtype, tz=tt.Tensor(whole.storage, whole.dtype, z.shape, (cols + 5, 1), 3))
+    turned = tt.Tensor.from_numpy(np.ascontiguousarray(z.T)).permute(1, 0)  # copied
+    check_distill(tt, z, ids, t, 1.5, None, dtype, tz=turned)
+
+
+# ---- gradients against differences, a whole step, graphs --------------------------------------------------------------------
+
+
+def slope_of(f, args, k, r, eps=1e-6):
+    d = r.normal(0, 1, args[k].shape)
+    up, down = list(args), list(args)
+    up[k], down[k] = args[k] + eps * d, args[k] - eps * d
+    return (f(*up) - f(*down)) / (2 * eps), d
+
+
+def student_step(tt, table, wg, wu, wo, ids, t_ids, t_logit, scale):
+    """Loss and gradients of tokens -> embedding -> gated pair -> output layer -> distillation loss; the table's gradient is
+    added onto its use as an output layer (logits over the vocabulary through a projection wo and the table)."""
+    x = tt.embedding(ids, table, scale=scale)
+    h, g, u = tt.gated_linear(x, wg, wu, activation="silu", save=True)
+    y = tt.linear(h, wo)
+    logits = tt.linear(y, table.permute(1, 0))
+    loss, dlogits = tt.distill_loss(logits, t_ids, t_logit, temperature=2.0)
+    dtable = tt.matmul(dlogits.permute(1, 0), y)                  # of the output layer, [vocab, dim]
+    dy = tt.matmul(dlogits, table)
+    dh, dwo, _ = tt.linear_backward(dy, h, wo, bias_grad=False)
+    dx, dwg, dwu, _, _ = tt.gated_linear_backward(dh, x, wg, wu, g, u, activation="silu", bias_grad=False)
+    tt.embedding_backward(dx, ids, table.size(0), scale=scale, out=dtable, accumulate=True)
+    return loss, dtable, dwg, dwu, dwo
+
+
+def student_data(r, dtype, count=60, vocab=50, dim=24, hidden=40, top=5):
+    n = lambda *s: r.normal(0, 1, s).astype(dtype)  # noqa: E731
+    return dict(table=n(vocab, dim) * dtype(0.5), wg=n(dim, hidden) * dtype(0.2), wu=n(dim, hidden) * dtype(0.2), wo=n(hidden, dim) * dtype(0.2)), \
+        dict(ids=r.integers(0, vocab, count).astype(np.int64), t_ids=np.stack([r.permutation(vocab)[:top] for _ in range(count)]).astype(np.int32), t_logit=n(count, top))
+
+
+def student_loss(table, wg, wu, wo, ids, t_ids, t_logit, scale):
+    x = table[ids] * scale
+    g, u = x @ wg, x @ wu
+    logits = (act_of(g, "silu")[0] * u) @ wo @ table.T
+    return distill_reference(logits, t_ids, t_logit, 2.0, np.full(len(ids), 1 / len(ids)))[0]
+
+
+def test_student_step_gradients(tt):
+    """The operators together, as a training step uses them: loss and all gradients against differences of the formula."""
+    r = rng_of(21)
+    weights, data = student_data(r, np.float64)
+    T = tt.Tensor.from_numpy
+    got = student_step(tt, **{k: T(v) for k, v in {**weights, **data}.items()}, scale=1.5)
+    f = lambda table, wg, wu, wo: student_loss(table, wg, wu, wo, **data, scale=1.5)  # noqa: E731
+    args = [weights[k] for k in ("table", "wg", "wu", "wo")]
+    assert abs(got[0].to_numpy()[0] - f(*args)) <= 1e-12 * abs(f(*args))
+    for k, grad in enumerate(got[1:]):
+        want, d = slope_of(f, args, k, r)
+        # central differences: eps^2 of the third derivative and 1e-16 / eps of the value
+        assert abs((grad.to_numpy() * d).sum() - want) <= 1e-7 * max(1, abs(want)), k
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+def test_gated_gradients_against_differences(tt, act):
+    r = rng_of(22)
+    x, wg, wu, bg, bu, dh = gated_data(r, np.float64, 6, 10, 14)
+
+    def f(x, wg, wu, bg, bu):
+        g, u = gated_reference(x, wg, wu, bg, bu, act)
+        return (act_of(g, act)[0] * u * dh).sum()
+
+    T = tt.Tensor.from_numpy
+    _, g, u = tt.gated_linear(T(x), T(wg), T(wu), T(bg), T(bu), activation=act, save=True)
+    got = tt.gated_linear_backward(T(dh), T(x), T(wg), T(wu), g, u, activation=act)
+    for k, grad in enumerate(got):
+        want, d = slope_of(f, [x, wg, wu, bg, bu], k, r)
+        assert abs((grad.to_numpy() * d).sum() - want) <= 1e-7 * max(1, abs(want)), k
+
+
+def test_student_step_as_a_graph(tt):
+    """The whole step captured once and replayed on fresh inputs, with eager work in between: the same bits as eager runs.
+    A second graph of the same step, replayed in turn, has workspaces of its own."""
+    r = rng_of(23)
+    weights, data = student_data(r, np.float32, count=300, vocab=700, dim=64, hidden=96, top=9)
+    T = tt.Tensor.from_numpy
+    be = tt.get_backend(tt.kAMD)
+    fixed = {k: T(v) for k, v in weights.items()}
+    streams = [tt.graph.Stream(), tt.graph.Stream(non_blocking=True)]
+    graphs, inputs = [], []
+    try:
+        for s in streams:
+            inp = {k: T(v) for k, v in data.items()}
+            be.synchronize(0)
+            inputs.append(inp)
+            graphs.append(tt.graph.Graph(s, lambda inp=inp: student_step(tt, **fixed, **inp, scale=1.25)))
+        for replay in range(3):
+            fresh = [student_data(rng_of(40 + replay, j), np.float32, count=300, vocab=700, dim=64, hidden=96, top=9)[1] for j in range(2)]
+            for inp, new, g in zip(inputs, fresh, graphs):
+                for k, v in new.items():
+                    g.copy_in(inp[k], v)
+            be.synchronize(0)
+            for g in graphs:
+                g.launch()      # both in flight together
+            for s in streams:
+                s.synchronize()
+            for new, g in zip(fresh, graphs):
+                got = [t.to_numpy() for t in g.outputs]
+                eager = [t.to_numpy() for t in student_step(tt, **fixed, **{k: T(v) for k, v in new.items()}, scale=1.25)]
+                for a, b in zip(got, eager):
+                    assert np.array_equal(a, b)
+            be.synchronize(0)
+    finally:
+        for g in graphs:
+            g.close()
+        for s in streams:
+            s.close()
+
+
+def test_on_another_stream(tt):
+    """The operators follow on_stream(): enqueued there, in order with what the stream did before."""
+    r = rng_of(24)
+    weights, data = student_data(r, np.float32)
+    T = tt.Tensor.from_numpy
+    dev = {k: T(v) for k, v in {**weights, **data}.items()}
+    want = [t.to_numpy() for t in student_step(tt, **dev, scale=1.0)]
+    stream = tt.graph.Stream(non_blocking=True)
+    try:
+        tt.get_backend(tt.kAMD).synchronize(0)
+        got = stream.run(lambda: student_step(tt, **dev, scale=1.0))
+        stream.synchronize()
+        for a, b in zip(want, got):
+            assert np.array_equal(a, b.to_numpy())
+        del got
+    finally:
+        stream.close()

@@ -16,7 +16,12 @@ BOOL, U8, I16, I32, I64, F32, F64 = range(7)
 BIN = {"add": 0, "sub": 1, "mul": 2, "div": 3, "pow": 4, "maximum": 5, "minimum": 6, "lt": 7, "le": 8, "gt": 9, "ge": 10,
        "eq": 11, "ne": 12}
 POOL = {"max": 0, "min": 1, "avg": 2}
+ACT = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 UN = {"relu": 0, "negate": 1, "abs": 2, "sqrt": 3, "exp": 4, "log": 5, "sigmoid": 6, "tanh": 7}
+
+
+class View2(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("offset", C.c_int64), ("stride", C.c_int64 * 2)]
 
 
 class View3(C.Structure):
@@ -70,6 +75,14 @@ def _bind(lib: C.CDLL) -> None:
         "ttamd_random_fill": (i, [i, i, i, C.c_double, C.c_double, C.POINTER(C.c_uint64), C.c_int64, vp, vp]),
         "ttamd_mse_loss": (i, [i, i, C.c_int64, C.c_int64, vp, vp, vp, vp, vp, vp]),
         "ttamd_linear_mse_head": (i, [i, i, C.c_int64, C.c_int64, C.c_int64, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+        "ttamd_embedding_forward": (i, [i, i, i] + [C.c_int64] * 3 + [vp, vp, C.c_int64, C.c_int64, C.c_double, vp, vp]),
+        "ttamd_embedding_backward_workspace": (i, [i] + [C.c_int64] * 3 + [C.POINTER(sz)]),
+        "ttamd_embedding_backward": (i, [i, i, i] + [C.c_int64] * 3 + [vp, vp, C.c_double, i, vp, vp, sz, vp]),
+        "ttamd_gated_linear_workspace": (i, [i] + [C.c_int64] * 3 + [i, C.POINTER(sz)]),
+        "ttamd_gated_linear_forward": (i, [i, i, i] + [C.c_int64] * 3 + [C.POINTER(View2)] * 3 + [vp] * 6 + [sz, vp]),
+        "ttamd_gated_linear_backward": (i, [i, i, i] + [C.c_int64] * 3 + [vp] + [C.POINTER(View2)] * 3 + [vp] * 8 + [sz, vp]),
+        "ttamd_distill_loss_workspace": (i, [i] + [C.c_int64] * 3 + [C.POINTER(sz)]),
+        "ttamd_distill_loss": (i, [i, i, i] + [C.c_int64] * 3 + [vp, C.c_int64, vp, vp, vp, C.c_double, vp, vp, vp, sz, vp]),
         "ttamd_random_fill_view": (i, [i, i, i, C.c_double, C.c_double, C.POINTER(C.c_uint64), i, C.POINTER(C.c_int64),
                                        C.POINTER(C.c_int64), vp, C.c_int64, vp]),
         "ttamd_random_fill_states": (i, [i, i, i, C.c_double, C.c_double, C.POINTER(C.c_uint64), i, C.POINTER(C.c_int64),

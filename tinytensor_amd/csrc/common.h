@@ -34,6 +34,13 @@ inline size_t dtype_size(ttamd_dtype dt) {
     return 0;
 }
 
+inline bool misaligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
+// Whether two byte ranges share a byte.
+inline bool overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a_bytes > 0 && b_bytes > 0 && x < y + b_bytes && y < x + a_bytes;
+}
+
 #define TTAMD_HIP_CHECK(expr)                                                                  \
     do {                                                                                       \
         hipError_t e_ = (expr);                                                                \

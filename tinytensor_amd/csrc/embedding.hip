@@ -1,0 +1,487 @@
+// embedding.hip — rows of a table looked up by token, scaled, and the table's gradient (gfx950).
+//
+//   out[i] = scale * table[index[i]]            (an index outside the table: a row of zeros)
+//   dtable[v] = scale * sum of dy[i] over the positions i with index[i] = v, in the order of the positions
+// No counterpart in the reference; the layer stands in front of nn::Linear (nn/linear.cpp:42-50).
+//
+// Bound: HBM in both directions.  The gradient of a token is a sum over positions that lie anywhere, so the positions are
+// first put in the order of their tokens (embedding_order_kernel), then every run of equal tokens is added up
+// (embedding_sum_kernel, embedding_join_kernel): each row of dy is read once, each row of the gradient written once, and
+// the order of every sum is fixed by the indices alone -- no atomics on floating point values.
+#include "common.h"
+
+namespace ttamd {
+namespace {
+
+template <typename T>
+struct Row;
+template <>
+struct Row<float> {
+    static constexpr int W = 4;
+    typedef float vec_t __attribute__((ext_vector_type(4), aligned(4)));  // (rows of any length: see misaligned rows below)
+};
+template <>
+struct Row<double> {
+    static constexpr int W = 2;
+    typedef double vec_t __attribute__((ext_vector_type(2), aligned(8)));
+};
+
+template <bool I64>
+__device__ __forceinline__ int64_t load_index(const void *index, int64_t i) {
+    if constexpr (I64) return static_cast<const int64_t *>(index)[i];
+    else return static_cast<const int32_t *>(index)[i];
+}
+
+// ---- forward ----------------------------------------------------------------------------------------------------------
+// 2^lanes_log lanes own a row and walk it in vectors.  A row whose length is no multiple of the vector ends in a vector
+// that is moved back to end with the row: its first elements are written twice, with the same values.  VEC = false: one
+// element at a time, for tables whose columns are not neighbours (a transposed view) and rows shorter than a vector.
+template <typename T, bool I64, bool VEC>
+__global__ void __launch_bounds__(256) embedding_forward_kernel(const T *__restrict__ table, int64_t row_stride, int64_t col_stride,
+                                                                const void *__restrict__ index, int64_t count, int64_t vocab, int64_t dim,
+                                                                T scale, T *__restrict__ out, int lanes_log) {
+    constexpr int W = VEC ? Row<T>::W : 1;
+    using V = typename Row<T>::vec_t;
+    const int lanes = 1 << lanes_log;
+    const int64_t step = (static_cast<int64_t>(gridDim.x) * 256) >> lanes_log;
+    const int lane = threadIdx.x & (lanes - 1);
+    const int64_t nvec = (dim + W - 1) / W;
+    for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> lanes_log; i < count; i += step) {
+        const int64_t v = load_index<I64>(index, i);
+        const bool ok = v >= 0 && v < vocab;
+        const T *src = table + (ok ? v : 0) * row_stride;
+        T *dst = out + i * dim;
+#pragma unroll 4
+        for (int64_t u = lane; u < nvec; u += lanes) {
+            if constexpr (VEC) {
+                const int64_t at = u * W + W <= dim ? u * W : dim - W;
+                V x = {};
+                if (ok) x = *reinterpret_cast<const V *>(src + at) * scale;
+                *reinterpret_cast<V *>(dst + at) = x;
+            } else {
+                dst[u] = ok ? src[u * col_stride] * scale : T(0);
+            }
+        }
+    }
+}
+
+// ---- gradient: the order of the positions ------------------------------------------------------------------------------
+// Workgroup b owns the tokens v with v % buckets == b (neighbouring tokens, often equally frequent, go to different
+// workgroups) and finds its positions by reading every index: count * 4 or 8 bytes out of L2 a workgroup, which for all
+// but the shortest rows is less than the time the rows themselves take, and spares the passes of a sort over the device.
+// A stable counting sort: wave w counts the tokens in the w-th sixteenth of the positions (the count of a (token, wave)
+// pair does not depend on the order of the additions), the counts are summed up in (token, wave) order, and the waves
+// walk their positions again and hand out the places.  What lies in lower buckets is counted on the same walk, so the
+// workgroups' places need no second kernel either.
+// The order is by (bucket, token); all that the sums need is that equal tokens lie together.
+constexpr int kOrderWaves = 16;
+constexpr int kOrderThreads = 64 * kOrderWaves;
+constexpr int kOrderTokens = 512;  // tokens of a bucket at most: their (token, wave) counters fill 32 KB of LDS
+
+struct OrderArgs {
+    const void *index;
+    int64_t count, vocab, dim;
+    int bucket_log;   // log2 of the number of buckets
+    int tokens;       // tokens a bucket has room for: ceil(vocab / buckets)
+    int32_t *position, *token;  // [count] in the order of the tokens
+    int32_t *total;   // positions whose index lies in the table
+    void *grad;       // rows of tokens that no position has are set to zero here, or null: left alone
+};
+
+template <typename T, bool I64>
+__global__ void __launch_bounds__(kOrderThreads) embedding_order_kernel(OrderArgs a) {
+    extern __shared__ int32_t counters[];  // [tokens][kOrderWaves]
+    __shared__ int32_t wave_sum[kOrderWaves], below_sum[kOrderWaves];
+    const int tid = threadIdx.x, lane = tid % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int buckets = 1 << a.bucket_log, mine = blockIdx.x;
+    const int cells = a.tokens * kOrderWaves;
+    for (int i = tid; i < cells; i += kOrderThreads) counters[i] = 0;
+    __syncthreads();
+    const int64_t per = (a.count + kOrderWaves - 1) / kOrderWaves;
+    const int64_t first = wave * per, last = first + per < a.count ? first + per : a.count;
+    int below = 0;
+    for (int64_t i = first + lane; i < last; i += 64) {
+        const int64_t v = load_index<I64>(a.index, i);
+        if (v < 0 || v >= a.vocab) continue;
+        const int b = static_cast<int>(v & (buckets - 1));
+        below += b < mine;
+        if (b == mine) atomicAdd(&counters[static_cast<int>(v >> a.bucket_log) * kOrderWaves + wave], 1);
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) below += __shfl_xor(below, d, 64);
+    if (lane == 0) below_sum[wave] = below;
+    __syncthreads();
+    // exclusive sums over the cells: a thread adds up its share of neighbouring cells, the threads' totals are added in order
+    const int share = (cells + kOrderThreads - 1) / kOrderThreads;
+    const int c0 = tid * share, c1 = c0 + share < cells ? c0 + share : cells;
+    int own = 0;
+    for (int i = c0; i < c1; ++i) own += counters[i];
+    int run = own;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(run, d, 64);
+        if (lane >= d) run += o;
+    }
+    if (lane == 63) wave_sum[wave] = run;
+    __syncthreads();
+    int base = 0, in_bucket = 0;
+#pragma unroll
+    for (int w = 0; w < kOrderWaves; ++w) {
+        base += below_sum[w];
+        in_bucket += wave_sum[w];
+    }
+    if (mine == buckets - 1 && tid == 0) *a.total = base + in_bucket;
+    int at = base + run - own;
+    for (int w = 0; w < wave; ++w) at += wave_sum[w];
+    for (int i = c0; i < c1; ++i) {
+        const int n = counters[i];
+        counters[i] = at;
+        at += n;
+    }
+    __syncthreads();
+    // Rows of tokens that nothing has: a token's run is empty when its first cell and the next token's begin at one place.
+    if (a.grad) {
+        const int end = base + in_bucket;
+        for (int t = wave; t < a.tokens; t += kOrderWaves) {
+            const int64_t v = (static_cast<int64_t>(t) << a.bucket_log) + mine;
+            if (v >= a.vocab) break;
+            const int next = t + 1 < a.tokens ? counters[(t + 1) * kOrderWaves] : end;
+            if (counters[t * kOrderWaves] != next) continue;
+            T *row = static_cast<T *>(a.grad) + v * a.dim;
+            for (int64_t d = lane; d < a.dim; d += 64) row[d] = T(0);
+        }
+    }
+    __syncthreads();  // the cells are moved on from here
+    for (int64_t i0 = first; i0 < last; i0 += 64) {
+        const int64_t i = i0 + lane;
+        const int64_t v = i < last ? load_index<I64>(a.index, i) : -1;
+        const bool in = v >= 0 && v < a.vocab && static_cast<int>(v & (buckets - 1)) == mine;
+        const int t = static_cast<int>(v >> a.bucket_log);
+        uint64_t left = __ballot(in);
+        while (left) {  // a round for each different token among the 64 positions
+            const int lead = __builtin_ctzll(left);
+            const int which = __builtin_amdgcn_readlane(t, lead);
+            const uint64_t same = __ballot(in && t == which);
+            const int cell = which * kOrderWaves + wave;
+            const int place = counters[cell];
+            if (in && t == which) {
+                const int p = place + __popcll(same & ((1ull << lane) - 1));
+                a.position[p] = static_cast<int32_t>(i);
+                a.token[p] = static_cast<int32_t>(v);
+            }
+            if (lane == lead) counters[cell] = place + __popcll(same);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the other lanes read the cell in a later round
+            left &= ~same;
+        }
+    }
+}
+
+// ---- gradient: the sums ------------------------------------------------------------------------------------------------
+// A wave adds up the rows of kRun ordered positions, 64 vectors of columns wide.  A run of equal tokens that lies inside
+// goes to the gradient; the part of one that began before is left in partial[2 c], of one that goes on in
+// partial[2 c + 1].  Sums are held in 64 bits: the conversions cost nothing beside the loads, and a frequent token's sum
+// over tens of thousands of rows keeps its last bits.
+constexpr int kRun = 16;
+constexpr int kJoinWaves = 4;
+
+template <typename T>
+struct SumArgs {
+    const T *dy;
+    T *grad;
+    double *partial;  // [2 * chunks][dim]
+    const int32_t *position, *token, *total;
+    int64_t dim;
+    double scale;
+    int accumulate;
+};
+
+template <typename T, int W>
+__device__ __forceinline__ void write_gradient(const SumArgs<T> &a, int64_t token, int64_t col, const double (&sum)[W]) {
+    T *g = a.grad + token * a.dim + col;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+        const double v = sum[k] * a.scale;
+        g[k] = a.accumulate ? static_cast<T>(static_cast<double>(g[k]) + v) : static_cast<T>(v);
+    }
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void write_partial(const SumArgs<T> &a, int64_t part, int64_t col, const double (&sum)[W]) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) a.partial[part * a.dim + col + k] = sum[k];
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void load_row(const T *p, T (&x)[W]) {
+    if constexpr (W == 1) {
+        x[0] = *p;
+    } else {
+        const typename Row<T>::vec_t v = *reinterpret_cast<const typename Row<T>::vec_t *>(p);
+#pragma unroll
+        for (int k = 0; k < W; ++k) x[k] = v[k];
+    }
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(64) embedding_sum_kernel(SumArgs<T> a) {
+    const int total = *a.total;
+    const int64_t c = blockIdx.x;
+    const int64_t s0 = c * kRun;
+    if (s0 >= total) return;
+    const int n = total - s0 < kRun ? static_cast<int>(total - s0) : kRun;
+    const int lane = threadIdx.x;
+    // (lanes beyond the row's end stay and work on its first columns: every lane's position is read by the others)
+    const bool live = (static_cast<int64_t>(blockIdx.y) * 64 + lane) * W < a.dim;
+    const int64_t col = live ? (static_cast<int64_t>(blockIdx.y) * 64 + lane) * W : 0;
+    // lane l knows the l-th position and token; lanes n and beyond repeat the last one
+    const int mine = lane < n ? lane : n - 1;
+    const int position = a.position[s0 + mine], token = a.token[s0 + mine];
+    const int before = c > 0 ? a.token[s0 - 1] : -1;
+    const int after = s0 + n < total ? a.token[s0 + n] : -1;
+    T x[kRun][W];
+#pragma unroll
+    for (int i = 0; i < kRun; ++i)
+        load_row<T, W>(a.dy + static_cast<int64_t>(__builtin_amdgcn_readlane(position, i)) * a.dim + col, x[i]);
+    double sum[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) sum[k] = 0;
+    int cur = __builtin_amdgcn_readfirstlane(token);
+    bool head = before == cur;
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        if (i < n) {
+            const int t = __builtin_amdgcn_readlane(token, i);
+            if (t != cur) {
+                if (live) {
+                    if (head) write_partial<T, W>(a, 2 * c, col, sum);
+                    else write_gradient<T, W>(a, cur, col, sum);
+                }
+                head = false;
+                cur = t;
+#pragma unroll
+                for (int k = 0; k < W; ++k) sum[k] = 0;
+            }
+#pragma unroll
+            for (int k = 0; k < W; ++k) sum[k] += static_cast<double>(x[i][k]);
+        }
+    }
+    if (!live) return;
+    if (head || after == cur) write_partial<T, W>(a, 2 * c + (head ? 0 : 1), col, sum);
+    else write_gradient<T, W>(a, cur, col, sum);
+}
+
+// The run that begins in chunk c and goes on: its parts are partial[2 c + 1] and partial[2 j] of the following chunks j
+// that begin with its token.  Each wave adds a contiguous share of them, the waves' sums are added in order.
+template <typename T, int W>
+__global__ void __launch_bounds__(64 * kJoinWaves) embedding_join_kernel(SumArgs<T> a) {
+    const int total = *a.total;
+    const int64_t c = blockIdx.x;
+    const int64_t next = (c + 1) * kRun;
+    if (next >= total) return;
+    const int token = a.token[next - 1];
+    if (a.token[next] != token) return;                            // no run crosses this border
+    if (c > 0 && a.token[c * kRun - 1] == token) return;           // it began in an earlier chunk
+    // the following chunks that begin with the token: a block of neighbours, found by doubling and halving
+    const int64_t chunks = (total + kRun - 1) / kRun;
+    int64_t lo = c + 1, hi = c + 2;                                // chunk lo begins with it
+    while (hi < chunks && a.token[hi * kRun] == token) {
+        lo = hi;
+        hi = c + 2 * (hi - c);
+    }
+    if (hi > chunks) hi = chunks;
+    while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) / 2;
+        if (a.token[mid * kRun] == token) lo = mid;
+        else hi = mid;
+    }
+    const int64_t parts = lo - c + 1;                              // chunks c .. lo
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int64_t col = (static_cast<int64_t>(blockIdx.y) * 64 + lane) * W;
+    __shared__ double waves[kJoinWaves][64 * W];
+    const int64_t per = (parts + kJoinWaves - 1) / kJoinWaves;
+    const int64_t p0 = wave * per, p1 = p0 + per < parts ? p0 + per : parts;
+    double sum[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) sum[k] = 0;
+    if (col < a.dim) {
+#pragma unroll 8
+        for (int64_t p = p0; p < p1; ++p) {
+            const double *src = a.partial + (p == 0 ? 2 * c + 1 : 2 * (c + p)) * a.dim + col;
+#pragma unroll
+            for (int k = 0; k < W; ++k) sum[k] += src[k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < W; ++k) waves[wave][lane * W + k] = sum[k];
+    __syncthreads();
+    if (wave == 0 && col < a.dim) {
+#pragma unroll
+        for (int w = 1; w < kJoinWaves; ++w)
+#pragma unroll
+            for (int k = 0; k < W; ++k) sum[k] += waves[w][lane * W + k];
+        write_gradient<T, W>(a, token, col, sum);
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------
+struct BackwardPlan {
+    int bucket_log, tokens;
+    int64_t chunks;
+    size_t position, token, total, partial, bytes;  // byte offsets into the workspace
+};
+
+BackwardPlan plan_backward(int64_t count, int64_t vocab, int64_t dim) {
+    BackwardPlan p{};
+    // 256 buckets, a workgroup for each CU; more where a bucket's tokens would not fit the counters, fewer for tiny tables
+    p.bucket_log = 8;
+    while (p.bucket_log > 0 && (int64_t(1) << (p.bucket_log - 1)) >= vocab) --p.bucket_log;
+    while ((vocab + (int64_t(1) << p.bucket_log) - 1) >> p.bucket_log > kOrderTokens) ++p.bucket_log;
+    p.tokens = static_cast<int>((vocab + (int64_t(1) << p.bucket_log) - 1) >> p.bucket_log);
+    p.chunks = (count + kRun - 1) / kRun;
+    const auto up = [](size_t b) { return (b + 255) / 256 * 256; };
+    p.position = 0;
+    p.token = p.position + up(static_cast<size_t>(count) * 4);
+    p.total = p.token + up(static_cast<size_t>(count) * 4);
+    p.partial = p.total + 256;
+    p.bytes = p.partial + static_cast<size_t>(2 * p.chunks) * static_cast<size_t>(dim) * sizeof(double);
+    return p;
+}
+
+template <typename T>
+ttamd_status launch_forward(int64_t count, int64_t vocab, int64_t dim, const void *index, bool index64, const void *table,
+                            int64_t row_stride, int64_t col_stride, double scale, void *out, hipStream_t st) {
+    const bool vec = col_stride == 1 && dim >= Row<T>::W;
+    const int64_t nvec = vec ? (dim + Row<T>::W - 1) / Row<T>::W : dim;
+    int lanes_log = 0;
+    while (lanes_log < 6 && (int64_t(1) << lanes_log) < nvec) ++lanes_log;
+    const int64_t blocks = ((count << lanes_log) + 255) / 256;
+    const dim3 grid(static_cast<unsigned>(blocks < (1 << 22) ? blocks : (1 << 22)));
+    const auto run = [&](auto kernel) {
+        kernel<<<grid, 256, 0, st>>>(static_cast<const T *>(table), row_stride, col_stride, index, count, vocab, dim, static_cast<T>(scale),
+                                     static_cast<T *>(out), lanes_log);
+    };
+    if (vec) index64 ? run(embedding_forward_kernel<T, true, true>) : run(embedding_forward_kernel<T, false, true>);
+    else index64 ? run(embedding_forward_kernel<T, true, false>) : run(embedding_forward_kernel<T, false, false>);
+    TTAMD_HIP_CHECK(hipGetLastError());
+    return TTAMD_OK;
+}
+
+template <typename T>
+ttamd_status launch_backward(int64_t count, int64_t vocab, int64_t dim, const void *grad_out, const void *index, bool index64, double scale,
+                             int accumulate, void *grad, void *workspace, hipStream_t st) {
+    const BackwardPlan p = plan_backward(count, vocab, dim);
+    char *ws = static_cast<char *>(workspace);
+    OrderArgs o{index, count, vocab, dim, p.bucket_log, p.tokens, reinterpret_cast<int32_t *>(ws + p.position),
+                reinterpret_cast<int32_t *>(ws + p.token), reinterpret_cast<int32_t *>(ws + p.total), accumulate ? nullptr : grad};
+    const size_t lds = static_cast<size_t>(p.tokens) * kOrderWaves * sizeof(int32_t);
+    if (index64) embedding_order_kernel<T, true><<<1u << p.bucket_log, kOrderThreads, lds, st>>>(o);
+    else embedding_order_kernel<T, false><<<1u << p.bucket_log, kOrderThreads, lds, st>>>(o);
+    TTAMD_HIP_CHECK(hipGetLastError());
+    if (count == 0) return TTAMD_OK;
+    const SumArgs<T> a{static_cast<const T *>(grad_out), static_cast<T *>(grad), reinterpret_cast<double *>(ws + p.partial), o.position,
+                       o.token, o.total, dim, scale, accumulate};
+    const bool vec = dim % Row<T>::W == 0;
+    const int w = vec ? Row<T>::W : 1;
+    const dim3 grid(static_cast<unsigned>(p.chunks), static_cast<unsigned>((dim + 64 * w - 1) / (64 * w)));
+    if (vec) embedding_sum_kernel<T, Row<T>::W><<<grid, 64, 0, st>>>(a);
+    else embedding_sum_kernel<T, 1><<<grid, 64, 0, st>>>(a);
+    TTAMD_HIP_CHECK(hipGetLastError());
+    if (vec) embedding_join_kernel<T, Row<T>::W><<<grid, 64 * kJoinWaves, 0, st>>>(a);
+    else embedding_join_kernel<T, 1><<<grid, 64 * kJoinWaves, 0, st>>>(a);
+    TTAMD_HIP_CHECK(hipGetLastError());
+    return TTAMD_OK;
+}
+
+ttamd_status check_shape(const char *what, ttamd_dtype dtype, int64_t count, int64_t vocab, int64_t dim) {
+    if (dtype != TTAMD_F32 && dtype != TTAMD_F64) {
+        set_error("%s: floating point dtypes only", what);
+        return TTAMD_ERR_UNSUPPORTED_DTYPE;
+    }
+    // (the column slabs of a row are a grid's second dimension: dim / 64 below 2^16)
+    if (count < 0 || vocab < 1 || dim < 1 || count > 0x7fffffffLL || vocab > (int64_t(1) << 28) || dim > (1 << 21)) {
+        set_error("%s: count %lld, vocab %lld, dim %lld: fewer than 2^31 indices, 1 to 2^28 rows of 1 to 2^21 elements", what,
+                  static_cast<long long>(count), static_cast<long long>(vocab), static_cast<long long>(dim));
+        return TTAMD_ERR_INVALID_ARGUMENT;
+    }
+    return TTAMD_OK;
+}
+
+ttamd_status check_index_dtype(const char *what, ttamd_dtype index_dtype) {
+    if (index_dtype == TTAMD_I32 || index_dtype == TTAMD_I64) return TTAMD_OK;
+    set_error("%s: indices are i32 or i64 (dtype code %d)", what, static_cast<int>(index_dtype));
+    return TTAMD_ERR_UNSUPPORTED_DTYPE;
+}
+
+}  // namespace
+}  // namespace ttamd
+
+using namespace ttamd;
+
+extern "C" {
+
+ttamd_status ttamd_embedding_forward(int device, ttamd_dtype dtype, ttamd_dtype index_dtype, int64_t count, int64_t vocab, int64_t dim,
+                                     const void *index, const void *table, int64_t row_stride, int64_t col_stride, double scale, void *out,
+                                     void *stream) {
+    const char *const what = "embedding";
+    if (ttamd_status s = check_shape(what, dtype, count, vocab, dim)) return s;
+    if (ttamd_status s = check_index_dtype(what, index_dtype)) return s;
+    if (row_stride < 0 || col_stride < 0 || row_stride > (int64_t(1) << 32) || col_stride > (int64_t(1) << 32)) {
+        set_error("%s: strides %lld, %lld of the table: 0 to 2^32", what, static_cast<long long>(row_stride), static_cast<long long>(col_stride));
+        return TTAMD_ERR_INVALID_ARGUMENT;
+    }
+    const size_t e = dtype_size(dtype);
+    if (count > 0 && (!index || !table || !out)) {
+        set_error("%s: NULL data pointer", what);
+        return TTAMD_ERR_INVALID_ARGUMENT;
+    }
+    if (misaligned(table, e) || misaligned(out, e) || misaligned(index, dtype_size(index_dtype))) {
+        set_error("%s: pointers must be aligned to the element size", what);
+        return TTAMD_ERR_INVALID_ARGUMENT;
+    }
+    if (ttamd_status s = use_device(device)) return s;
+    if (count == 0) return TTAMD_OK;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool i64 = index_dtype == TTAMD_I64;
+    if (dtype == TTAMD_F32) return launch_forward<float>(count, vocab, dim, index, i64, table, row_stride, col_stride, scale, out, st);
+    return launch_forward<double>(count, vocab, dim, index, i64, table, row_stride, col_stride, scale, out, st);
+}
+
+ttamd_status ttamd_embedding_backward_workspace(ttamd_dtype dtype, int64_t count, int64_t vocab, int64_t dim, size_t *bytes) {
+    if (ttamd_status s = check_shape("embedding_backward", dtype, count, vocab, dim)) return s;
+    if (!bytes) {
+        set_error("embedding_backward: bytes is NULL");
+        return TTAMD_ERR_INVALID_ARGUMENT;
+    }
+    *bytes = plan_backward(count, vocab, dim).bytes;
+    return TTAMD_OK;
+}
+
+ttamd_status ttamd_embedding_backward(int device, ttamd_dtype dtype, ttamd_dtype index_dtype, int64_t count, int64_t vocab, int64_t dim,
+                                      const void *grad_out, const void *index, double scale, int accumulate, void *grad_table,
+                                      void *workspace, size_t workspace_bytes, void *stream) {
+    const char *const what = "embedding_backward";
+    size_t need = 0;
+    if (ttamd_status s = ttamd_embedding_backward_workspace(dtype, count, vocab, dim, &need)) return s;
+    if (ttamd_status s = check_index_dtype(what, index_dtype)) return s;
+    const size_t e = dtype_size(dtype);
+    if (!grad_table || !workspace || (count > 0 && (!index || !grad_out))) {
+        set_error("%s: NULL data pointer", what);
+        return TTAMD_ERR_INVALID_ARGUMENT;
+    }
+    if (misaligned(grad_out, e) || misaligned(grad_table, e) || misaligned(index, dtype_size(index_dtype)) || misaligned(workspace, sizeof(double))) {
+        set_error("%s: pointers must be aligned to the element size, the workspace to 8 bytes", what);
+        return TTAMD_ERR_INVALID_ARGUMENT;
+    }
+    if (workspace_bytes < need) {
+        set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
+        return TTAMD_ERR_INVALID_ARGUMENT;
+    }
+    if (ttamd_status s = use_device(device)) return s;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool i64 = index_dtype == TTAMD_I64;
+    if (dtype == TTAMD_F32) return launch_backward<float>(count, vocab, dim, grad_out, index, i64, scale, accumulate, grad_table, workspace, st);
+    return launch_backward<double>(count, vocab, dim, grad_out, index, i64, scale, accumulate, grad_table, workspace, st);
+}
+
+}  // extern "C"

@@ -276,6 +276,14 @@ class Tensor:
         get_backend(self.device).random_fill_(self, 1, mu, std, gen)
         return self
 
+    def view2(self) -> _capi.View2:
+        v = _capi.View2()
+        v.data = self.storage.ptr
+        v.offset = self.offset
+        for i in range(2):
+            v.stride[i] = self.stride[i]
+        return v
+
     def view3(self) -> _capi.View3:
         v = _capi.View3()
         v.data = self.storage.ptr
@@ -955,6 +963,168 @@ def linear_mse_head(input: Tensor, weight: Tensor, bias: Tensor | None, target: 
     _check(lib.ttamd_linear_mse_head(input.device.id, input.dtype, rows, fin, fout, ptr(input), ptr(weight), ptr(bias), ptr(target),
                                      ptr(relu_input), ptr(y), ptr(loss), ptr(dy), ptr(dx), ptr(dW), ptr(db), _stream_arg()))
     return y, loss, dx, dW, db
+
+
+# ---- operators of a language-model student (include/ttamd.h): an embedding, a gated block, a distillation loss -------------
+_FLOATS = (_capi.F32, _capi.F64)
+
+
+def _ptr(t: Tensor | None):
+    return C.c_void_p(t.storage.ptr + t.offset * t.itemsize) if t is not None else None
+
+
+def _result(out: Tensor | None, shape, dtype: int, device: Device, what: str) -> Tensor:
+    """A new dense tensor, or the caller's `out` after a look at it."""
+    shape = tuple(shape)
+    if out is None:
+        return Tensor.empty(shape, dtype, device)
+    dense = all(n == 1 or st == d for n, st, d in zip(out.shape, out.stride, _dense_strides(out.shape)))
+    if out.shape != shape or out.dtype != dtype or out.device != device or not dense:
+        raise TTException(f"{what}: the result's tensor must be dense, {shape}, of the operands' dtype and device")
+    return out
+
+
+def _workspace(query, *args, device: Device) -> _Storage:
+    n = C.c_size_t()
+    _check(query(*args, C.byref(n)))
+    return _Storage(max(n.value, 1), device)
+
+
+def _check_operands(what: str, first: Tensor, *others: Tensor | None) -> None:
+    if first.dtype not in _FLOATS or any(t is not None and t.dtype != first.dtype for t in others):
+        raise TTException(f"{what}: operands of one floating point dtype")
+    if any(t is not None and t.device != first.device for t in others):
+        raise TTException(f"{what}: operands on one device")
+
+
+def _check_indices(what: str, indices: Tensor, device: Device) -> Tensor:
+    if indices.dtype in _FLOATS or indices.dtype == _capi.BOOL:
+        raise TTException(f"{what}: indices are integers")
+    if indices.device != device:
+        raise TTException(f"{what}: operands on one device")
+    return (indices if indices.dtype in (_capi.I32, _capi.I64) else indices.to(_capi.I32)).contiguous()
+
+
+def embedding(indices: Tensor, table: Tensor, scale: float = 1.0, out: Tensor | None = None) -> Tensor:
+    """Rows of `table` [vocab, dim] by token, scaled: out[..., :] = scale * table[indices[...], :] (ttamd_embedding_forward).
+    `table` may be any view (a transposed Linear weight: tied embeddings) and is read in place; integer indices of any
+    shape.  An index outside the table gives zeros (padding)."""
+    if table.dim() != 2:
+        raise TTException("embedding: the table must be 2-D")
+    _check_operands("embedding", table)
+    idx = _check_indices("embedding", indices, table.device)
+    vocab, dim = table.shape
+    out = _result(out, indices.shape + (dim,), table.dtype, table.device, "embedding")
+    _check(lib.ttamd_embedding_forward(table.device.id, table.dtype, idx.dtype, idx.numel(), vocab, dim, _ptr(idx), _ptr(table),
+                                       table.stride[0], table.stride[1], scale, _ptr(out), _stream_arg()))
+    return out
+
+
+def embedding_backward(grad_output: Tensor, indices: Tensor, vocab: int, scale: float = 1.0, out: Tensor | None = None,
+                       accumulate: bool = False) -> Tensor:
+    """Gradient of embedding() with respect to its table: [vocab, dim], scale * the sum of grad_output's rows of each token
+    (ttamd_embedding_backward).  accumulate: added to `out` (tied weights: onto the output layer's gradient)."""
+    if grad_output.dim() < 1 or grad_output.shape[:-1] != indices.shape:
+        raise TTException(f"embedding_backward: a gradient of {grad_output.shape} for indices of {indices.shape}")
+    if accumulate and out is None:
+        raise TTException("embedding_backward: accumulate needs the tensor to add to")
+    _check_operands("embedding_backward", grad_output)
+    idx = _check_indices("embedding_backward", indices, grad_output.device)
+    dy = grad_output.contiguous()
+    dim = grad_output.shape[-1]
+    out = _result(out, (vocab, dim), dy.dtype, dy.device, "embedding_backward")
+    ws = _workspace(lib.ttamd_embedding_backward_workspace, dy.dtype, idx.numel(), vocab, dim, device=dy.device)
+    _check(lib.ttamd_embedding_backward(dy.device.id, dy.dtype, idx.dtype, idx.numel(), vocab, dim, _ptr(dy), _ptr(idx), scale,
+                                        int(accumulate), _ptr(out), C.c_void_p(ws.ptr), ws.nbytes, _stream_arg()))
+    return out
+
+
+def _gated_operands(what: str, x2: Tensor, w_gate: Tensor, w_up: Tensor, activation: str):
+    if activation not in _capi.ACT:
+        raise TTException(f"{what}: unknown activation {activation!r} (one of {', '.join(_capi.ACT)})")
+    if w_gate.dim() != 2 or w_up.shape != w_gate.shape or x2.size(1) != w_gate.size(0):
+        raise TTException(f"Invalid shape for matrix multiplication. LHS={x2.shape} and RHS={w_gate.shape}, {w_up.shape}")
+    return x2.size(0), w_gate.size(0), w_gate.size(1)
+
+
+def gated_linear(input: Tensor, w_gate: Tensor, w_up: Tensor, b_gate: Tensor | None = None, b_up: Tensor | None = None,
+                 activation: str = "silu", save: bool = False, out: Tensor | None = None, gate_out: Tensor | None = None,
+                 up_out: Tensor | None = None):
+    """The gated pair of Linear layers of a feed-forward block (ttamd_gated_linear_forward): act(input . w_gate + b_gate) *
+    (input . w_up + b_up), weights [in, hidden] like linear()'s and, like them, any views.  activation: silu, gelu (erf),
+    relu or sigmoid.  save: also return the two products (g, u) that gated_linear_backward() reads -> (h, g, u)."""
+    if input.dim() < 1:
+        raise TTException("gated_linear: the input needs a dimension")
+    x2 = input.unsqueeze(0) if input.dim() == 1 else input.flatten(0, -2) if input.dim() != 2 else input
+    rows, inner, hidden = _gated_operands("gated_linear", x2, w_gate, w_up, activation)
+    _check_operands("gated_linear", x2, w_gate, w_up, b_gate, b_up)
+    if any(b is not None and b.shape != (hidden,) for b in (b_gate, b_up)):
+        raise TTException(f"gated_linear: a bias holds {hidden} elements")
+    bg, bu = (b.contiguous() if b is not None else None for b in (b_gate, b_up))
+    shape = input.shape[:-1] + (hidden,)
+    save = save or gate_out is not None or up_out is not None
+    out = _result(out, shape, x2.dtype, x2.device, "gated_linear")
+    g = _result(gate_out, shape, x2.dtype, x2.device, "gated_linear") if save else None
+    u = _result(up_out, shape, x2.dtype, x2.device, "gated_linear") if save else None
+    ws = _workspace(lib.ttamd_gated_linear_workspace, x2.dtype, rows, inner, hidden, 0, device=x2.device)
+    xv, gv, uv = x2.view2(), w_gate.view2(), w_up.view2()
+    _check(lib.ttamd_gated_linear_forward(x2.device.id, x2.dtype, _capi.ACT[activation], rows, inner, hidden, C.byref(xv), C.byref(gv),
+                                          C.byref(uv), _ptr(bg), _ptr(bu), _ptr(out), _ptr(g), _ptr(u), C.c_void_p(ws.ptr), ws.nbytes,
+                                          _stream_arg()))
+    return (out, g, u) if save else out
+
+
+def gated_linear_backward(grad_output: Tensor, input: Tensor, w_gate: Tensor, w_up: Tensor, gate: Tensor, up: Tensor,
+                          activation: str = "silu", bias_grad: bool = True, out: tuple | None = None):
+    """Backward of gated_linear() for 2-D operands from the saved products `gate` and `up` (ttamd_gated_linear_backward).
+    Returns (dx, dw_gate, dw_up, db_gate, db_up), the last two None without bias_grad.  out: five tensors (None for what is
+    to be allocated) to write into."""
+    if input.dim() != 2:
+        raise TTException("gated_linear_backward: 2-D operands")
+    rows, inner, hidden = _gated_operands("gated_linear_backward", input, w_gate, w_up, activation)
+    _check_operands("gated_linear_backward", input, grad_output, w_gate, w_up, gate, up)
+    if any(t.shape != (rows, hidden) for t in (grad_output, gate, up)):
+        raise TTException(f"gated_linear_backward: grad_output, gate and up must be {(rows, hidden)}")
+    dh, g, u = grad_output.contiguous(), gate.contiguous(), up.contiguous()
+    shapes = [(rows, inner), (inner, hidden), (inner, hidden)] + [(hidden,)] * 2
+    given = out if out is not None else (None,) * 5
+    if len(given) != 5:
+        raise TTException("gated_linear_backward: out holds five tensors or None")
+    res = [_result(o, s, input.dtype, input.device, "gated_linear_backward") if i < 3 or bias_grad else None
+           for i, (o, s) in enumerate(zip(given, shapes))]
+    ws = _workspace(lib.ttamd_gated_linear_workspace, input.dtype, rows, inner, hidden, 1, device=input.device)
+    xv, gv, uv = input.view2(), w_gate.view2(), w_up.view2()
+    _check(lib.ttamd_gated_linear_backward(input.device.id, input.dtype, _capi.ACT[activation], rows, inner, hidden, _ptr(dh), C.byref(xv),
+                                           C.byref(gv), C.byref(uv), _ptr(g), _ptr(u), *(_ptr(r) for r in res), C.c_void_p(ws.ptr),
+                                           ws.nbytes, _stream_arg()))
+    return tuple(res)
+
+
+def distill_loss(input: Tensor, teacher_index: Tensor, teacher_logit: Tensor, temperature: float = 1.0, row_weight: Tensor | None = None,
+                 out: tuple | None = None):
+    """Distillation of the logits `input` [rows, cols] from a teacher's top logits [rows, top] at the columns
+    `teacher_index`, with its gradient in the same call (ttamd_distill_loss) -> (loss [1], grad_input [rows, cols]): the sum
+    over rows of row_weight (None: 1 / rows) * temperature^2 * KL(teacher's softmax over its slots || input's softmax).  An
+    index outside the columns is padding; a row of weight 0 or without a valid slot adds nothing.  input's columns must be
+    neighbours (else it is copied)."""
+    if input.dim() != 2 or teacher_logit.dim() != 2 or teacher_index.shape != teacher_logit.shape or teacher_logit.size(0) != input.size(0):
+        raise TTException("distill_loss: input must be [rows, cols], teacher_index and teacher_logit [rows, top]")
+    rows, cols = input.shape
+    _check_operands("distill_loss", input, teacher_logit, row_weight)
+    if row_weight is not None and row_weight.shape != (rows,):
+        raise TTException("distill_loss: row_weight must hold an element a row")
+    idx, logit = _check_indices("distill_loss", teacher_index, input.device), teacher_logit.contiguous()
+    weight = row_weight.contiguous() if row_weight is not None else None
+    z = input if (cols == 1 or input.stride[1] == 1) and (rows == 1 or input.stride[0] >= cols) else get_backend(input.device).identity(input)
+    if out is not None and len(out) != 2:
+        raise TTException("distill_loss: out holds the loss and the gradient")
+    loss = _result(out[0] if out else None, (1,), input.dtype, input.device, "distill_loss")
+    grad = _result(out[1] if out else None, (rows, cols), input.dtype, input.device, "distill_loss")
+    ws = _workspace(lib.ttamd_distill_loss_workspace, input.dtype, rows, cols, teacher_logit.size(1), device=input.device)
+    _check(lib.ttamd_distill_loss(input.device.id, input.dtype, idx.dtype, rows, cols, teacher_logit.size(1), _ptr(z), max(z.stride[0], cols),
+                                  _ptr(idx), _ptr(logit), _ptr(weight), temperature, _ptr(loss), _ptr(grad), C.c_void_p(ws.ptr), ws.nbytes,
+                                  _stream_arg()))
+    return loss, grad
 
 
 def conv2d(input: Tensor, weight: Tensor, bias: Tensor | None = None, stride: int = 1, padding: int = 0) -> Tensor:
