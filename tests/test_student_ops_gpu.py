@@ -399,11 +399,38 @@ def distill_data(r, rows, cols, top, dtype):
 @pytest.mark.parametrize("rows, cols, top", [(1, 1, 1), (3, 2, 2), (5, 3, 1), (4, 10, 4), (130, 10, 10), (7, 17, 5), (3, 64, 8), (9, 65, 33), (2, 257, 64),
                                              (5, 1000, 100), (3, 1024, 7), (3, 1025, 64), (2, 2051, 300), (6, 4096, 64), (3, 8191, 1), (2, 8200, 1024),
                                              (2, 16390, 16), (1, 33001, 128), (3, 65537, 70), (2, 98305, 33), (1, 131073, 64), (140, 5000, 12), (2, 200003, 9),
-                                             (300, 2000, 3), (0, 8, 2)])
+                                             (300, 2000, 3), (0, 8, 2), (2, 3, 300),
+                                             (5, 1, 1024), (3, 70, 1000), (4, 2, 65), (3, 64, 64), (3, 63, 257), (2, 1024, 256), (2, 900, 257)])
 def test_distill_loss(tt, dtype, rows, cols, top):
     r = rng_of(rows, cols, top)
     z, ids, t = distill_data(r, rows, cols, top, dtype)
     check_distill(tt, z, ids, t, 1.0 if cols % 2 else 2.5, None, dtype, index=np.int32 if top % 2 else np.int64)
+
+
+@pytest.mark.parametrize("dtype, rows, cols", [(np.float32, 140, 60001), (np.float32, 130, 98309), (np.float32, 140, 131072), (np.float32, 129, 200003),
+                                               (np.float64, 131, 65538), (np.float64, 129, 100001), (np.float32, 1600, 33000), (np.float32, 400, 131071),
+                                               (np.float64, 700, 37001), (np.float32, 15000, 3501)])
+def test_distill_loss_many_long_rows(tt, dtype, rows, cols):
+    """Rows that fill a workgroup's registers and more, and matrices beyond the caches: three rows' data over and over."""
+    r = rng_of(rows, cols)
+    top = 20
+    z, ids, t = distill_data(r, 3, cols, top, dtype)
+    of = np.arange(rows) % 3
+    w = (r.integers(0, 3, rows) / rows).astype(dtype)
+    _, grad, rel, _ = distill_reference(z, ids, t, 2.0, np.ones(3))
+    T = tt.Tensor.from_numpy
+    loss, got = tt.distill_loss(T(z[of]), T(ids[of]), T(t[of]), temperature=2.0, row_weight=T(w))
+    each = [distill_reference(z[k:k + 1], ids[k:k + 1], t[k:k + 1], 2.0, np.ones(1)) for k in range(3)]
+    got = got.to_numpy()
+    for k in range(3):
+        at = np.flatnonzero(of == k)
+        first = {}
+        for i in at:     # equal rows and weights give equal bits
+            assert np.array_equal(first.setdefault(w[i], got[i]), got[i])
+        for weight, g in first.items():
+            assert np.all(np.abs(g - weight * grad[k]) <= U[dtype] * (weight * rel[k] + 2 * np.abs(weight * grad[k])) + 1e-300)
+    want = sum(each[of[i]][0] * float(w[i]) for i in range(rows))
+    assert abs(loss.to_numpy()[0] - want) <= U[dtype] * (sum(each[of[i]][3] * float(w[i]) for i in range(rows)) + abs(want))
 
 
 # sizes of every way through the operator: tiny rows, a wave, workgroups of several sizes, rows cut into parts

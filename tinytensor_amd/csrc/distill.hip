@@ -13,6 +13,7 @@ namespace ttamd {
 namespace {
 
 constexpr int kMaxTop = 1024;  // slots a row may have: their indices, probabilities and student logits are kept in LDS
+constexpr int kLdsVecs = 8;    // vectors a lane may keep in LDS: 128 KB of the 160 KB for 1024 lanes, beside 20 KB of slots
 
 template <typename T>
 struct Num;
@@ -56,8 +57,10 @@ struct DistillArgs {
 // What a row's slots come to, in LDS.  p is 0 in a slot that does not count: an index outside the columns, a logit of -inf.
 template <typename T>
 struct Slots {
-    T p[kMaxTop], z[kMaxTop];
-    int index[kMaxTop];
+    T *p, *z;
+    int *index;
+    static size_t bytes(int64_t top) { return (static_cast<size_t>(top) * (2 * sizeof(T) + sizeof(int)) + 15) / 16 * 16; }
+    __device__ __forceinline__ Slots(void *lds, int top) : p(static_cast<T *>(lds)), z(p + top), index(reinterpret_cast<int *>(z + top)) {}
 };
 
 template <typename T>
@@ -83,7 +86,7 @@ __device__ __forceinline__ int slot_index(const DistillArgs<T> &a, int64_t row, 
 // One wave reads the row's slots into `s` (probabilities, student logits, indices); false when none counts, and the row
 // then contributes nothing.
 template <typename T>
-__device__ __forceinline__ bool read_slots(const DistillArgs<T> &a, int64_t row, int lane, Slots<T> &s) {
+__device__ __forceinline__ bool read_slots(const DistillArgs<T> &a, int64_t row, int lane, const Slots<T> &s) {
     const T *zr = a.z + row * a.z_row;
     T most = Num<T>::neg_inf();
     bool nan = false;
@@ -143,58 +146,147 @@ __device__ __forceinline__ T block_reduce(T v, T *lds) {
     return r;
 }
 
-// A workgroup a row: largest logit, then the sum of the exponentials, then the gradient.
+// A row that weighs nothing, or whose slots are all empty: no loss, a gradient of zeros.
 template <typename T, int BT>
-__global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a) {
+__device__ __forceinline__ void empty_row(const DistillArgs<T> &a, int64_t row) {
     using V = typename Num<T>::vec_t;
     constexpr int W = Num<T>::W;
-    __shared__ Slots<T> slots;
+    T *gr = a.grad + row * a.cols;
+    const int nvec = a.cols / W;
+    V zero;
+#pragma unroll
+    for (int k = 0; k < W; ++k) zero[k] = T(0);
+    for (int v = threadIdx.x; v < nvec; v += BT) reinterpret_cast<V *>(gr)[v] = zero;
+    for (int i = nvec * W + threadIdx.x; i < a.cols; i += BT) gr[i] = T(0);
+    if (threadIdx.x == 0) a.row_loss[row] = 0.0;
+}
+
+// A workgroup a row.  The row is requested once and stays: NV vectors of it in every lane's registers, `lds_vecs` more in
+// the lane's own places in LDS, and only what is beyond both is read again for the sum and for the gradient (a row of
+// 131072 floats just fits: 24 vectors in registers, 8 in LDS).  Columns behind the row's last whole vector go one by one.
+// NT: loads and stores that leave the caches alone, for matrices that would not stay in them anyway.
+// Traffic is the floor's, read once and written once: 2048 x 32000 f32 with 64 slots 97 us (5.4 TB/s; a copy of 2 GiB
+// reaches 4.9), 4096 x 131072 842 us (5.1 TB/s); as three reads and a write these took 199 and 1641 us.
+template <typename T, int BT, int NV, bool NT>
+__global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int lds_vecs) {
+    using V = typename Num<T>::vec_t;
+    typedef T lds_t __attribute__((ext_vector_type(Num<T>::W)));
+    constexpr int W = Num<T>::W;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    lds_t *const more = reinterpret_cast<lds_t *>(smem);  // [lds_vecs][BT]
+    const Slots<T> slots(smem + static_cast<size_t>(lds_vecs) * BT * sizeof(lds_t), a.top);
     __shared__ T red[2][BT / 64];
     __shared__ int counts;
     const int64_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid % 64;
     const T *zr = a.z + row * a.z_row;
     T *gr = a.grad + row * a.cols;
-    const int nvec = a.cols / W, tail0 = nvec * W;
+    const int nvec = a.cols / W, tail = nvec * W + tid;
     const T w = a.weight ? a.weight[row] : a.uniform_weight;
-    if (tid < 64) {
-        const bool on = w != T(0) && read_slots(a, row, lane, slots);
-        if (tid == 0) counts = on;
-    }
-    __syncthreads();
-    if (!counts) {  // a row that weighs nothing, or whose slots are all empty: no loss, no gradient, nothing read
-        V zero;
-#pragma unroll
-        for (int k = 0; k < W; ++k) zero[k] = T(0);
-        for (int v = tid; v < nvec; v += BT) reinterpret_cast<V *>(gr)[v] = zero;
-        if (tail0 + tid < a.cols) gr[tail0 + tid] = T(0);
-        if (tid == 0) a.row_loss[row] = 0.0;
+    if (w == T(0)) {  // (the same for the whole workgroup)
+        empty_row<T, BT>(a, row);
         return;
     }
-    T most = Num<T>::neg_inf();
-    for (int v = tid; v < nvec; v += BT) {
+    if (tid < 64) {  // (while the other waves request the row; with the vectors already held it would run out of registers)
+        const bool on = read_slots(a, row, lane, slots);
+        if (tid == 0) counts = on;
+    }
+    // Every lane requests its vectors before any is used.  A place behind the row's end repeats the last vector and is set
+    // to -inf afterwards, which leaves the maximum alone and adds 0 to the sum: a branch around each load would wait for
+    // each load.  (A row shorter than a vector comes here for its many slots; it requests its first column for nothing.)
+    V held[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = tid + i * BT;
+        if (nvec == 0) {
+            held[i] = V{} + zr[0];
+            continue;
+        }
+        const V *at = &reinterpret_cast<const V *>(zr)[v < nvec ? v : nvec - 1];
+        if constexpr (NT) held[i] = __builtin_nontemporal_load(at);
+        else held[i] = *at;
+    }
+    T last = tail < a.cols ? zr[tail] : Num<T>::neg_inf();
+    const int lds_end = (NV + lds_vecs) * BT < nvec ? (NV + lds_vecs) * BT : nvec;
+    T most = last;
+    for (int v = NV * BT + tid; v < lds_end; v += BT) {
+        const V x = reinterpret_cast<const V *>(zr)[v];
+        lds_t y;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            y[k] = x[k];
+            most = Num<T>::max_(most, x[k]);
+        }
+        more[v - NV * BT] = y;
+    }
+    for (int v = (NV + lds_vecs) * BT + tid; v < nvec; v += BT) {
         const V x = reinterpret_cast<const V *>(zr)[v];
 #pragma unroll
         for (int k = 0; k < W; ++k) most = Num<T>::max_(most, x[k]);
     }
-    if (tail0 + tid < a.cols) most = Num<T>::max_(most, zr[tail0 + tid]);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const bool in = tid + i * BT < nvec;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            held[i][k] = in ? held[i][k] : Num<T>::neg_inf();
+            most = Num<T>::max_(most, held[i][k]);
+        }
+    }
     most = block_reduce<T, BT, true>(most, red[0]);
     T total = T(0);
-    for (int v = tid; v < nvec; v += BT) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            held[i][k] = Num<T>::exp_scaled(held[i][k] - most, a.c);
+            total += held[i][k];
+        }
+    for (int v = NV * BT + tid; v < lds_end; v += BT) {
+        lds_t x = more[v - NV * BT];
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            x[k] = Num<T>::exp_scaled(x[k] - most, a.c);
+            total += x[k];
+        }
+        more[v - NV * BT] = x;
+    }
+    for (int v = (NV + lds_vecs) * BT + tid; v < nvec; v += BT) {
         const V x = reinterpret_cast<const V *>(zr)[v];
 #pragma unroll
         for (int k = 0; k < W; ++k) total += Num<T>::exp_scaled(x[k] - most, a.c);
     }
-    if (tail0 + tid < a.cols) total += Num<T>::exp_scaled(zr[tail0 + tid] - most, a.c);
+    last = tail < a.cols ? Num<T>::exp_scaled(last - most, a.c) : T(0);
+    total += last;
     total = block_reduce<T, BT, false>(total, red[1]);
+    if (!counts) {
+        empty_row<T, BT>(a, row);
+        return;
+    }
     const T wt = w * static_cast<T>(a.temperature), f = wt / total;
-    for (int v = tid; v < nvec; v += BT) {
+    const auto put = [&](int v, V x) {
+        if constexpr (NT) __builtin_nontemporal_store(x, &reinterpret_cast<V *>(gr)[v]);
+        else reinterpret_cast<V *>(gr)[v] = x;
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int v = tid + i * BT;
+        if (v < nvec) put(v, held[i] * f);
+    }
+    for (int v = NV * BT + tid; v < lds_end; v += BT) {
+        const lds_t x = more[v - NV * BT];
+        V y;
+#pragma unroll
+        for (int k = 0; k < W; ++k) y[k] = x[k] * f;
+        put(v, y);
+    }
+    for (int v = (NV + lds_vecs) * BT + tid; v < nvec; v += BT) {
         V x = reinterpret_cast<const V *>(zr)[v];
 #pragma unroll
         for (int k = 0; k < W; ++k) x[k] = Num<T>::exp_scaled(x[k] - most, a.c) * f;
-        reinterpret_cast<V *>(gr)[v] = x;
+        put(v, x);
     }
-    if (tail0 + tid < a.cols) gr[tail0 + tid] = Num<T>::exp_scaled(zr[tail0 + tid] - most, a.c) * f;
+    if (tail < a.cols) gr[tail] = last * f;
     if (tid < 64) {
         const double loss = slots_loss(a, lane, slots, most, total);
         if (tid == 0) a.row_loss[row] = static_cast<double>(w) * loss;
@@ -205,6 +297,211 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a) {
             gr[slots.index[j]] = Num<T>::exp_scaled(slots.z[j] - most, a.c) * f - wt * slot_share(slots, a.top, j);
 }
 
+// Short rows: G lanes own a row, E columns each (lane l: columns l, l + G, ..), up to 4 G slots.  Everything stays in
+// registers; the slots go round the group one by one and the lane that holds a slot's column takes its share off.
+template <typename T, int G, int E>
+__global__ void __launch_bounds__(256) distill_short_kernel(DistillArgs<T> a) {
+    constexpr int S = 4;  // slots a lane
+    const int64_t row_of = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / G;
+    const bool live = row_of < a.rows;
+    const int64_t row = live ? row_of : a.rows - 1;  // (every lane takes part in the shuffles)
+    const int lane = threadIdx.x % G;
+    const T *zr = a.z + row * a.z_row;
+    const T w = a.weight ? a.weight[row] : a.uniform_weight;
+    T e[E], zs[S], p[S];
+    int index[S];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int c = lane + i * G;
+        e[i] = zr[c < a.cols ? c : a.cols - 1];
+    }
+    T tmost = Num<T>::neg_inf();
+    int nan = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int j = lane + s * G;
+        index[s] = -1;
+        p[s] = Num<T>::neg_inf();
+        if (j < a.top) {
+            index[s] = slot_index(a, row, j);
+            if (index[s] >= 0) p[s] = a.teacher[row * a.top + j];
+        }
+        zs[s] = zr[index[s] >= 0 ? index[s] : 0];
+        tmost = Num<T>::max_(tmost, p[s]);
+        nan |= p[s] != p[s];
+    }
+    T most = Num<T>::neg_inf();
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (lane + i * G >= a.cols) e[i] = Num<T>::neg_inf();
+        most = Num<T>::max_(most, e[i]);
+    }
+#pragma unroll
+    for (int d = G / 2; d > 0; d /= 2) {
+        most = Num<T>::max_(most, __shfl_xor(most, d, G));
+        tmost = Num<T>::max_(tmost, __shfl_xor(tmost, d, G));
+        nan |= __shfl_xor(nan, d, G);
+    }
+    T total = T(0), ptotal = T(0);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        e[i] = Num<T>::exp_scaled(e[i] - most, a.c);
+        if (lane + i * G >= a.cols) e[i] = T(0);
+        total += e[i];
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        p[s] = index[s] >= 0 ? Num<T>::exp_scaled(p[s] - tmost, a.c) : T(0);
+        ptotal += p[s];
+    }
+#pragma unroll
+    for (int d = G / 2; d > 0; d /= 2) {
+        total += __shfl_xor(total, d, G);
+        ptotal += __shfl_xor(ptotal, d, G);
+    }
+    const bool on = w != T(0) && (tmost != Num<T>::neg_inf() || nan);
+    const double inv = 1.0 / a.temperature, log_total = log(static_cast<double>(total));
+    double loss = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        p[s] /= ptotal;
+        const double pj = index[s] >= 0 ? static_cast<double>(p[s]) : 0.0;
+        if (pj != 0.0) loss += pj * (log(pj) - ((static_cast<double>(zs[s]) - static_cast<double>(most)) * inv - log_total));
+    }
+#pragma unroll
+    for (int d = G / 2; d > 0; d /= 2) loss += __shfl_xor(loss, d, G);
+    const T wt = w * static_cast<T>(a.temperature), f = wt / total;
+    T share[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) share[i] = T(0);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int n = a.top - s * G < G ? a.top - s * G : G;
+        for (int k = 0; k < n; ++k) {
+            const int c = __shfl(index[s], k, G);
+            const T pk = __shfl(p[s], k, G);
+#pragma unroll
+            for (int i = 0; i < E; ++i) share[i] += c == lane + i * G ? pk : T(0);
+        }
+    }
+    if (!live) return;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int c = lane + i * G;
+        if (c < a.cols) a.grad[row * a.cols + c] = on ? e[i] * f - wt * share[i] : T(0);
+    }
+    if (lane == 0) a.row_loss[row] = on ? static_cast<double>(w) * a.temperature * a.temperature * loss : 0.0;
+}
+
+// Few long rows: a workgroup has a part of a row, kPartVecs vectors a lane.  The first kernel leaves the part's largest
+// logit and its sum of exponentials below that; the second joins the row's parts and writes the part's gradient, from
+// logits that are still in a cache.
+constexpr int kPartThreads = 256, kPartVecs = 4;
+
+template <typename T>
+struct PartSums {
+    T most, total;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kPartThreads) distill_part_kernel(DistillArgs<T> a, PartSums<T> *parts) {
+    using V = typename Num<T>::vec_t;
+    constexpr int W = Num<T>::W;
+    __shared__ T red[2][kPartThreads / 64];
+    const int64_t row = blockIdx.y;
+    const int tid = threadIdx.x;
+    if (a.weight && a.weight[row] == T(0)) return;  // (nobody reads its parts)
+    const T *zr = a.z + row * a.z_row;
+    const int nvec = a.cols / W, first = blockIdx.x * (kPartThreads * kPartVecs) + tid;
+    const int tail = nvec * W + tid;
+    V x[kPartVecs];
+#pragma unroll
+    for (int i = 0; i < kPartVecs; ++i) {
+        const int v = first + i * kPartThreads;
+        x[i] = reinterpret_cast<const V *>(zr)[v < nvec ? v : nvec - 1];
+    }
+    const T last = blockIdx.x == 0 && tail < a.cols ? zr[tail] : Num<T>::neg_inf();  // (the odd columns belong to part 0)
+    T most = last;
+#pragma unroll
+    for (int i = 0; i < kPartVecs; ++i)
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            if (first + i * kPartThreads >= nvec) x[i][k] = Num<T>::neg_inf();
+            most = Num<T>::max_(most, x[i][k]);
+        }
+    most = block_reduce<T, kPartThreads, true>(most, red[0]);
+    const T base = most == Num<T>::neg_inf() ? T(0) : most;  // a part of nothing but -inf adds 0 to its row (a NaN stays one)
+    T total = Num<T>::exp_scaled(last - base, a.c);
+#pragma unroll
+    for (int i = 0; i < kPartVecs; ++i)
+#pragma unroll
+        for (int k = 0; k < W; ++k) total += Num<T>::exp_scaled(x[i][k] - base, a.c);
+    total = block_reduce<T, kPartThreads, false>(total, red[1]);
+    if (tid == 0) parts[row * gridDim.x + blockIdx.x] = {most, total};
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPartThreads) distill_join_kernel(DistillArgs<T> a, const PartSums<T> *parts) {
+    using V = typename Num<T>::vec_t;
+    constexpr int W = Num<T>::W;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const Slots<T> slots(smem, a.top);
+    __shared__ T red[2][kPartThreads / 64];
+    __shared__ int counts;
+    const int64_t row = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid % 64;
+    const T *zr = a.z + row * a.z_row;
+    T *gr = a.grad + row * a.cols;
+    const int nvec = a.cols / W, first = blockIdx.x * (kPartThreads * kPartVecs) + tid;
+    const int tail = nvec * W + tid;
+    const T w = a.weight ? a.weight[row] : a.uniform_weight;
+    const bool mine = blockIdx.x == 0;
+    V x[kPartVecs];
+    T last = Num<T>::neg_inf();
+    if (w != T(0)) {
+#pragma unroll
+        for (int i = 0; i < kPartVecs; ++i) {
+            const int v = first + i * kPartThreads;
+            x[i] = reinterpret_cast<const V *>(zr)[v < nvec ? v : nvec - 1];
+        }
+        if (mine && tail < a.cols) last = zr[tail];
+        if (tid < 64) {
+            const bool on = read_slots(a, row, lane, slots);
+            if (tid == 0) counts = on;
+        }
+    }
+    T most = Num<T>::neg_inf(), total = T(0);
+    if (w != T(0)) {
+        const PartSums<T> *own = parts + row * gridDim.x;
+        for (int i = tid; i < static_cast<int>(gridDim.x); i += kPartThreads) most = Num<T>::max_(most, own[i].most);
+        most = block_reduce<T, kPartThreads, true>(most, red[0]);
+        for (int i = tid; i < static_cast<int>(gridDim.x); i += kPartThreads) total += own[i].total * Num<T>::exp_scaled(own[i].most - most, a.c);
+        total = block_reduce<T, kPartThreads, false>(total, red[1]);
+    }
+    const bool on = w != T(0) && counts;  // (counts: written before the reductions' barriers)
+    const T wt = w * static_cast<T>(a.temperature), f = wt / total;
+#pragma unroll
+    for (int i = 0; i < kPartVecs; ++i) {
+        const int v = first + i * kPartThreads;
+#pragma unroll
+        for (int k = 0; k < W; ++k) x[i][k] = on ? Num<T>::exp_scaled(x[i][k] - most, a.c) * f : T(0);
+        if (v < nvec) reinterpret_cast<V *>(gr)[v] = x[i];
+    }
+    if (mine && tail < a.cols) gr[tail] = on ? Num<T>::exp_scaled(last - most, a.c) * f : T(0);
+    if (mine && tid < 64) {
+        const double loss = on ? slots_loss(a, lane, slots, most, total) : 0.0;
+        if (tid == 0) a.row_loss[row] = on ? static_cast<double>(w) * loss : 0.0;
+    }
+    if (!on) return;
+    __syncthreads();  // the bulk first, then the teacher's columns that lie in this part
+    const int c0 = blockIdx.x * (kPartThreads * kPartVecs * W), c1 = c0 + kPartThreads * kPartVecs * W;
+    for (int j = tid; j < a.top; j += kPartThreads) {
+        const int c = slots.index[j];
+        if (c >= 0 && (c >= nvec * W ? mine : c >= c0 && c < c1))
+            gr[c] = Num<T>::exp_scaled(slots.z[j] - most, a.c) * f - wt * slot_share(slots, a.top, j);
+    }
+}
+
 // loss = sum of the rows' losses: a lane adds every 1024th, the lanes are added in a fixed order.
 template <typename T>
 __global__ void __launch_bounds__(1024) distill_sum_kernel(const double *row_loss, int64_t rows, T *out) {
@@ -213,6 +510,60 @@ __global__ void __launch_bounds__(1024) distill_sum_kernel(const double *row_los
     for (int64_t r = threadIdx.x; r < rows; r += 1024) v += row_loss[r];
     v = block_reduce<double, 1024, false>(v, red);
     if (threadIdx.x == 0) out[0] = static_cast<T>(v);
+}
+
+// Where the parts' sums begin in the workspace, behind the rows' losses, and how many parts a row is cut into (0: none).
+size_t part_offset(int64_t rows) { return (static_cast<size_t>(rows) * sizeof(double) + 15) / 16 * 16; }
+
+int64_t parts_of(size_t item, int64_t rows, int64_t cols) {
+    const int64_t vec = 16 / static_cast<int64_t>(item), per = kPartThreads * kPartVecs * vec;
+    const int64_t row_bytes = cols * static_cast<int64_t>(item);
+    return rows <= 128 && row_bytes > 32768 ? (cols + per - 1) / per : 0;
+}
+
+template <typename T>
+ttamd_status launch_rows(const DistillArgs<T> &a, void *parts, hipStream_t st) {
+    const size_t slots = Slots<T>::bytes(a.top);
+    if (a.cols <= 64 && a.top <= 64) {
+        distill_short_kernel<T, 16, 4><<<static_cast<unsigned>((a.rows + 15) / 16), 256, 0, st>>>(a);
+    } else if (a.cols <= 1024 && a.top <= 256) {
+        distill_short_kernel<T, 64, 16><<<static_cast<unsigned>((a.rows + 3) / 4), 256, 0, st>>>(a);
+    } else if (const int64_t n = parts_of(sizeof(T), a.rows, a.cols)) {
+        const dim3 grid(static_cast<unsigned>(n), static_cast<unsigned>(a.rows));
+        distill_part_kernel<T><<<grid, kPartThreads, 0, st>>>(a, static_cast<PartSums<T> *>(parts));
+        TTAMD_HIP_CHECK(hipGetLastError());
+        distill_join_kernel<T><<<grid, kPartThreads, slots, st>>>(a, static_cast<const PartSums<T> *>(parts));
+    } else {
+        const int64_t nvec = a.cols / Num<T>::W;
+        const auto run = [&](auto kernel, int threads, int held) -> ttamd_status {
+            const int64_t left = nvec - static_cast<int64_t>(threads) * held;
+            int64_t lds_vecs = left > 0 ? (left + threads - 1) / threads : 0;
+            if (lds_vecs > kLdsVecs) lds_vecs = kLdsVecs;
+            const size_t lds = static_cast<size_t>(lds_vecs) * threads * 16 + slots;
+            if (lds > 48 * 1024)
+                TTAMD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+            kernel<<<static_cast<unsigned>(a.rows), threads, lds, st>>>(a, static_cast<int>(lds_vecs));
+            return TTAMD_OK;
+        };
+        // The smallest form that keeps the row: small workgroups share a CU and one's loads run under another's stores
+        // (4096 x 8000 f32: 51 us with 256 x 8, 117 with 1024 x 8; 2048 x 64000: 214 with 1024 x 16, 294 with 256 x 32).
+        // 24 vectors a lane only where they keep a row that 16 and LDS would not: they spill (rows beyond that: 488 us with
+        // 16, 517 with 24 at 1024 x 100003 f64).
+        const auto pick = [&]<bool NT>() {
+            if (nvec <= 256 * 4) return run(distill_row_kernel<T, 256, 4, NT>, 256, 4);
+            if (nvec <= 256 * 8) return run(distill_row_kernel<T, 256, 8, NT>, 256, 8);
+            if (nvec <= 512 * 8) return run(distill_row_kernel<T, 512, 8, NT>, 512, 8);
+            if (nvec <= 512 * 16) return run(distill_row_kernel<T, 512, 16, NT>, 512, 16);
+            if (nvec > 1024 * 24 && nvec <= 1024 * 32) return run(distill_row_kernel<T, 1024, 24, NT>, 1024, 24);
+            return run(distill_row_kernel<T, 1024, 16, NT>, 1024, 16);
+        };
+        // Logits and gradient beyond 1.5 times the 256 MB Infinity Cache pass it by (2 x 262 MB: 97 us against 112;
+        // 2 x 131 MB: 56 against 55, and there the next kernel finds part of the gradient in it).
+        const bool beyond = static_cast<double>(a.rows) * a.cols * sizeof(T) > 192.0 * (1 << 20);
+        if (ttamd_status s = beyond ? pick.template operator()<true>() : pick.template operator()<false>()) return s;
+    }
+    TTAMD_HIP_CHECK(hipGetLastError());
+    return TTAMD_OK;
 }
 
 template <typename T>
@@ -235,8 +586,7 @@ ttamd_status launch_distill(int64_t rows, int64_t cols, int64_t top, const void 
         a.temperature = temperature;
         a.c = static_cast<T>(sizeof(T) == 4 ? 1.4426950408889634 / temperature : 1.0 / temperature);
         a.uniform_weight = static_cast<T>(1.0 / static_cast<double>(rows));
-        distill_row_kernel<T, 256><<<dim3(static_cast<unsigned>(rows)), 256, 0, st>>>(a);
-        TTAMD_HIP_CHECK(hipGetLastError());
+        if (ttamd_status s = launch_rows(a, static_cast<char *>(workspace) + part_offset(rows), st)) return s;
     }
     distill_sum_kernel<T><<<1, 1024, 0, st>>>(static_cast<const double *>(workspace), rows, static_cast<T *>(loss_out));
     TTAMD_HIP_CHECK(hipGetLastError());
@@ -269,7 +619,8 @@ ttamd_status ttamd_distill_loss_workspace(ttamd_dtype dtype, int64_t rows, int64
         set_error("distill_loss: bytes is NULL");
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
-    *bytes = static_cast<size_t>(rows) * sizeof(double);
+    const size_t e = dtype_size(dtype);
+    *bytes = part_offset(rows) + static_cast<size_t>(parts_of(e, rows, cols) * rows) * 2 * e;
     return TTAMD_OK;
 }
 
