@@ -32,6 +32,18 @@ __device__ __forceinline__ int64_t load_index(const void *index, int64_t i) {
     else return static_cast<const int32_t *>(index)[i];
 }
 
+// A wave sets a row to zero; the last vector is moved back to end with the row.
+template <typename T>
+__device__ __forceinline__ void zero_row(T *row, int64_t dim, int lane) {
+    using V = typename Row<T>::vec_t;
+    constexpr int W = Row<T>::W;
+    if (dim < W) {
+        if (lane < dim) row[lane] = T(0);
+        return;
+    }
+    for (int64_t d = lane * W; d < dim; d += 64 * W) *reinterpret_cast<V *>(row + (d + W <= dim ? d : dim - W)) = V{};
+}
+
 // ---- forward ----------------------------------------------------------------------------------------------------------
 // 2^lanes_log lanes own a row and walk it in vectors.  A row whose length is no multiple of the vector ends in a vector
 // that is moved back to end with the row: its first elements are written twice, with the same values.  VEC = false: one
@@ -84,9 +96,25 @@ struct OrderArgs {
     int bucket_log;   // log2 of the number of buckets
     int tokens;       // tokens a bucket has room for: ceil(vocab / buckets)
     int32_t *position, *token;  // [count] in the order of the tokens
-    int32_t *total;   // positions whose index lies in the table
+    int32_t *total;   // [0]: positions whose index lies in the table; [1]: 0
     void *grad;       // rows of tokens that no position has are set to zero here, or null: left alone
 };
+
+constexpr int kBatch = 8;  // loads of 64 indices in flight: with one at a time a scan of 60000 indices took 27 us of waiting
+
+// The next kBatch x 64 positions of a wave's share: lane l's u-th index is that of position i0 + 64 u + l; -1 where there is
+// none, or where it names no row.
+template <bool I64>
+__device__ __forceinline__ void load_batch(const OrderArgs &a, int64_t i0, int64_t last, int lane, int (&v)[kBatch]) {
+    int64_t x[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+        const int64_t i = i0 + u * 64 + lane;
+        x[u] = load_index<I64>(a.index, i < last ? i : last - 1);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) v[u] = i0 + u * 64 + lane < last && x[u] >= 0 && x[u] < a.vocab ? static_cast<int>(x[u]) : -1;
+}
 
 template <typename T, bool I64>
 __global__ void __launch_bounds__(kOrderThreads) embedding_order_kernel(OrderArgs a) {
@@ -101,12 +129,15 @@ __global__ void __launch_bounds__(kOrderThreads) embedding_order_kernel(OrderArg
     const int64_t per = (a.count + kOrderWaves - 1) / kOrderWaves;
     const int64_t first = wave * per, last = first + per < a.count ? first + per : a.count;
     int below = 0;
-    for (int64_t i = first + lane; i < last; i += 64) {
-        const int64_t v = load_index<I64>(a.index, i);
-        if (v < 0 || v >= a.vocab) continue;
-        const int b = static_cast<int>(v & (buckets - 1));
-        below += b < mine;
-        if (b == mine) atomicAdd(&counters[static_cast<int>(v >> a.bucket_log) * kOrderWaves + wave], 1);
+    int v[kBatch];
+    for (int64_t i0 = first; i0 < last; i0 += kBatch * 64) {
+        load_batch<I64>(a, i0, last, lane, v);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int b = v[u] & (buckets - 1);
+            below += v[u] >= 0 && b < mine;
+            if (v[u] >= 0 && b == mine) atomicAdd(&counters[(v[u] >> a.bucket_log) * kOrderWaves + wave], 1);
+        }
     }
 #pragma unroll
     for (int d = 32; d > 0; d /= 2) below += __shfl_xor(below, d, 64);
@@ -131,7 +162,10 @@ __global__ void __launch_bounds__(kOrderThreads) embedding_order_kernel(OrderArg
         base += below_sum[w];
         in_bucket += wave_sum[w];
     }
-    if (mine == buckets - 1 && tid == 0) *a.total = base + in_bucket;
+    if (mine == buckets - 1 && tid == 0) {
+        a.total[0] = base + in_bucket;
+        a.total[1] = 0;  // (the sums' list of crossing runs)
+    }
     int at = base + run - own;
     for (int w = 0; w < wave; ++w) at += wave_sum[w];
     for (int i = c0; i < c1; ++i) {
@@ -144,73 +178,63 @@ __global__ void __launch_bounds__(kOrderThreads) embedding_order_kernel(OrderArg
     if (a.grad) {
         const int end = base + in_bucket;
         for (int t = wave; t < a.tokens; t += kOrderWaves) {
-            const int64_t v = (static_cast<int64_t>(t) << a.bucket_log) + mine;
-            if (v >= a.vocab) break;
+            const int64_t row = (static_cast<int64_t>(t) << a.bucket_log) + mine;
+            if (row >= a.vocab) break;
             const int next = t + 1 < a.tokens ? counters[(t + 1) * kOrderWaves] : end;
             if (counters[t * kOrderWaves] != next) continue;
-            T *row = static_cast<T *>(a.grad) + v * a.dim;
-            for (int64_t d = lane; d < a.dim; d += 64) row[d] = T(0);
+            zero_row(static_cast<T *>(a.grad) + row * a.dim, a.dim, lane);
         }
     }
     __syncthreads();  // the cells are moved on from here
-    for (int64_t i0 = first; i0 < last; i0 += 64) {
-        const int64_t i = i0 + lane;
-        const int64_t v = i < last ? load_index<I64>(a.index, i) : -1;
-        const bool in = v >= 0 && v < a.vocab && static_cast<int>(v & (buckets - 1)) == mine;
-        const int t = static_cast<int>(v >> a.bucket_log);
-        uint64_t left = __ballot(in);
-        while (left) {  // a round for each different token among the 64 positions
-            const int lead = __builtin_ctzll(left);
-            const int which = __builtin_amdgcn_readlane(t, lead);
-            const uint64_t same = __ballot(in && t == which);
-            const int cell = which * kOrderWaves + wave;
-            const int place = counters[cell];
-            if (in && t == which) {
-                const int p = place + __popcll(same & ((1ull << lane) - 1));
-                a.position[p] = static_cast<int32_t>(i);
-                a.token[p] = static_cast<int32_t>(v);
+    for (int64_t i0 = first; i0 < last; i0 += kBatch * 64) {
+        if (per > kBatch * 64) load_batch<I64>(a, i0, last, lane, v);  // (a share of one batch is still there)
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const bool in = v[u] >= 0 && (v[u] & (buckets - 1)) == mine;
+            const int t = v[u] >> a.bucket_log;
+            uint64_t left = __ballot(in);
+            while (left) {  // a round for each different token among the 64 positions
+                const int lead = __builtin_ctzll(left);
+                const int which = __builtin_amdgcn_readlane(t, lead);
+                const uint64_t same = __ballot(in && t == which);
+                const int cell = which * kOrderWaves + wave;
+                const int place = counters[cell];
+                if (in && t == which) {
+                    const int p = place + __popcll(same & ((1ull << lane) - 1));
+                    a.position[p] = static_cast<int32_t>(i0 + u * 64 + lane);
+                    a.token[p] = v[u];
+                }
+                if (lane == lead) counters[cell] = place + __popcll(same);
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the other lanes read the cell in a later round
+                left &= ~same;
             }
-            if (lane == lead) counters[cell] = place + __popcll(same);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the other lanes read the cell in a later round
-            left &= ~same;
         }
     }
 }
 
 // ---- gradient: the sums ------------------------------------------------------------------------------------------------
-// A wave adds up the rows of kRun ordered positions, 64 vectors of columns wide.  A run of equal tokens that lies inside
-// goes to the gradient; the part of one that began before is left in partial[2 c], of one that goes on in
+// A wave adds up the rows of a chunk of ordered positions, 64 vectors of columns wide.  A run of equal tokens that lies
+// inside goes to the gradient; the part of one that began before is left in partial[2 c], of one that goes on in
 // partial[2 c + 1].  Sums are held in 64 bits: the conversions cost nothing beside the loads, and a frequent token's sum
 // over tens of thousands of rows keeps its last bits.
-constexpr int kRun = 16;
-constexpr int kJoinWaves = 4;
+// Chunks of 64 positions leave a quarter of the parts of chunks of 16, but a quarter of the waves: plan_backward.
+constexpr int kRows = 8;       // rows in flight ahead of those that are being added
+constexpr int kJoinWaves = 16;
+constexpr int kLongRun = 64;   // parts from which a whole workgroup joins a run
 
 template <typename T>
 struct SumArgs {
     const T *dy;
     T *grad;
     double *partial;  // [2 * chunks][dim]
-    const int32_t *position, *token, *total;
+    const int32_t *position, *token;
+    int32_t *total;   // [0]: ordered positions; [1]: chunks in `crossing`
+    int32_t *crossing;  // [chunks] those whose last run begins in them and goes on
     int64_t dim;
+    int chunk;  // positions a chunk: 16 or 64
     double scale;
     int accumulate;
 };
-
-template <typename T, int W>
-__device__ __forceinline__ void write_gradient(const SumArgs<T> &a, int64_t token, int64_t col, const double (&sum)[W]) {
-    T *g = a.grad + token * a.dim + col;
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-        const double v = sum[k] * a.scale;
-        g[k] = a.accumulate ? static_cast<T>(static_cast<double>(g[k]) + v) : static_cast<T>(v);
-    }
-}
-
-template <typename T, int W>
-__device__ __forceinline__ void write_partial(const SumArgs<T> &a, int64_t part, int64_t col, const double (&sum)[W]) {
-#pragma unroll
-    for (int k = 0; k < W; ++k) a.partial[part * a.dim + col + k] = sum[k];
-}
 
 template <typename T, int W>
 __device__ __forceinline__ void load_row(const T *p, T (&x)[W]) {
@@ -224,12 +248,45 @@ __device__ __forceinline__ void load_row(const T *p, T (&x)[W]) {
 }
 
 template <typename T, int W>
+__device__ __forceinline__ void write_gradient(const SumArgs<T> &a, int64_t token, int64_t col, const double (&sum)[W]) {
+    T *g = a.grad + token * a.dim + col;
+    T x[W];
+    if (a.accumulate) load_row<T, W>(g, x);
+#pragma unroll
+    for (int k = 0; k < W; ++k) x[k] = static_cast<T>(a.accumulate ? static_cast<double>(x[k]) + sum[k] * a.scale : sum[k] * a.scale);
+    if constexpr (W == 1) {
+        *g = x[0];
+    } else {
+        typename Row<T>::vec_t v;
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[k] = x[k];
+        *reinterpret_cast<typename Row<T>::vec_t *>(g) = v;
+    }
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void write_partial(const SumArgs<T> &a, int64_t part, int64_t col, const double (&sum)[W]) {
+    double *p = a.partial + part * a.dim + col;
+    if constexpr (W == 1) {
+        *p = sum[0];
+    } else {
+#pragma unroll
+        for (int k = 0; k < W; k += 2) {
+            Row<double>::vec_t v;
+            v[0] = sum[k];
+            v[1] = sum[k + 1];
+            *reinterpret_cast<Row<double>::vec_t *>(p + k) = v;
+        }
+    }
+}
+
+template <typename T, int W>
 __global__ void __launch_bounds__(64) embedding_sum_kernel(SumArgs<T> a) {
-    const int total = *a.total;
+    const int total = a.total[0];
     const int64_t c = blockIdx.x;
-    const int64_t s0 = c * kRun;
+    const int64_t s0 = c * a.chunk;
     if (s0 >= total) return;
-    const int n = total - s0 < kRun ? static_cast<int>(total - s0) : kRun;
+    const int n = total - s0 < a.chunk ? static_cast<int>(total - s0) : a.chunk;
     const int lane = threadIdx.x;
     // (lanes beyond the row's end stay and work on its first columns: every lane's position is read by the others)
     const bool live = (static_cast<int64_t>(blockIdx.y) * 64 + lane) * W < a.dim;
@@ -239,19 +296,22 @@ __global__ void __launch_bounds__(64) embedding_sum_kernel(SumArgs<T> a) {
     const int position = a.position[s0 + mine], token = a.token[s0 + mine];
     const int before = c > 0 ? a.token[s0 - 1] : -1;
     const int after = s0 + n < total ? a.token[s0 + n] : -1;
-    T x[kRun][W];
+    T x[2][kRows][W];
+    const auto load = [&](int i0, T (&to)[kRows][W]) {
 #pragma unroll
-    for (int i = 0; i < kRun; ++i)
-        load_row<T, W>(a.dy + static_cast<int64_t>(__builtin_amdgcn_readlane(position, i)) * a.dim + col, x[i]);
+        for (int i = 0; i < kRows; ++i)
+            load_row<T, W>(a.dy + static_cast<int64_t>(__builtin_amdgcn_readlane(position, i0 + i)) * a.dim + col, to[i]);
+    };
     double sum[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) sum[k] = 0;
     int cur = __builtin_amdgcn_readfirstlane(token);
     bool head = before == cur;
+    const auto add = [&](int i0, const T (&from)[kRows][W]) {
 #pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-        if (i < n) {
-            const int t = __builtin_amdgcn_readlane(token, i);
+        for (int i = 0; i < kRows; ++i) {
+            if (i0 + i >= n) break;
+            const int t = __builtin_amdgcn_readlane(token, i0 + i);
             if (t != cur) {
                 if (live) {
                     if (head) write_partial<T, W>(a, 2 * c, col, sum);
@@ -263,87 +323,122 @@ __global__ void __launch_bounds__(64) embedding_sum_kernel(SumArgs<T> a) {
                 for (int k = 0; k < W; ++k) sum[k] = 0;
             }
 #pragma unroll
-            for (int k = 0; k < W; ++k) sum[k] += static_cast<double>(x[i][k]);
+            for (int k = 0; k < W; ++k) sum[k] += static_cast<double>(from[i][k]);
         }
+    };
+    load(0, x[0]);
+    for (int i0 = 0; i0 < n; i0 += 2 * kRows) {  // (n <= 64 lanes: the lanes named below exist)
+        load(i0 + kRows, x[1]);
+        add(i0, x[0]);
+        if (i0 + 2 * kRows < n) load(i0 + 2 * kRows, x[0]);
+        add(i0 + kRows, x[1]);
     }
+    if (!head && after == cur && blockIdx.y == 0 && lane == 0) a.crossing[atomicAdd(&a.total[1], 1)] = static_cast<int32_t>(c);
     if (!live) return;
     if (head || after == cur) write_partial<T, W>(a, 2 * c + (head ? 0 : 1), col, sum);
     else write_gradient<T, W>(a, cur, col, sum);
 }
 
-// The run that begins in chunk c and goes on: its parts are partial[2 c + 1] and partial[2 j] of the following chunks j
-// that begin with its token.  Each wave adds a contiguous share of them, the waves' sums are added in order.
+// The sum of parts p0 .. p1 - 1 of the run that begins in chunk c.
 template <typename T, int W>
-__global__ void __launch_bounds__(64 * kJoinWaves) embedding_join_kernel(SumArgs<T> a) {
-    const int total = *a.total;
-    const int64_t c = blockIdx.x;
-    const int64_t next = (c + 1) * kRun;
-    if (next >= total) return;
-    const int token = a.token[next - 1];
-    if (a.token[next] != token) return;                            // no run crosses this border
-    if (c > 0 && a.token[c * kRun - 1] == token) return;           // it began in an earlier chunk
-    // the following chunks that begin with the token: a block of neighbours, found by doubling and halving
-    const int64_t chunks = (total + kRun - 1) / kRun;
-    int64_t lo = c + 1, hi = c + 2;                                // chunk lo begins with it
-    while (hi < chunks && a.token[hi * kRun] == token) {
-        lo = hi;
-        hi = c + 2 * (hi - c);
-    }
-    if (hi > chunks) hi = chunks;
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) / 2;
-        if (a.token[mid * kRun] == token) lo = mid;
-        else hi = mid;
-    }
-    const int64_t parts = lo - c + 1;                              // chunks c .. lo
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const int64_t col = (static_cast<int64_t>(blockIdx.y) * 64 + lane) * W;
-    __shared__ double waves[kJoinWaves][64 * W];
-    const int64_t per = (parts + kJoinWaves - 1) / kJoinWaves;
-    const int64_t p0 = wave * per, p1 = p0 + per < parts ? p0 + per : parts;
-    double sum[W];
+__device__ __forceinline__ void add_parts(const SumArgs<T> &a, int64_t c, int64_t p0, int64_t p1, int64_t col, double (&sum)[W]) {
 #pragma unroll
     for (int k = 0; k < W; ++k) sum[k] = 0;
-    if (col < a.dim) {
 #pragma unroll 8
-        for (int64_t p = p0; p < p1; ++p) {
-            const double *src = a.partial + (p == 0 ? 2 * c + 1 : 2 * (c + p)) * a.dim + col;
+    for (int64_t p = p0; p < p1; ++p) {
+        const double *src = a.partial + (p == 0 ? 2 * c + 1 : 2 * (c + p)) * a.dim + col;
 #pragma unroll
-            for (int k = 0; k < W; ++k) sum[k] += src[k];
-        }
+        for (int k = 0; k < W; ++k) sum[k] += src[k];
     }
+}
+
+// The run that begins in chunk c and goes on: its parts are partial[2 c + 1] and partial[2 j] of the following chunks j
+// that begin with its token.  A wave joins a run; one of many parts is left to the whole workgroup, whose waves add
+// contiguous shares, and the shares' sums are added in order.  The runs come in the order in which their chunks were listed,
+// which changes from call to call and no result with it.
+template <typename T, int W>
+__global__ void __launch_bounds__(64 * kJoinWaves) embedding_join_kernel(SumArgs<T> a) {
+    __shared__ double waves[kJoinWaves][64 * W];
+    __shared__ int64_t long_chunk[kJoinWaves], long_parts[kJoinWaves];
+    const int total = a.total[0], runs = a.total[1];
+    const int64_t chunks = (static_cast<int64_t>(total) + a.chunk - 1) / a.chunk;
+    const int lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int64_t col = (static_cast<int64_t>(blockIdx.y) * 64 + lane) * W;
+    double sum[W];
+    for (int r0 = blockIdx.x * kJoinWaves; r0 < runs; r0 += gridDim.x * kJoinWaves) {
+        int64_t parts = 0, c = 0;
+        if (r0 + wave < runs) {
+            c = a.crossing[r0 + wave];
+            const int token = a.token[(c + 1) * a.chunk];
+            // the following chunks that begin with the token: a block of neighbours, found by doubling and halving
+            int64_t lo = c + 1, hi = c + 2;  // chunk lo begins with it
+            while (hi < chunks && a.token[hi * a.chunk] == token) {
+                lo = hi;
+                hi = c + 2 * (hi - c);
+            }
+            if (hi > chunks) hi = chunks;
+            while (hi - lo > 1) {
+                const int64_t mid = (lo + hi) / 2;
+                if (a.token[mid * a.chunk] == token) lo = mid;
+                else hi = mid;
+            }
+            parts = lo - c + 1;  // chunks c .. lo
+            if (parts < kLongRun && col < a.dim) {
+                add_parts<T, W>(a, c, 0, parts, col, sum);
+                write_gradient<T, W>(a, token, col, sum);
+            }
+        }
+        if (lane == 0) {
+            long_chunk[wave] = c;
+            long_parts[wave] = parts >= kLongRun ? parts : 0;
+        }
+        __syncthreads();
+        for (int w = 0; w < kJoinWaves; ++w) {
+            const int64_t m = long_parts[w];
+            if (m == 0) continue;  // (the same for the whole workgroup)
+            const int64_t first = long_chunk[w];
+            const int64_t per = (m + kJoinWaves - 1) / kJoinWaves;
+            const int64_t p0 = wave * per, p1 = p0 + per < m ? p0 + per : m;
+            if (col < a.dim) add_parts<T, W>(a, first, p0, p1, col, sum);
 #pragma unroll
-    for (int k = 0; k < W; ++k) waves[wave][lane * W + k] = sum[k];
-    __syncthreads();
-    if (wave == 0 && col < a.dim) {
+            for (int k = 0; k < W; ++k) waves[wave][lane * W + k] = sum[k];
+            __syncthreads();
+            if (wave == 0 && col < a.dim) {
+                for (int v = 1; v < kJoinWaves; ++v)
 #pragma unroll
-        for (int w = 1; w < kJoinWaves; ++w)
-#pragma unroll
-            for (int k = 0; k < W; ++k) sum[k] += waves[w][lane * W + k];
-        write_gradient<T, W>(a, token, col, sum);
+                    for (int k = 0; k < W; ++k) sum[k] += waves[v][lane * W + k];
+                write_gradient<T, W>(a, a.token[(first + 1) * a.chunk], col, sum);
+            }
+            __syncthreads();
+        }
+        __syncthreads();  // the list of long runs is read
     }
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------
 struct BackwardPlan {
-    int bucket_log, tokens;
+    int bucket_log, tokens, chunk;
     int64_t chunks;
-    size_t position, token, total, partial, bytes;  // byte offsets into the workspace
+    size_t position, token, total, crossing, partial, bytes;  // byte offsets into the workspace
 };
 
-BackwardPlan plan_backward(int64_t count, int64_t vocab, int64_t dim) {
+BackwardPlan plan_backward(size_t item, int64_t count, int64_t vocab, int64_t dim) {
     BackwardPlan p{};
     // 256 buckets, a workgroup for each CU; more where a bucket's tokens would not fit the counters, fewer for tiny tables
     p.bucket_log = 8;
     while (p.bucket_log > 0 && (int64_t(1) << (p.bucket_log - 1)) >= vocab) --p.bucket_log;
     while ((vocab + (int64_t(1) << p.bucket_log) - 1) >> p.bucket_log > kOrderTokens) ++p.bucket_log;
     p.tokens = static_cast<int>((vocab + (int64_t(1) << p.bucket_log) - 1) >> p.bucket_log);
-    p.chunks = (count + kRun - 1) / kRun;
+    const int64_t slab = dim % (16 / static_cast<int64_t>(item)) == 0 ? 64 * (16 / static_cast<int64_t>(item)) : 64;
+    p.chunk = count / 64 * ((dim + slab - 1) / slab) >= 2048 ? 64 : 16;
+    p.chunks = (count + p.chunk - 1) / p.chunk;
     const auto up = [](size_t b) { return (b + 255) / 256 * 256; };
     p.position = 0;
     p.token = p.position + up(static_cast<size_t>(count) * 4);
     p.total = p.token + up(static_cast<size_t>(count) * 4);
-    p.partial = p.total + 256;
+    p.crossing = p.total + 256;
+    p.partial = p.crossing + up(static_cast<size_t>(p.chunks) * 4);
     p.bytes = p.partial + static_cast<size_t>(2 * p.chunks) * static_cast<size_t>(dim) * sizeof(double);
     return p;
 }
@@ -370,7 +465,7 @@ ttamd_status launch_forward(int64_t count, int64_t vocab, int64_t dim, const voi
 template <typename T>
 ttamd_status launch_backward(int64_t count, int64_t vocab, int64_t dim, const void *grad_out, const void *index, bool index64, double scale,
                              int accumulate, void *grad, void *workspace, hipStream_t st) {
-    const BackwardPlan p = plan_backward(count, vocab, dim);
+    const BackwardPlan p = plan_backward(sizeof(T), count, vocab, dim);
     char *ws = static_cast<char *>(workspace);
     OrderArgs o{index, count, vocab, dim, p.bucket_log, p.tokens, reinterpret_cast<int32_t *>(ws + p.position),
                 reinterpret_cast<int32_t *>(ws + p.token), reinterpret_cast<int32_t *>(ws + p.total), accumulate ? nullptr : grad};
@@ -380,15 +475,17 @@ ttamd_status launch_backward(int64_t count, int64_t vocab, int64_t dim, const vo
     TTAMD_HIP_CHECK(hipGetLastError());
     if (count == 0) return TTAMD_OK;
     const SumArgs<T> a{static_cast<const T *>(grad_out), static_cast<T *>(grad), reinterpret_cast<double *>(ws + p.partial), o.position,
-                       o.token, o.total, dim, scale, accumulate};
+                       o.token, o.total, reinterpret_cast<int32_t *>(ws + p.crossing), dim, p.chunk, scale, accumulate};
     const bool vec = dim % Row<T>::W == 0;
     const int w = vec ? Row<T>::W : 1;
     const dim3 grid(static_cast<unsigned>(p.chunks), static_cast<unsigned>((dim + 64 * w - 1) / (64 * w)));
     if (vec) embedding_sum_kernel<T, Row<T>::W><<<grid, 64, 0, st>>>(a);
     else embedding_sum_kernel<T, 1><<<grid, 64, 0, st>>>(a);
     TTAMD_HIP_CHECK(hipGetLastError());
-    if (vec) embedding_join_kernel<T, Row<T>::W><<<grid, 64 * kJoinWaves, 0, st>>>(a);
-    else embedding_join_kernel<T, 1><<<grid, 64 * kJoinWaves, 0, st>>>(a);
+    const int64_t groups = (p.chunks + kJoinWaves - 1) / kJoinWaves;
+    const dim3 join(static_cast<unsigned>(groups < 256 ? groups : 256), grid.y);
+    if (vec) embedding_join_kernel<T, Row<T>::W><<<join, 64 * kJoinWaves, 0, st>>>(a);
+    else embedding_join_kernel<T, 1><<<join, 64 * kJoinWaves, 0, st>>>(a);
     TTAMD_HIP_CHECK(hipGetLastError());
     return TTAMD_OK;
 }
@@ -453,7 +550,7 @@ ttamd_status ttamd_embedding_backward_workspace(ttamd_dtype dtype, int64_t count
         set_error("embedding_backward: bytes is NULL");
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
-    *bytes = plan_backward(count, vocab, dim).bytes;
+    *bytes = plan_backward(dtype_size(dtype), count, vocab, dim).bytes;
     return TTAMD_OK;
 }
 
