@@ -133,6 +133,22 @@ def test_embedding_gradient_runs(tt, pattern):
     assert np.array_equal(got.astype(np.float64), embedding_gradient(dy, ids, vocab, 1.0)[0])
 
 
+@pytest.mark.parametrize("dtype, count, vocab, dim", [(np.float32, 70000, 300, 520), (np.float32, 4097, 5, 2047), (np.float64, 40000, 30000, 421), (np.float32, 30000, 3, 64)])
+def test_embedding_gradient_of_many(tt, dtype, count, vocab, dim):
+    """Long lists: chunks of both lengths, tokens of thousands of positions, rows loaded past the caches; the forward too."""
+    r = rng_of(count, vocab, dim)
+    ids = ((vocab + 1) ** r.random(count) - 1).astype(np.int64)
+    dy = r.integers(-8, 9, (64, dim)).astype(dtype)[r.integers(0, 64, count)]  # whole numbers: the sums are exact
+    got = tt.embedding_backward(tt.Tensor.from_numpy(dy), tt.Tensor.from_numpy(ids), vocab).to_numpy()
+    want = np.zeros((vocab, dim))
+    order = np.argsort(ids, kind="stable")
+    starts = np.flatnonzero(np.r_[True, np.diff(ids[order]) > 0])
+    want[ids[order][starts]] = np.add.reduceat(dy[order].astype(np.float64), starts, axis=0)
+    assert np.array_equal(got.astype(np.float64), want)
+    table = r.integers(-100, 101, (vocab, dim)).astype(dtype)
+    assert np.array_equal(tt.embedding(tt.Tensor.from_numpy(ids), tt.Tensor.from_numpy(table), scale=0.5).to_numpy(), table[ids] * dtype(0.5))
+
+
 # ---- the gated pair ------------------------------------------------------------------------------------------------------
 
 
