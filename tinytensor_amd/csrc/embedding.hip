@@ -93,12 +93,12 @@ constexpr int kOrderTokens = 512;  // tokens of a bucket at most: their (token, 
 
 struct OrderArgs {
     const void *index;
-    int64_t count, vocab, dim;
+    int64_t count, vocab;
     int bucket_log;   // log2 of the number of buckets
     int tokens;       // tokens a bucket has room for: ceil(vocab / buckets)
     int32_t *position, *token;  // [count] in the order of the tokens
     int32_t *total;   // [0]: positions whose index lies in the table; [1], [2]: 0
-    void *grad;       // rows of tokens that no position has are set to zero here, or null: left alone
+    uint8_t *absent;  // [buckets][tokens] 1 for a token that no position has, or null
 };
 
 constexpr int kBatch = 8;  // loads of 64 indices in flight: with one at a time a scan of 60000 indices took 27 us of waiting
@@ -129,7 +129,7 @@ __device__ __forceinline__ void load_batch(const OrderArgs &a, int64_t i0, int64
     }
 }
 
-template <typename T, bool I64>
+template <bool I64>
 __global__ void __launch_bounds__(kOrderThreads) embedding_order_kernel(OrderArgs a) {
     extern __shared__ int32_t counters[];  // [tokens][kOrderWaves]
     __shared__ int32_t wave_sum[kOrderWaves], below_sum[kOrderWaves];
@@ -197,16 +197,11 @@ __global__ void __launch_bounds__(kOrderThreads) embedding_order_kernel(OrderArg
         at += n;
     }
     __syncthreads();
-    // Rows of tokens that nothing has: a token's run is empty when its first cell and the next token's begin at one place.
-    if (a.grad) {
+    // Which tokens nothing has: a token's run is empty when its first cell and the next token's begin at one place.
+    if (a.absent) {
         const int end = base + in_bucket;
-        for (int t = wave; t < a.tokens; t += kOrderWaves) {
-            const int64_t row = (static_cast<int64_t>(t) << a.bucket_log) + mine;
-            if (row >= a.vocab) break;
-            const int next = t + 1 < a.tokens ? counters[(t + 1) * kOrderWaves] : end;
-            if (counters[t * kOrderWaves] != next) continue;
-            zero_row(static_cast<T *>(a.grad) + row * a.dim, a.dim, lane);
-        }
+        for (int t = tid; t < a.tokens; t += kOrderThreads)
+            a.absent[static_cast<int64_t>(mine) * a.tokens + t] = counters[t * kOrderWaves] == (t + 1 < a.tokens ? counters[(t + 1) * kOrderWaves] : end);
     }
     __syncthreads();  // the cells are moved on from here
     const auto place = [&](bool in, int position, int token) {
@@ -251,6 +246,7 @@ __global__ void __launch_bounds__(kOrderThreads) embedding_order_kernel(OrderArg
 // over tens of thousands of rows keeps its last bits.
 // Chunks of 64 positions leave a quarter of the parts of chunks of 16, but a quarter of the waves: plan_backward.
 constexpr int kRows = 8;       // rows in flight ahead of those that are being added
+constexpr int kZeroRows = 16;  // table rows a wave looks after when it fills those of absent tokens
 constexpr int kJoinWaves = 16;
 constexpr int kLongRun = 24;   // parts from which a whole workgroup joins a run
 
@@ -268,6 +264,10 @@ struct SumArgs {
     int chunk;  // positions a chunk: 16 or 64
     double scale;
     int accumulate;
+    // rows of absent tokens, set to zero by the workgroups behind the chunks' (none when accumulating)
+    const uint8_t *absent;
+    int bucket_log, tokens;
+    int64_t vocab;
 };
 
 template <typename T, int W, bool NT = false>
@@ -316,10 +316,32 @@ __device__ __forceinline__ void write_partial(const SumArgs<T> &a, int64_t part,
     }
 }
 
+// A wave sets the rows of those among kZeroRows tokens to zero that nothing has (bucket by bucket, as `absent` lists them).
+// It rides in the sums' launch: on its own the fill (131 MB of a 32000 x 1024 f32 table) held up the sums for 17 us, here
+// its stores run under their loads.
+template <typename T>
+__device__ __forceinline__ void zero_absent(const SumArgs<T> &a, int64_t q0, int lane) {
+    const int64_t all = static_cast<int64_t>(a.tokens) << a.bucket_log;
+    const int64_t q = q0 + lane;
+    const bool here = lane < kZeroRows && q < all;
+    uint64_t left = __ballot(here && a.absent[here ? q : 0] != 0);
+    while (left) {
+        const int64_t at = q0 + __builtin_ctzll(left);
+        left &= left - 1;
+        const int64_t bucket = at / a.tokens;
+        const int64_t row = ((at - bucket * a.tokens) << a.bucket_log) + bucket;
+        if (row < a.vocab) zero_row(a.grad + row * a.dim, a.dim, lane);
+    }
+}
+
 template <typename T, int W, bool NT>
 __global__ void __launch_bounds__(64) embedding_sum_kernel(SumArgs<T> a) {
-    const int total = a.total[0];
     const int64_t c = blockIdx.x;
+    if (c >= a.list) {
+        zero_absent(a, ((c - a.list) * gridDim.y + blockIdx.y) * kZeroRows, static_cast<int>(threadIdx.x));
+        return;
+    }
+    const int total = a.total[0];
     const int64_t s0 = c * a.chunk;
     if (s0 >= total) return;
     const int n = total - s0 < a.chunk ? static_cast<int>(total - s0) : a.chunk;
@@ -449,7 +471,7 @@ __global__ void __launch_bounds__(64 * kJoinWaves) embedding_join_kernel(SumArgs
 struct BackwardPlan {
     int bucket_log, tokens, chunk;
     int64_t chunks;
-    size_t position, token, total, crossing, partial, bytes;  // byte offsets into the workspace
+    size_t position, token, total, crossing, absent, partial, bytes;  // byte offsets into the workspace
 };
 
 BackwardPlan plan_backward(size_t item, int64_t count, int64_t vocab, int64_t dim) {
@@ -467,7 +489,8 @@ BackwardPlan plan_backward(size_t item, int64_t count, int64_t vocab, int64_t di
     p.token = p.position + up(static_cast<size_t>(count) * 4);
     p.total = p.token + up(static_cast<size_t>(count) * 4);
     p.crossing = p.total + 256;
-    p.partial = p.crossing + up(static_cast<size_t>(p.chunks) * sizeof(int4));
+    p.absent = p.crossing + up(static_cast<size_t>(p.chunks) * sizeof(int4));
+    p.partial = p.absent + up(static_cast<size_t>(p.tokens) << p.bucket_log);
     p.bytes = p.partial + static_cast<size_t>(2 * p.chunks) * static_cast<size_t>(dim) * sizeof(double);
     return p;
 }
@@ -499,19 +522,23 @@ ttamd_status launch_backward(int64_t count, int64_t vocab, int64_t dim, const vo
                              int accumulate, void *grad, void *workspace, hipStream_t st) {
     const BackwardPlan p = plan_backward(sizeof(T), count, vocab, dim);
     char *ws = static_cast<char *>(workspace);
-    OrderArgs o{index, count, vocab, dim, p.bucket_log, p.tokens, reinterpret_cast<int32_t *>(ws + p.position),
-                reinterpret_cast<int32_t *>(ws + p.token), reinterpret_cast<int32_t *>(ws + p.total), accumulate ? nullptr : grad};
+    uint8_t *absent = accumulate ? nullptr : reinterpret_cast<uint8_t *>(ws + p.absent);
+    const OrderArgs o{index, count, vocab, p.bucket_log, p.tokens, reinterpret_cast<int32_t *>(ws + p.position),
+                      reinterpret_cast<int32_t *>(ws + p.token), reinterpret_cast<int32_t *>(ws + p.total), absent};
     const size_t lds = static_cast<size_t>(p.tokens) * kOrderWaves * sizeof(int32_t);
-    if (index64) embedding_order_kernel<T, true><<<1u << p.bucket_log, kOrderThreads, lds, st>>>(o);
-    else embedding_order_kernel<T, false><<<1u << p.bucket_log, kOrderThreads, lds, st>>>(o);
+    if (index64) embedding_order_kernel<true><<<1u << p.bucket_log, kOrderThreads, lds, st>>>(o);
+    else embedding_order_kernel<false><<<1u << p.bucket_log, kOrderThreads, lds, st>>>(o);
     TTAMD_HIP_CHECK(hipGetLastError());
-    if (count == 0) return TTAMD_OK;
+    if (count == 0 && accumulate) return TTAMD_OK;
     const SumArgs<T> a{static_cast<const T *>(grad_out), static_cast<T *>(grad), reinterpret_cast<double *>(ws + p.partial), o.position,
-                       o.token, o.total, reinterpret_cast<int4 *>(ws + p.crossing), p.chunks, dim, p.chunk, scale, accumulate};
+                       o.token, o.total, reinterpret_cast<int4 *>(ws + p.crossing), p.chunks, dim, p.chunk, scale, accumulate,
+                       absent, p.bucket_log, p.tokens, vocab};
     // (columns that two lanes write may not be added to what is there twice)
     const bool vec = accumulate ? dim % Row<T>::W == 0 : dim >= Row<T>::W;
     const int w = vec ? Row<T>::W : 1;
-    const dim3 grid(static_cast<unsigned>(p.chunks), static_cast<unsigned>((dim + 64 * w - 1) / (64 * w)));
+    const int64_t slabs = (dim + 64 * w - 1) / (64 * w);
+    const int64_t fill = accumulate ? 0 : ((static_cast<int64_t>(p.tokens) << p.bucket_log) + kZeroRows * slabs - 1) / (kZeroRows * slabs);
+    const dim3 grid(static_cast<unsigned>(p.chunks + fill), static_cast<unsigned>(slabs));
     // rows beyond half of the 256 MB Infinity Cache are loaded past it (65536 x 1024 f32: 216 -> 187 us in all; 8192 x 1024:
     // 44.3 without, 45.3 with)
     const bool beyond = static_cast<double>(count) * dim * sizeof(T) > 128.0 * (1 << 20);
@@ -519,6 +546,7 @@ ttamd_status launch_backward(int64_t count, int64_t vocab, int64_t dim, const vo
     else if (vec) embedding_sum_kernel<T, Row<T>::W, false><<<grid, 64, 0, st>>>(a);
     else embedding_sum_kernel<T, 1, false><<<grid, 64, 0, st>>>(a);
     TTAMD_HIP_CHECK(hipGetLastError());
+    if (count == 0) return TTAMD_OK;
     const int64_t groups = (p.chunks + kJoinWaves - 1) / kJoinWaves;
     const dim3 join(static_cast<unsigned>(groups < 256 ? groups : 256), grid.y);
     if (vec) embedding_join_kernel<T, Row<T>::W><<<join, 64 * kJoinWaves, 0, st>>>(a);
