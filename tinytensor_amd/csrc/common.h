@@ -79,6 +79,14 @@ inline FastDiv make_fastdiv(uint32_t d) {
 // buffers.  Growing allocates (hipMalloc, at least double the size); the outgrown buffer is kept until the process
 // ends, because kernels in flight and captured graphs may still refer to it.
 ttamd_status stream_scratch(int device, hipStream_t stream, size_t bytes, void **out);
+// While one lives, calls of its thread get their scratch from this memory instead (which must be enough for them): for an
+// entry point that runs others inside and promises that a call uses its caller's workspace alone.
+struct ScratchLoan {
+    ScratchLoan(void *memory, size_t bytes);
+    ~ScratchLoan();
+    ScratchLoan(const ScratchLoan &) = delete;
+    ScratchLoan &operator=(const ScratchLoan &) = delete;
+};
 // Whole-device synchronisations (ttamd_device_synchronize) of `device`: how many have started, how many have finished.
 // A use of shared memory that notes `started` at its launch is known to be over once `completed` exceeds that note.
 uint64_t device_sync_started(int device);

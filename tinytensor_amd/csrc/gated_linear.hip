@@ -5,47 +5,12 @@
 // No counterpart in the reference; it stands beside nn::Linear (nn/linear.cpp:42-50) followed by an activation.
 //
 // Bound: the matrix cores for many rows (4 and 8 rows x inner x hidden flop), HBM (the weights) for a few.
-#include "common.h"
+#include "gated.h"
+
+#include <initializer_list>
 
 namespace ttamd {
 namespace {
-
-constexpr int kSilu = 0, kGelu = 1, kRelu = 2, kSigmoid = 3;
-
-template <typename T>
-__device__ __forceinline__ T sigmoid(T g) {
-    if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-g));
-    else return 1.0 / (1.0 + exp(-g));
-}
-template <typename T>
-__device__ __forceinline__ T normal_cdf(T g) {
-    if constexpr (sizeof(T) == 4) return 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-    else return 0.5 * (1.0 + erf(g * 0.70710678118654752));
-}
-
-// act(g) and act'(g).  relu's derivative is where(g < 0, 0, 1), as TensorRelu::backward has it (autograd/unary_ops.cpp:568-573).
-template <typename T, int ACT>
-__device__ __forceinline__ T activate(T g) {
-    if constexpr (ACT == kRelu) return g > T(0) ? g : T(0);
-    if constexpr (ACT == kGelu) return g * normal_cdf(g);
-    const T s = sigmoid(g);
-    return ACT == kSigmoid ? s : g * s;
-}
-template <typename T, int ACT>
-__device__ __forceinline__ void activate(T g, T &value, T &slope) {
-    if constexpr (ACT == kRelu) {
-        value = g > T(0) ? g : T(0);
-        slope = g < T(0) ? T(0) : T(1);
-    } else if constexpr (ACT == kGelu) {
-        const T cdf = normal_cdf(g);
-        value = g * cdf;
-        slope = cdf + g * (T(0.3989422804014327) * (sizeof(T) == 4 ? static_cast<T>(expf(static_cast<float>(T(-0.5) * g * g))) : static_cast<T>(exp(T(-0.5) * g * g))));
-    } else {
-        const T s = sigmoid(g);
-        value = ACT == kSigmoid ? s : g * s;
-        slope = ACT == kSigmoid ? s * (T(1) - s) : s * (T(1) + g * (T(1) - s));
-    }
-}
 
 template <typename T>
 struct VecOf;
@@ -82,39 +47,151 @@ __global__ void __launch_bounds__(256) gated_product_kernel(const T *gate, const
     if (VEC && first < n - whole * W) out[whole * W + first] = activate<T, ACT>(gate[whole * W + first]) * up[whole * W + first];
 }
 
-// dg = dh * u * act'(g) and du = dh * act(g) over n elements.
-template <typename T, int ACT, bool VEC>
-__global__ void __launch_bounds__(256) gated_slope_kernel(const T *__restrict__ dh, const T *__restrict__ gate, const T *__restrict__ up,
-                                                          T *__restrict__ dg, T *__restrict__ du, int64_t n) {
+// What a pass needs before its products, in one launch: the gradients of the two products' results, and copies of operands
+// whose rows are no whole aligned vectors.
+//   dg = dh * u * act'(g), du = dh * act(g): dense dh, g, u [rows, hidden] in, rows of d_row elements out (a multiple of the
+//   vector; zeros behind the columns).  A workgroup has 64 vectors of columns and kSlopeRows rows, a wave every fourth of
+//   them; with `sums` it also leaves its rows' column sums, the bias gradients' parts: sums[row block][2][d_row].
+//   A copy: element (r, c) of any view to dst[r * dst_row + c], zeros from (rows, cols) to (dst_rows, dst_row).
+constexpr int kSlopeRows = 32, kCopies = 3;
+template <typename T>
+struct CopyJob {
+    const T *src;
+    int64_t s0, s1, rows, cols, dst_rows, dst_row;
+    T *dst;
+    int blocks;  // 64 x 64 tiles of dst; 0: nothing to copy
+};
+template <typename T>
+struct PrepareArgs {
+    const T *dh, *gate, *up;
+    T *dg, *du, *sums;
+    int64_t rows, d_row;
+    int hidden;
+    int slope_blocks, slope_blocks_n;  // workgroups of the gradients; of them side by side
+    CopyJob<T> copy[kCopies];
+};
+
+template <typename T>
+__device__ __forceinline__ void copy_tile(const CopyJob<T> &j, int block, T (*tile)[65]) {
+    const int tiles_n = static_cast<int>((j.dst_row + 63) / 64);
+    const int64_t r0 = static_cast<int64_t>(block / tiles_n) * 64, c0 = static_cast<int64_t>(block % tiles_n) * 64;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const bool by_rows = j.s0 < j.s1;  // lanes run along the rows (a transposed view) and the tile is turned in LDS
+#pragma unroll 4
+    for (int i = wave; i < 64; i += 4) {
+        const int64_t r = r0 + (by_rows ? lane : i), c = c0 + (by_rows ? i : lane);
+        const T v = r < j.rows && c < j.cols ? j.src[r * j.s0 + c * j.s1] : T(0);
+        if (by_rows) tile[i][lane] = v;
+        else if (r < j.dst_rows && c < j.dst_row) j.dst[r * j.dst_row + c] = v;
+    }
+    if (!by_rows) return;  // (the same for the whole workgroup)
+    __syncthreads();
+#pragma unroll 4
+    for (int i = wave; i < 64; i += 4)
+        if (r0 + i < j.dst_rows && c0 + lane < j.dst_row) j.dst[(r0 + i) * j.dst_row + c0 + lane] = tile[lane][i];
+}
+
+template <typename T, int ACT>
+__global__ void __launch_bounds__(256) gated_prepare_kernel(PrepareArgs<T> a) {
     using V = typename VecOf<T>::type;
-    constexpr int W = VEC ? VecOf<T>::W : 1;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, whole = n / W;
-    const auto one = [&](int64_t i) {
-        T value, slope;
-        activate<T, ACT>(gate[i], value, slope);
-        const T d = dh[i];
-        dg[i] = d * up[i] * slope;
-        du[i] = d * value;
-    };
-    for (int64_t i = first; i < whole; i += step) {
-        if constexpr (VEC) {
-            const V d = reinterpret_cast<const V *>(dh)[i], g = reinterpret_cast<const V *>(gate)[i], u = reinterpret_cast<const V *>(up)[i];
-            V a, b;
+    typedef T near_t __attribute__((ext_vector_type(VecOf<T>::W), aligned(sizeof(T))));
+    constexpr int W = VecOf<T>::W;
+    __shared__ T lds[64][65];
+    int block = blockIdx.x;
+    if (block >= a.slope_blocks) {
+        block -= a.slope_blocks;
+#pragma unroll
+        for (int k = 0; k < kCopies; ++k) {
+            if (block < a.copy[k].blocks) {
+                copy_tile(a.copy[k], block, lds);
+                return;
+            }
+            block -= a.copy[k].blocks;
+        }
+        return;
+    }
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int row_block = block / a.slope_blocks_n, col_block = block - row_block * a.slope_blocks_n;
+    const int64_t c = (static_cast<int64_t>(col_block) * 64 + lane) * W;
+    const int64_t r0 = static_cast<int64_t>(row_block) * kSlopeRows;
+    T sg[W], su[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) sg[k] = su[k] = T(0);
+    if (c < a.d_row) {
+        const bool whole = c + W <= a.hidden;
+#pragma unroll 2
+        for (int i = wave; i < kSlopeRows; i += 4) {
+            if (r0 + i >= a.rows) break;
+            const int64_t at = (r0 + i) * a.hidden + c;
+            T d[W], g[W], u[W];
+            if (whole) {
+                const near_t x = *reinterpret_cast<const near_t *>(a.dh + at), y = *reinterpret_cast<const near_t *>(a.gate + at),
+                             z = *reinterpret_cast<const near_t *>(a.up + at);
+#pragma unroll
+                for (int k = 0; k < W; ++k) {
+                    d[k] = x[k];
+                    g[k] = y[k];
+                    u[k] = z[k];
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < W; ++k) {
+                    const bool in = c + k < a.hidden;
+                    d[k] = in ? a.dh[at + k] : T(0);
+                    g[k] = in ? a.gate[at + k] : T(0);
+                    u[k] = in ? a.up[at + k] : T(0);
+                }
+            }
+            V x, y;
 #pragma unroll
             for (int k = 0; k < W; ++k) {
                 T value, slope;
                 activate<T, ACT>(g[k], value, slope);
-                a[k] = d[k] * u[k] * slope;
-                b[k] = d[k] * value;
+                x[k] = d[k] * u[k] * slope;
+                y[k] = d[k] * value;
+                sg[k] += x[k];
+                su[k] += y[k];
             }
-            reinterpret_cast<V *>(dg)[i] = a;
-            reinterpret_cast<V *>(du)[i] = b;
-        } else {
-            one(i);
+            *reinterpret_cast<V *>(a.dg + (r0 + i) * a.d_row + c) = x;
+            *reinterpret_cast<V *>(a.du + (r0 + i) * a.d_row + c) = y;
         }
     }
-    if (VEC && first < n - whole * W) one(whole * W + first);
+    if (!a.sums) return;
+    T *const part = &lds[0][0];  // [wave][2][W][64]
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+        part[((wave * 2 + 0) * W + k) * 64 + lane] = sg[k];
+        part[((wave * 2 + 1) * W + k) * 64 + lane] = su[k];
+    }
+    __syncthreads();
+    if (wave < 2 && c < a.d_row) {  // wave 0 adds up dg's columns, wave 1 du's
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            T v = T(0);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) v += part[((w * 2 + wave) * W + k) * 64 + lane];
+            a.sums[(static_cast<int64_t>(row_block) * 2 + wave) * a.d_row + c + k] = v;
+        }
+    }
+}
+
+// Bias gradients from the parts: dbg[c] = sum over b of sums[b][0][c], dbu of sums[b][1][c].  A wave adds every fourth row
+// block, the waves' sums are added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) gated_bias_kernel(const T *sums, int64_t blocks, int64_t d_row, int hidden, T *dbg, T *dbu) {
+    __shared__ T part[4][64];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    T *const out = blockIdx.y == 0 ? dbg : dbu;
+    if (!out) return;
+    T v = T(0);
+    if (c < hidden) {
+#pragma unroll 8
+        for (int64_t b = wave; b < blocks; b += 4) v += sums[(b * 2 + blockIdx.y) * d_row + c];
+    }
+    part[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0 && c < hidden) out[c] = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
 }
 
 template <typename F>
@@ -151,37 +228,70 @@ ttamd_status launch_product(int act, const void *gate, const void *up, void *out
     return TTAMD_OK;
 }
 
-template <typename T>
-ttamd_status launch_slope(int act, const void *dh, const void *gate, const void *up, void *dg, void *du, int64_t n, hipStream_t st) {
-    if (n == 0) return TTAMD_OK;
-    const bool vec = aligned16({dh, gate, up, dg, du});
-    const unsigned blocks = stream_blocks(vec ? n / VecOf<T>::W : n);
-    for_activation(act, [&]<int ACT>() {
-        const auto *d = static_cast<const T *>(dh), *g = static_cast<const T *>(gate), *u = static_cast<const T *>(up);
-        if (vec) gated_slope_kernel<T, ACT, true><<<blocks, 256, 0, st>>>(d, g, u, static_cast<T *>(dg), static_cast<T *>(du), n);
-        else gated_slope_kernel<T, ACT, false><<<blocks, 256, 0, st>>>(d, g, u, static_cast<T *>(dg), static_cast<T *>(du), n);
-    });
-    TTAMD_HIP_CHECK(hipGetLastError());
-    return TTAMD_OK;
-}
-
+// Sizes of a pass: padded row lengths and the workspace's layout (bytes).  What a call needs of it depends on its views;
+// the space covers every case.
 struct GatedSizes {
-    size_t item, hidden_matrix;  // bytes of an element; of a [rows, hidden] matrix, rounded up to 256
+    size_t item;
+    int64_t vec;                   // elements of 16 bytes
+    int64_t inner_row, hidden_row; // inner and hidden rounded up to whole vectors
+    size_t first, second;          // forward: g and u; backward: dg and du, rows of hidden_row elements
+    size_t sums;                   // backward: the bias gradients' parts
+    size_t x, wg, wu;              // copies of operands
+    size_t parts;                  // backward: parts of reductions that the tile kernel cuts
+    GatedSplit split;
+    size_t scratch, scratch_bytes; // lent to separate products: partial tiles of split reductions
+    size_t bytes;
 };
 
-ttamd_status check_gated(const char *what, ttamd_dtype dtype, int64_t rows, int64_t inner, int64_t hidden, GatedSizes *out) {
+GatedSizes sizes_of(ttamd_dtype dtype, int64_t rows, int64_t inner, int64_t hidden, bool backward) {
+    GatedSizes z{};
+    z.item = dtype_size(dtype);
+    z.vec = 16 / static_cast<int64_t>(z.item);
+    z.inner_row = (inner + z.vec - 1) / z.vec * z.vec;
+    z.hidden_row = (hidden + z.vec - 1) / z.vec * z.vec;
+    size_t at = 0;
+    const auto take = [&](int64_t elements) {
+        const size_t here = at;
+        at += (static_cast<size_t>(elements) * z.item + 255) / 256 * 256;
+        return here;
+    };
+    z.first = take(rows * z.hidden_row);
+    z.second = take(rows * z.hidden_row);
+    z.sums = take(backward ? (rows + kSlopeRows - 1) / kSlopeRows * 2 * z.hidden_row : 0);
+    z.x = take(rows * z.inner_row);
+    z.wg = take(z.inner_row * z.hidden_row);
+    z.wu = take(z.inner_row * z.hidden_row);
+    // (the last stretch serves the tile kernel or the separate products)
+    z.parts = z.scratch = at;
+    size_t parts = 0;
+    if (backward && rows > 0) {
+        z.split = plan_gated_split(z.item, rows, inner, hidden, z.hidden_row);
+        parts = static_cast<size_t>(z.split.x_parts + z.split.w_parts + z.split.b_parts) * z.item;
+    }
+    // A product of fewer than 128 tiles of 64 x 64 may be split into up to 64 reductions, 32 MiB of partial tiles at most.
+    const auto split = [&](int64_t m, int64_t n) {
+        if ((m + 63) / 64 * ((n + 63) / 64) >= 128) return size_t(0);
+        const size_t b = static_cast<size_t>(64 * m * n) * z.item;
+        return b < (size_t(32) << 20) ? b : size_t(32) << 20;
+    };
+    const size_t a = backward ? split(rows, inner) : split(rows, hidden), b = backward ? split(inner, hidden) : 0;
+    z.scratch_bytes = a > b ? a : b;
+    z.bytes = at + (z.scratch_bytes > parts ? z.scratch_bytes : parts);
+    return z;
+}
+
+ttamd_status check_gated(const char *what, ttamd_dtype dtype, int64_t rows, int64_t inner, int64_t hidden) {
     if (dtype != TTAMD_F32 && dtype != TTAMD_F64) {
         set_error("%s: floating point dtypes only", what);
         return TTAMD_ERR_UNSUPPORTED_DTYPE;
     }
-    constexpr int64_t most = 0x7fffffffLL;
-    if (rows < 0 || inner < 1 || hidden < 1 || rows > most || inner > most || hidden > most) {
-        set_error("%s: rows %lld, inner %lld, hidden %lld: rows from 0, the others from 1, all below 2^31", what, static_cast<long long>(rows),
-                  static_cast<long long>(inner), static_cast<long long>(hidden));
+    constexpr int64_t most = int64_t(1) << 30;  // (and below 2^40 elements a matrix: every size in bytes fits 64 bits)
+    if (rows < 0 || inner < 1 || hidden < 1 || rows > most || inner > most || hidden > most || rows * inner > most << 10 ||
+        rows * hidden > most << 10 || inner * hidden > most << 10) {
+        set_error("%s: rows %lld, inner %lld, hidden %lld: rows from 0, the others from 1, up to 2^30 each and 2^40 elements a matrix", what,
+                  static_cast<long long>(rows), static_cast<long long>(inner), static_cast<long long>(hidden));
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
-    out->item = dtype_size(dtype);
-    out->hidden_matrix = (static_cast<size_t>(rows) * static_cast<size_t>(hidden) * out->item + 255) / 256 * 256;
     return TTAMD_OK;
 }
 
@@ -203,8 +313,178 @@ ttamd_status check_view(const char *what, const char *name, const ttamd_view2 *v
     return TTAMD_OK;
 }
 
-ttamd_view3 lift(const ttamd_view2 &v) { return {v.data, v.offset, {0, v.stride[0], v.stride[1]}}; }
-ttamd_view3 lift_transposed(const ttamd_view2 &v) { return {v.data, v.offset, {0, v.stride[1], v.stride[0]}}; }
+// A matrix as the kernels take it: the caller's own, or its copy in the workspace.
+template <typename T>
+struct Operand {
+    const T *data;
+    int64_t s0, s1;
+};
+
+template <typename T>
+Operand<T> operand_of(const ttamd_view2 &v) {
+    return {static_cast<const T *>(v.data) + v.offset, v.stride[0], v.stride[1]};
+}
+// Rows of whole 16-byte vectors at aligned addresses, in order.
+template <typename T>
+bool row_vectors(const Operand<T> &m, int64_t cols) {
+    constexpr int64_t W = VecOf<T>::W;
+    return m.s1 == 1 && m.s0 % W == 0 && cols % W == 0 && !misaligned(m.data, 16);
+}
+// The same in either direction: what the separate products read with 16-byte loads.
+template <typename T>
+bool any_vectors(const Operand<T> &m) {
+    constexpr int64_t W = VecOf<T>::W;
+    return !misaligned(m.data, 16) && ((m.s1 == 1 && m.s0 % W == 0) || (m.s0 == 1 && m.s1 % W == 0));
+}
+template <typename T>
+CopyJob<T> copy_job(Operand<T> &m, int64_t rows, int64_t cols, int64_t dst_rows, int64_t dst_row, void *dst) {
+    const int64_t blocks = (dst_rows + 63) / 64 * ((dst_row + 63) / 64);
+    const CopyJob<T> j{m.data, m.s0, m.s1, rows, cols, dst_rows, dst_row, static_cast<T *>(dst), static_cast<int>(blocks)};
+    m = {static_cast<const T *>(dst), dst_row, 1};
+    return j;
+}
+template <typename T>
+ttamd_view3 view_of(const Operand<T> &m, bool transposed = false) {
+    return {m.data, 0, {0, transposed ? m.s1 : m.s0, transposed ? m.s0 : m.s1}};
+}
+
+template <typename T>
+ttamd_status launch_prepare(int act, const PrepareArgs<T> &a, hipStream_t st) {
+    int64_t blocks = a.slope_blocks;
+    for (const CopyJob<T> &j : a.copy) blocks += j.blocks;
+    if (blocks == 0) return TTAMD_OK;
+    for_activation(act, [&]<int ACT>() { gated_prepare_kernel<T, ACT><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a); });
+    TTAMD_HIP_CHECK(hipGetLastError());
+    return TTAMD_OK;
+}
+
+// Sizes whose byte offsets inside a tile's operands and results fit the tile kernels' 32 bits.
+bool tiles_reach(const GatedSizes &z, int64_t rows, int64_t inner, int64_t hidden, const int64_t (&strides)[3]) {
+    const int64_t most = 0x7fffffffLL / static_cast<int64_t>(z.item);
+    for (int64_t s : strides)
+        if ((inner + 256) * s > most || (rows + 256) * s > most) return false;
+    return rows * z.hidden_row < most && rows * z.inner_row < most && z.inner_row * z.hidden_row < most && 256 * hidden < most && 256 * inner < most;
+}
+
+struct Pass {
+    int device, act;
+    ttamd_dtype dtype;
+    int64_t rows, inner, hidden;
+    ttamd_view2 x, wg, wu;
+    char *ws;
+    void *stream;
+};
+
+template <typename T>
+ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, void *out, void *gate, void *up) {
+    hipStream_t st = static_cast<hipStream_t>(p.stream);
+    const int64_t rows = p.rows, inner = p.inner, hidden = p.hidden;
+    const GatedSizes z = sizes_of(p.dtype, rows, inner, hidden, false);
+    Operand<T> x = operand_of<T>(p.x), wg = operand_of<T>(p.wg), wu = operand_of<T>(p.wu);
+    PrepareArgs<T> prep{};
+    // One grid of both products (gated_tiles.hip), unless it would be few tiles of a long reduction, which the separate
+    // products cut (128 x 1024 x 2048 f32: 64 tiles, 38 us against 28 in three launches; 256 x 1024 x 4096: 256 tiles, 38
+    // against 49).
+    const int64_t tiles = (rows + 63) / 64 * ((hidden + (z.item == 4 ? 63 : 31)) / (z.item == 4 ? 64 : 32));
+    const bool few = inner > 256 && (rows <= 32 || tiles < 96);
+    if (!few && tiles_reach(z, rows, inner, hidden, {x.s0, wg.s0, wu.s0})) {
+        const bool own = inner % z.vec == 0;  // (x's padding meets rows of zeros in the weights' copies)
+        if (!row_vectors(x, inner)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
+        if (!own || !row_vectors(wg, hidden)) prep.copy[1] = copy_job(wg, inner, hidden, z.inner_row, z.hidden_row, p.ws + z.wg);
+        if (!own || !row_vectors(wu, hidden)) prep.copy[2] = copy_job(wu, inner, hidden, z.inner_row, z.hidden_row, p.ws + z.wu);
+        if (ttamd_status s = launch_prepare(p.act, prep, st)) return s;
+        const GatedForward<T> a{x.data, wg.data, wu.data, x.s0, wg.s0, wu.s0, static_cast<int>(rows), static_cast<int>(z.inner_row),
+                                static_cast<int>(z.hidden_row), static_cast<int>(hidden), p.act, static_cast<const T *>(gate_bias),
+                                static_cast<const T *>(up_bias), static_cast<T *>(out), static_cast<T *>(gate), static_cast<T *>(up)};
+        return launch_gated_forward_tiles<T>(a, p.device, st);
+    }
+    if (rows >= 16) {
+        if (!any_vectors(x)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
+        if (!any_vectors(wg)) prep.copy[1] = copy_job(wg, inner, hidden, inner, z.hidden_row, p.ws + z.wg);
+        if (!any_vectors(wu)) prep.copy[2] = copy_job(wu, inner, hidden, inner, z.hidden_row, p.ws + z.wu);
+        if (ttamd_status s = launch_prepare(p.act, prep, st)) return s;
+    }
+    const ScratchLoan loan(p.ws + z.scratch, z.scratch_bytes);
+    void *g = gate ? gate : p.ws + z.first, *u = gate ? up : p.ws + z.second;
+    const int R = static_cast<int>(rows), K = static_cast<int>(inner), H = static_cast<int>(hidden);
+    const ttamd_view3 xv = view_of(x), gv = view_of(wg), uv = view_of(wu);
+    ttamd_epilogue eg{}, eu{};
+    eg.bias = gate_bias;
+    eg.bias_mode = gate_bias ? 1 : 0;
+    eu.bias = up_bias;
+    eu.bias_mode = up_bias ? 1 : 0;
+    if (ttamd_status s = ttamd_batched_matmul(p.device, p.dtype, 1, R, K, H, &xv, &gv, g, &eg, p.stream)) return s;
+    if (ttamd_status s = ttamd_batched_matmul(p.device, p.dtype, 1, R, K, H, &xv, &uv, u, &eu, p.stream)) return s;
+    return launch_product<T>(p.act, g, u, out, rows * hidden, st);
+}
+
+template <typename T>
+ttamd_status backward(const Pass &p, const void *grad_out, const void *gate, const void *up, void *dx, void *dwg, void *dwu, void *dbg, void *dbu) {
+    hipStream_t st = static_cast<hipStream_t>(p.stream);
+    const int64_t rows = p.rows, inner = p.inner, hidden = p.hidden;
+    const GatedSizes z = sizes_of(p.dtype, rows, inner, hidden, true);
+    Operand<T> x = operand_of<T>(p.x), wg = operand_of<T>(p.wg), wu = operand_of<T>(p.wu);
+    PrepareArgs<T> prep{};
+    T *const dg = reinterpret_cast<T *>(p.ws + z.first), *const du = reinterpret_cast<T *>(p.ws + z.second);
+    if (rows > 0) {
+        prep.dh = static_cast<const T *>(grad_out);
+        prep.gate = static_cast<const T *>(gate);
+        prep.up = static_cast<const T *>(up);
+        prep.dg = dg;
+        prep.du = du;
+        prep.rows = rows;
+        prep.d_row = z.hidden_row;
+        prep.hidden = static_cast<int>(hidden);
+        prep.slope_blocks_n = static_cast<int>((z.hidden_row / z.vec + 63) / 64);
+        prep.slope_blocks = static_cast<int>((rows + kSlopeRows - 1) / kSlopeRows) * prep.slope_blocks_n;
+    }
+    // One grid of all three products' 64 x 64 tiles; separate products with tiles up to 256 x 256 from 64 Gflop on
+    // (4096 x 1024 x 4096 f32: 1110 us against 1035; 4096 x 1024 x 1024: 275 against 285).
+    const bool huge = 8.0 * rows * inner * hidden > 64e9;
+    if (!huge && rows > 0 && tiles_reach(z, rows, inner, hidden, {x.s0, wg.s0, wu.s0})) {
+        if (!row_vectors(x, inner)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
+        if (!row_vectors(wg, hidden)) prep.copy[1] = copy_job(wg, inner, hidden, inner, z.hidden_row, p.ws + z.wg);
+        if (!row_vectors(wu, hidden)) prep.copy[2] = copy_job(wu, inner, hidden, inner, z.hidden_row, p.ws + z.wu);
+        if (ttamd_status s = launch_prepare(p.act, prep, st)) return s;
+        const GatedBackward<T> a{x.data, wg.data, wu.data, x.s0, wg.s0, wu.s0, dg, du, z.hidden_row, static_cast<int>(rows), static_cast<int>(inner),
+                                 static_cast<int>(z.inner_row), static_cast<int>(hidden), static_cast<int>(z.hidden_row), static_cast<T *>(dx),
+                                 static_cast<T *>(dwg), static_cast<T *>(dwu), static_cast<T *>(dbg), static_cast<T *>(dbu),
+                                 z.split, reinterpret_cast<T *>(p.ws + z.parts), reinterpret_cast<T *>(p.ws + z.parts) + z.split.x_parts,
+                                 reinterpret_cast<T *>(p.ws + z.parts) + z.split.x_parts + z.split.w_parts};
+        return launch_gated_backward_tiles<T>(a, p.device, st);
+    }
+    if (rows >= 16) {
+        if (!any_vectors(x)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
+        if (!any_vectors(wg)) prep.copy[1] = copy_job(wg, inner, hidden, inner, z.hidden_row, p.ws + z.wg);
+        if (!any_vectors(wu)) prep.copy[2] = copy_job(wu, inner, hidden, inner, z.hidden_row, p.ws + z.wu);
+    }
+    T *const sums = reinterpret_cast<T *>(p.ws + z.sums);
+    if (dbg || dbu) prep.sums = sums;
+    if (ttamd_status s = launch_prepare(p.act, prep, st)) return s;
+    if (dbg || dbu) {
+        gated_bias_kernel<T><<<dim3(static_cast<unsigned>((hidden + 63) / 64), 2), 256, 0, st>>>(
+            sums, (rows + kSlopeRows - 1) / kSlopeRows, z.hidden_row, static_cast<int>(hidden), static_cast<T *>(dbg), static_cast<T *>(dbu));
+        TTAMD_HIP_CHECK(hipGetLastError());
+    }
+    const ScratchLoan loan(p.ws + z.scratch, z.scratch_bytes);
+    const int R = static_cast<int>(rows), K = static_cast<int>(inner), H = static_cast<int>(hidden);
+    const ttamd_view3 gv{dg, 0, {0, z.hidden_row, 1}}, uv{du, 0, {0, z.hidden_row, 1}};
+    const ttamd_view3 xt = view_of(x, true), wgt = view_of(wg, true), wut = view_of(wu, true);
+    ttamd_epilogue add{};
+    add.accumulate = 1;
+    if (rows > 0) {
+        if (ttamd_status s = ttamd_batched_matmul(p.device, p.dtype, 1, R, H, K, &gv, &wgt, dx, nullptr, p.stream)) return s;
+        if (ttamd_status s = ttamd_batched_matmul(p.device, p.dtype, 1, R, H, K, &uv, &wut, dx, &add, p.stream)) return s;
+    }
+    if (ttamd_status s = ttamd_batched_matmul(p.device, p.dtype, 1, K, R, H, &xt, &gv, dwg, nullptr, p.stream)) return s;
+    return ttamd_batched_matmul(p.device, p.dtype, 1, K, R, H, &xt, &uv, dwu, nullptr, p.stream);
+}
+
+ttamd_status check_workspace(const char *what, const void *workspace, size_t given, size_t needed) {
+    if (workspace && !misaligned(workspace, 16) && given >= needed) return TTAMD_OK;
+    set_error("%s: workspace %p of %zu bytes: %zu are needed, aligned to 16", what, workspace, given, needed);
+    return TTAMD_ERR_INVALID_ARGUMENT;
+}
 
 }  // namespace
 }  // namespace ttamd
@@ -214,13 +494,12 @@ using namespace ttamd;
 extern "C" {
 
 ttamd_status ttamd_gated_linear_workspace(ttamd_dtype dtype, int64_t rows, int64_t inner, int64_t hidden, int backward, size_t *bytes) {
-    GatedSizes z;
-    if (ttamd_status s = check_gated("gated_linear", dtype, rows, inner, hidden, &z)) return s;
+    if (ttamd_status s = check_gated("gated_linear", dtype, rows, inner, hidden)) return s;
     if (!bytes) {
         set_error("gated_linear: bytes is NULL");
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
-    *bytes = 2 * z.hidden_matrix;  // g and u, or dg and du
+    *bytes = rows > 0 ? sizes_of(dtype, rows, inner, hidden, backward != 0).bytes : 0;
     return TTAMD_OK;
 }
 
@@ -229,14 +508,14 @@ ttamd_status ttamd_gated_linear_forward(int device, ttamd_dtype dtype, int activ
                                         const void *gate_bias, const void *up_bias, void *out, void *gate_out, void *up_out, void *workspace,
                                         size_t workspace_bytes, void *stream) {
     const char *const what = "gated_linear";
-    GatedSizes z;
-    if (ttamd_status s = check_gated(what, dtype, rows, inner, hidden, &z)) return s;
+    if (ttamd_status s = check_gated(what, dtype, rows, inner, hidden)) return s;
     if (ttamd_status s = check_activation(what, activation)) return s;
+    const size_t item = dtype_size(dtype);
     const bool work = rows > 0;
-    if (ttamd_status s = check_view(what, "input", input, z.item, work)) return s;
-    if (ttamd_status s = check_view(what, "gate weight", gate_weight, z.item, work)) return s;
-    if (ttamd_status s = check_view(what, "up weight", up_weight, z.item, work)) return s;
-    if (work && (!out || (!workspace && !(gate_out && up_out)))) {
+    if (ttamd_status s = check_view(what, "input", input, item, work)) return s;
+    if (ttamd_status s = check_view(what, "gate weight", gate_weight, item, work)) return s;
+    if (ttamd_status s = check_view(what, "up weight", up_weight, item, work)) return s;
+    if (work && !out) {
         set_error("%s: NULL data pointer", what);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
@@ -244,31 +523,18 @@ ttamd_status ttamd_gated_linear_forward(int device, ttamd_dtype dtype, int activ
         set_error("%s: gate_out and up_out are given together or not at all", what);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
-    if (misaligned(out, z.item) || misaligned(gate_out, z.item) || misaligned(up_out, z.item) || misaligned(gate_bias, z.item) ||
-        misaligned(up_bias, z.item) || misaligned(workspace, 16)) {
-        set_error("%s: pointers must be aligned to the element size, the workspace to 16 bytes", what);
-        return TTAMD_ERR_INVALID_ARGUMENT;
-    }
-    if (workspace_bytes < 2 * z.hidden_matrix && !gate_out) {
-        set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, 2 * z.hidden_matrix);
-        return TTAMD_ERR_INVALID_ARGUMENT;
-    }
+    for (const void *q : {static_cast<const void *>(out), static_cast<const void *>(gate_out), static_cast<const void *>(up_out), gate_bias, up_bias})
+        if (misaligned(q, item)) {
+            set_error("%s: pointers must be aligned to the element size", what);
+            return TTAMD_ERR_INVALID_ARGUMENT;
+        }
+    if (work)
+        if (ttamd_status s = check_workspace(what, workspace, workspace_bytes, sizes_of(dtype, rows, inner, hidden, false).bytes)) return s;
     if (ttamd_status s = use_device(device)) return s;
     if (!work) return TTAMD_OK;
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    void *g = gate_out ? gate_out : workspace;
-    void *u = up_out ? up_out : static_cast<char *>(workspace) + z.hidden_matrix;
-    const int R = static_cast<int>(rows), K = static_cast<int>(inner), H = static_cast<int>(hidden);
-    const ttamd_view3 x = lift(*input), wg = lift(*gate_weight), wu = lift(*up_weight);
-    ttamd_epilogue eg{}, eu{};
-    eg.bias = gate_bias;
-    eg.bias_mode = gate_bias ? 1 : 0;
-    eu.bias = up_bias;
-    eu.bias_mode = up_bias ? 1 : 0;
-    if (ttamd_status s = ttamd_batched_matmul(device, dtype, 1, R, K, H, &x, &wg, g, &eg, stream)) return s;
-    if (ttamd_status s = ttamd_batched_matmul(device, dtype, 1, R, K, H, &x, &wu, u, &eu, stream)) return s;
-    const int64_t n = rows * hidden;
-    return dtype == TTAMD_F32 ? launch_product<float>(activation, g, u, out, n, st) : launch_product<double>(activation, g, u, out, n, st);
+    const Pass p{device, activation, dtype, rows, inner, hidden, *input, *gate_weight, *up_weight, static_cast<char *>(workspace), stream};
+    return dtype == TTAMD_F32 ? forward<float>(p, gate_bias, up_bias, out, gate_out, up_out)
+                              : forward<double>(p, gate_bias, up_bias, out, gate_out, up_out);
 }
 
 ttamd_status ttamd_gated_linear_backward(int device, ttamd_dtype dtype, int activation, int64_t rows, int64_t inner, int64_t hidden,
@@ -277,48 +543,29 @@ ttamd_status ttamd_gated_linear_backward(int device, ttamd_dtype dtype, int acti
                                          void *grad_gate_weight, void *grad_up_weight, void *grad_gate_bias, void *grad_up_bias,
                                          void *workspace, size_t workspace_bytes, void *stream) {
     const char *const what = "gated_linear_backward";
-    GatedSizes z;
-    if (ttamd_status s = check_gated(what, dtype, rows, inner, hidden, &z)) return s;
+    if (ttamd_status s = check_gated(what, dtype, rows, inner, hidden)) return s;
     if (ttamd_status s = check_activation(what, activation)) return s;
+    const size_t item = dtype_size(dtype);
     const bool work = rows > 0;
-    if (ttamd_status s = check_view(what, "input", input, z.item, work)) return s;
-    if (ttamd_status s = check_view(what, "gate weight", gate_weight, z.item, work)) return s;
-    if (ttamd_status s = check_view(what, "up weight", up_weight, z.item, work)) return s;
-    if (!grad_gate_weight || !grad_up_weight || (work && (!grad_out || !gate || !up || !grad_input || !workspace))) {
+    if (ttamd_status s = check_view(what, "input", input, item, work)) return s;
+    if (ttamd_status s = check_view(what, "gate weight", gate_weight, item, work)) return s;
+    if (ttamd_status s = check_view(what, "up weight", up_weight, item, work)) return s;
+    if (!grad_gate_weight || !grad_up_weight || (work && (!grad_out || !gate || !up || !grad_input))) {
         set_error("%s: NULL data pointer", what);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
-    for (const void *p : {grad_out, gate, up, static_cast<const void *>(grad_input), static_cast<const void *>(grad_gate_weight),
+    for (const void *q : {grad_out, gate, up, static_cast<const void *>(grad_input), static_cast<const void *>(grad_gate_weight),
                           static_cast<const void *>(grad_up_weight), static_cast<const void *>(grad_gate_bias), static_cast<const void *>(grad_up_bias)})
-        if (misaligned(p, z.item)) {
+        if (misaligned(q, item)) {
             set_error("%s: pointers must be aligned to the element size", what);
             return TTAMD_ERR_INVALID_ARGUMENT;
         }
-    if (work && (misaligned(workspace, 16) || workspace_bytes < 2 * z.hidden_matrix)) {
-        set_error("%s: workspace of %zu bytes, %zu needed, aligned to 16", what, workspace_bytes, 2 * z.hidden_matrix);
-        return TTAMD_ERR_INVALID_ARGUMENT;
-    }
+    if (work)
+        if (ttamd_status s = check_workspace(what, workspace, workspace_bytes, sizes_of(dtype, rows, inner, hidden, true).bytes)) return s;
     if (ttamd_status s = use_device(device)) return s;
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    const int R = static_cast<int>(rows), K = static_cast<int>(inner), H = static_cast<int>(hidden);
-    void *dg = workspace, *du = static_cast<char *>(workspace) + z.hidden_matrix;
-    const int64_t n = rows * hidden;
-    if (ttamd_status s = dtype == TTAMD_F32 ? launch_slope<float>(activation, grad_out, gate, up, dg, du, n, st)
-                                            : launch_slope<double>(activation, grad_out, gate, up, dg, du, n, st))
-        return s;
-    // dx = dg . Wg^T, then += du . Wu^T; each weight's gradient with its bias gradient (no rows: zeros)
-    const ttamd_view3 vg{dg, 0, {n, hidden, 1}}, vu{du, 0, {n, hidden, 1}};
-    const ttamd_view3 xt = lift_transposed(*input), wgt = lift_transposed(*gate_weight), wut = lift_transposed(*up_weight);
-    ttamd_epilogue add{}, eg{}, eu{};
-    add.accumulate = 1;
-    eg.rhs_colsum_out = grad_gate_bias;
-    eu.rhs_colsum_out = grad_up_bias;
-    if (work) {
-        if (ttamd_status s = ttamd_batched_matmul(device, dtype, 1, R, H, K, &vg, &wgt, grad_input, nullptr, stream)) return s;
-        if (ttamd_status s = ttamd_batched_matmul(device, dtype, 1, R, H, K, &vu, &wut, grad_input, &add, stream)) return s;
-    }
-    if (ttamd_status s = ttamd_batched_matmul(device, dtype, 1, K, R, H, &xt, &vg, grad_gate_weight, &eg, stream)) return s;
-    return ttamd_batched_matmul(device, dtype, 1, K, R, H, &xt, &vu, grad_up_weight, &eu, stream);
+    const Pass p{device, activation, dtype, rows, inner, hidden, *input, *gate_weight, *up_weight, static_cast<char *>(workspace), stream};
+    return dtype == TTAMD_F32 ? backward<float>(p, grad_out, gate, up, grad_input, grad_gate_weight, grad_up_weight, grad_gate_bias, grad_up_bias)
+                              : backward<double>(p, grad_out, gate, up, grad_input, grad_gate_weight, grad_up_weight, grad_gate_bias, grad_up_bias);
 }
 
 }  // extern "C"
