@@ -302,6 +302,46 @@ def test_gated_linear_views(tt, dtype, rows, form):
     check_gated(tt, dtype, "silu", x, wg, wu, bg, None, tx, twg, twu, dh=dh)
 
 
+def test_gated_linear_beyond_32_bit_offsets(tt):
+    """Matrices of more than 2^31 bytes, and rows that lie that far apart: whole numbers, so every sum is exact."""
+    r = rng_of(31)
+    T = tt.Tensor
+    rows, inner, hidden = 300, 4, 1 << 20
+    x, wg, wu = r.integers(-2, 3, (rows, inner)).astype(np.float64), *(r.integers(-2, 3, (inner, hidden)).astype(np.float64) for _ in range(2))
+    dh = T.from_numpy(r.integers(-1, 2, (1, hidden)).astype(np.float64)).expand((rows, hidden))
+    tx, twg, twu = (T.from_numpy(a) for a in (x, wg, wu))
+    h, g, u = tt.gated_linear(tx, twg, twu, activation="relu", save=True)
+    part = lambda t, c: T(t.storage, t.dtype, (rows, 1000), (hidden, 1), c).contiguous().to_numpy()  # noqa: E731
+    for c in (0, 1 << 19, hidden - 1000):
+        wantg, wantu = x @ wg[:, c:c + 1000], x @ wu[:, c:c + 1000]
+        assert np.array_equal(part(g, c), wantg) and np.array_equal(part(u, c), wantu) and np.array_equal(part(h, c), np.maximum(wantg, 0) * wantu)
+    del h
+    dx, dwg, dwu, dbg, dbu = (t.to_numpy() for t in tt.gated_linear_backward(dh, tx, twg, twu, g, u, activation="relu"))
+    d, sum_dx = T(dh.storage, dh.dtype, (hidden,), (1,), 0).to_numpy(), np.zeros((rows, inner))
+    for c in range(0, hidden, 1 << 16):
+        s = slice(c, c + (1 << 16))
+        wantg, wantu = x @ wg[:, s], x @ wu[:, s]
+        pg, pu = d[s] * wantu * (wantg >= 0), d[s] * np.maximum(wantg, 0)
+        assert np.array_equal(dwg[:, s], x.T @ pg) and np.array_equal(dwu[:, s], x.T @ pu)
+        assert np.array_equal(dbg[s], pg.sum(0)) and np.array_equal(dbu[s], pu.sum(0))
+        sum_dx += pg @ wg[:, s].T + pu @ wu[:, s].T
+    assert np.array_equal(dx, sum_dx)
+    del g, u
+    # two rows of x 2^31 bytes apart
+    far = T.empty(((1 << 28) + 64,), tt._capi.F64)
+    for i, at in enumerate((0, 1 << 28)):
+        T(far.storage, far.dtype, (40,), (1,), at).assign(T.from_numpy(np.arange(40, dtype=np.float64) + 100 * i))
+    xf = T(far.storage, far.dtype, (2, 40), (1 << 28, 1), 0)
+    host = np.stack([np.arange(40.0), np.arange(40.0) + 100])
+    w = r.integers(-2, 3, (40, 24)).astype(np.float64)
+    h, g, u = tt.gated_linear(xf, T.from_numpy(w), T.from_numpy(w), activation="relu", save=True)
+    assert np.array_equal(g.to_numpy(), host @ w) and np.array_equal(h.to_numpy(), np.maximum(host @ w, 0) * (host @ w))
+    ones = T.from_numpy(np.ones((2, 24)))
+    got = tt.gated_linear_backward(ones, xf, T.from_numpy(w), T.from_numpy(w), g, u, activation="relu")
+    pg, pu = (host @ w) * ((host @ w) >= 0), np.maximum(host @ w, 0)
+    assert np.array_equal(got[1].to_numpy(), host.T @ pg) and np.array_equal(got[2].to_numpy(), host.T @ pu)
+
+
 def test_gated_linear_shapes(tt):
     r = rng_of(11)
     x, wg, wu, bg, bu, _ = gated_data(r, np.float32, 24, 40, 36)

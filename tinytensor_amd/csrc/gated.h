@@ -64,6 +64,7 @@ struct GatedForward {
 // How the backward products' reductions are cut: dx's two reductions of k each into x_splits chunks of x_chunk (0: both in
 // one piece), the weights' reductions of `rows` into w_splits chunks of w_chunk (0: one piece).
 struct GatedSplit {
+    int tile;  // 64, or 128 for f32
     int x_splits, x_chunk, w_splits, w_chunk;
     int64_t x_parts, w_parts, b_parts;  // elements of the parts of dx, of dWg and dWu, of the bias gradients
 };

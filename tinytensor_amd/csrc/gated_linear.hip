@@ -358,13 +358,9 @@ ttamd_status launch_prepare(int act, const PrepareArgs<T> &a, hipStream_t st) {
     return TTAMD_OK;
 }
 
-// Sizes whose byte offsets inside a tile's operands and results fit the tile kernels' 32 bits.
-bool tiles_reach(const GatedSizes &z, int64_t rows, int64_t inner, int64_t hidden, const int64_t (&strides)[3]) {
-    const int64_t most = 0x7fffffffLL / static_cast<int64_t>(z.item);
-    for (int64_t s : strides)
-        if ((inner + 256) * s > most || (rows + 256) * s > most) return false;
-    return rows * z.hidden_row < most && rows * z.inner_row < most && z.inner_row * z.hidden_row < most && 256 * hidden < most && 256 * inner < most;
-}
+// Offsets inside a tile's operand or result are 32-bit: `lines` rows of `row` elements must lie within 2^31 bytes.
+bool within_reach(size_t item, int64_t lines, int64_t row) { return (lines + 64) * row < 0x7fffffffLL / static_cast<int64_t>(item); }
+constexpr int64_t kTileLines = 256;  // of the largest tile
 
 struct Pass {
     int device, act;
@@ -384,14 +380,16 @@ ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, 
     PrepareArgs<T> prep{};
     // One grid of both products (gated_tiles.hip), unless it would be few tiles of a long reduction, which the separate
     // products cut (128 x 1024 x 2048 f32: 64 tiles, 38 us against 28 in three launches; 256 x 1024 x 4096: 256 tiles, 38
-    // against 49).
+    // against 49), or the weights are beyond its reach.
     const int64_t tiles = (rows + 63) / 64 * ((hidden + (z.item == 4 ? 63 : 31)) / (z.item == 4 ? 64 : 32));
     const bool few = inner > 256 && (rows <= 32 || tiles < 96);
-    if (!few && tiles_reach(z, rows, inner, hidden, {x.s0, wg.s0, wu.s0})) {
+    if (!few && within_reach(z.item, z.inner_row, z.hidden_row) && within_reach(z.item, kTileLines, z.inner_row) &&
+        within_reach(z.item, kTileLines, z.hidden_row)) {
         const bool own = inner % z.vec == 0;  // (x's padding meets rows of zeros in the weights' copies)
-        if (!row_vectors(x, inner)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
-        if (!own || !row_vectors(wg, hidden)) prep.copy[1] = copy_job(wg, inner, hidden, z.inner_row, z.hidden_row, p.ws + z.wg);
-        if (!own || !row_vectors(wu, hidden)) prep.copy[2] = copy_job(wu, inner, hidden, z.inner_row, z.hidden_row, p.ws + z.wu);
+        const auto far = [&](const Operand<T> &w) { return !own || !row_vectors(w, hidden) || !within_reach(z.item, inner, w.s0); };
+        if (!row_vectors(x, inner) || !within_reach(z.item, kTileLines, x.s0)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
+        if (far(wg)) prep.copy[1] = copy_job(wg, inner, hidden, z.inner_row, z.hidden_row, p.ws + z.wg);
+        if (far(wu)) prep.copy[2] = copy_job(wu, inner, hidden, z.inner_row, z.hidden_row, p.ws + z.wu);
         if (ttamd_status s = launch_prepare(p.act, prep, st)) return s;
         const GatedForward<T> a{x.data, wg.data, wu.data, x.s0, wg.s0, wu.s0, static_cast<int>(rows), static_cast<int>(z.inner_row),
                                 static_cast<int>(z.hidden_row), static_cast<int>(hidden), p.act, static_cast<const T *>(gate_bias),
@@ -438,13 +436,14 @@ ttamd_status backward(const Pass &p, const void *grad_out, const void *gate, con
         prep.slope_blocks_n = static_cast<int>((z.hidden_row / z.vec + 63) / 64);
         prep.slope_blocks = static_cast<int>((rows + kSlopeRows - 1) / kSlopeRows) * prep.slope_blocks_n;
     }
-    // One grid of all three products' 64 x 64 tiles; separate products with tiles up to 256 x 256 from 64 Gflop on
-    // (4096 x 1024 x 4096 f32: 1110 us against 1035; 4096 x 1024 x 1024: 275 against 285).
-    const bool huge = 8.0 * rows * inner * hidden > 64e9;
-    if (!huge && rows > 0 && tiles_reach(z, rows, inner, hidden, {x.s0, wg.s0, wu.s0})) {
-        if (!row_vectors(x, inner)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
-        if (!row_vectors(wg, hidden)) prep.copy[1] = copy_job(wg, inner, hidden, inner, z.hidden_row, p.ws + z.wg);
-        if (!row_vectors(wu, hidden)) prep.copy[2] = copy_job(wu, inner, hidden, inner, z.hidden_row, p.ws + z.wu);
+    // One grid of all three products (gated_tiles.hip) unless rows or weights are beyond its reach.
+    const int64_t piece = z.split.w_splits ? z.split.w_chunk : rows;  // rows under a tile of a weight's gradient
+    if (rows > 0 && within_reach(z.item, piece, z.hidden_row) && within_reach(z.item, piece, z.inner_row) &&
+        within_reach(z.item, kTileLines, z.hidden_row) && within_reach(z.item, kTileLines, z.inner_row)) {
+        const auto far = [&](const Operand<T> &w) { return !row_vectors(w, hidden) || !within_reach(z.item, kTileLines, w.s0); };
+        if (!row_vectors(x, inner) || !within_reach(z.item, piece, x.s0)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
+        if (far(wg)) prep.copy[1] = copy_job(wg, inner, hidden, inner, z.hidden_row, p.ws + z.wg);
+        if (far(wu)) prep.copy[2] = copy_job(wu, inner, hidden, inner, z.hidden_row, p.ws + z.wu);
         if (ttamd_status s = launch_prepare(p.act, prep, st)) return s;
         const GatedBackward<T> a{x.data, wg.data, wu.data, x.s0, wg.s0, wu.s0, dg, du, z.hidden_row, static_cast<int>(rows), static_cast<int>(inner),
                                  static_cast<int>(z.inner_row), static_cast<int>(hidden), static_cast<int>(z.hidden_row), static_cast<T *>(dx),
@@ -476,8 +475,21 @@ ttamd_status backward(const Pass &p, const void *grad_out, const void *gate, con
         if (ttamd_status s = ttamd_batched_matmul(p.device, p.dtype, 1, R, H, K, &gv, &wgt, dx, nullptr, p.stream)) return s;
         if (ttamd_status s = ttamd_batched_matmul(p.device, p.dtype, 1, R, H, K, &uv, &wut, dx, &add, p.stream)) return s;
     }
-    if (ttamd_status s = ttamd_batched_matmul(p.device, p.dtype, 1, K, R, H, &xt, &gv, dwg, nullptr, p.stream)) return s;
-    return ttamd_batched_matmul(p.device, p.dtype, 1, K, R, H, &xt, &uv, dwu, nullptr, p.stream);
+    // the weights' gradients in runs of rows whose offsets fit the products' 32 bits
+    const int64_t longest = z.hidden_row > x.s0 + x.s1 * inner ? z.hidden_row : x.s0 + x.s1 * inner;
+    int64_t run = 0x3fffffffLL / static_cast<int64_t>(z.item) / longest;
+    if (run < 64) run = 64;
+    for (int64_t r = 0; r == 0 || r < rows; r += run) {
+        const int n = static_cast<int>(rows - r < run ? rows - r : run);
+        ttamd_view3 xr = xt, gr = gv, ur = uv;
+        xr.offset += r * x.s0;
+        gr.offset += r * z.hidden_row;
+        ur.offset += r * z.hidden_row;
+        const ttamd_epilogue *ep = r ? &add : nullptr;
+        if (ttamd_status s = ttamd_batched_matmul(p.device, p.dtype, 1, K, n, H, &xr, &gr, dwg, ep, p.stream)) return s;
+        if (ttamd_status s = ttamd_batched_matmul(p.device, p.dtype, 1, K, n, H, &xr, &ur, dwu, ep, p.stream)) return s;
+    }
+    return TTAMD_OK;
 }
 
 ttamd_status check_workspace(const char *what, const void *workspace, size_t given, size_t needed) {

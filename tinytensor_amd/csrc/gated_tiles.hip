@@ -175,30 +175,26 @@ gated_forward_kernel(GatedForward<T> a, int tiles_m, int tiles_n, int k_half) {
     }
 }
 
-// The backward pass's products as one grid of 64 x 64 tiles: first the tiles of dx = dg . Wg^T + du . Wu^T (two reductions
-// into the same accumulators), then those of dWg = x^T . dg and dWu = x^T . du, whose first rows of tiles also add up the
-// vectors of dg / du that they stage: the bias gradients.
-template <typename T>
-struct SmallTile;
-template <>
-struct SmallTile<float> {
-    static constexpr int BK = 32;
-};
-template <>
-struct SmallTile<double> {
-    static constexpr int BK = 16;
+// The backward pass's products as one grid of B x B tiles: first the tiles of dx = dg . Wg^T + du . Wu^T (two reductions into
+// the same accumulators), then those of dWg = x^T . dg and dWu = x^T . du, whose first rows of tiles also add up the vectors
+// of dg / du that they stage: the bias gradients.  At least two workgroups share a CU, and one's first loads and stores run
+// under the other's products; the long reductions of dx go first and the weights' tiles fill up beside them.
+template <typename T, int B>
+struct BackwardTile {
+    static constexpr int BK = sizeof(T) == 4 && B == 64 ? 32 : 16;
+    static constexpr int PF = B == 64 ? 2 : 1;
 };
 
-template <typename T, int PF>
+template <typename T, int B>
 __device__ __forceinline__ void gated_dx_tile(const GatedBackward<T> &a, int item, int tiles, int tiles_n, T *smem) {
-    constexpr int BK = SmallTile<T>::BK, VK = Mfma<T>::VK;
-    using St = Stager<T, 64, BK, true, VK, PF>;
-    using Engine = TileEngine<T, 64, 64, BK, 2, 2, St, St>;
+    constexpr int BK = BackwardTile<T, B>::BK, PF = BackwardTile<T, B>::PF, VK = Mfma<T>::VK;
+    using St = Stager<T, B, BK, true, VK, PF>;
+    using Engine = TileEngine<T, B, B, BK, 2, 2, St, St>;
     const int tid = threadIdx.x;
     const int part = item / tiles;  // of both reductions; 0 when they are not cut
     int batch, tm, tn;
     decode_tile(remap_xcd(item - part * tiles, tiles), tiles / tiles_n, tiles_n, batch, tm, tn);
-    const int m0 = tm * 64, n0 = tn * 64;
+    const int m0 = tm * B, n0 = tn * B;
     const int splits = a.split.x_splits;
     Engine eng;
     eng.init(tid);
@@ -219,19 +215,19 @@ __device__ __forceinline__ void gated_dx_tile(const GatedBackward<T> &a, int ite
     store_tile_dense<T, true>(eng, out, a.rows, a.inner, m0, n0, static_cast<const T *>(nullptr), 0, 0, 0);
 }
 
-template <typename T, int PF>
+template <typename T, int B>
 __device__ __forceinline__ void gated_dw_tile(const GatedBackward<T> &a, int item, int tiles, int tiles_n, T *smem) {
-    constexpr int BK = SmallTile<T>::BK, VK = Mfma<T>::VK;
-    using StA = Stager<T, 64, BK, false, VK, PF>;
-    using StB = Stager<T, 64, BK, false, VK, PF, true>;
-    using Engine = TileEngine<T, 64, 64, BK, 2, 2, StA, StB>;
-    static_assert(static_cast<size_t>(StB::kSumParts) * 64 * sizeof(T) <= Engine::kLdsBytes, "the operand sums fit the tile buffers");
+    constexpr int BK = BackwardTile<T, B>::BK, PF = BackwardTile<T, B>::PF, VK = Mfma<T>::VK;
+    using StA = Stager<T, B, BK, false, VK, PF>;
+    using StB = Stager<T, B, BK, false, VK, PF, true>;
+    using Engine = TileEngine<T, B, B, BK, 2, 2, StA, StB>;
+    static_assert(static_cast<size_t>(StB::kSumParts) * B * sizeof(T) <= Engine::kLdsBytes, "the operand sums fit the tile buffers");
     const int tid = threadIdx.x;
     const int which = item / tiles;  // 2 x chunk + (0: dWg, 1: dWu)
     const bool second = which & 1;
     int batch, tm, tn;
     decode_tile(remap_xcd(item - which * tiles, tiles), tiles / tiles_n, tiles_n, batch, tm, tn);
-    const int m0 = tm * 64, n0 = tn * 64;
+    const int m0 = tm * B, n0 = tn * B;
     const int splits = a.split.w_splits;
     const int r0 = splits ? which / 2 * a.split.w_chunk : 0;
     const int R = splits && a.rows - r0 > a.split.w_chunk ? a.split.w_chunk : a.rows - r0;
@@ -250,25 +246,25 @@ __device__ __forceinline__ void gated_dw_tile(const GatedBackward<T> &a, int ite
     eng.run(sa, sb, smem, R, true);
     if (bias && tm == 0) {  // (workgroup-uniform) a lane's rows were added in order; the lanes of a column follow in lane order
         __syncthreads();
-        *reinterpret_cast<typename StB::V *>(&smem[sb.sum_part() * 64 + sb.sum_row0()]) = sb.sum;
+        *reinterpret_cast<typename StB::V *>(&smem[sb.sum_part() * B + sb.sum_row0()]) = sb.sum;
         __syncthreads();
-        if (tid < 64 && n0 + tid < a.hidden) {
+        if (tid < B && n0 + tid < a.hidden) {
             T v = T(0);
 #pragma unroll
-            for (int r = 0; r < StB::kSumParts; ++r) v += smem[r * 64 + tid];
+            for (int r = 0; r < StB::kSumParts; ++r) v += smem[r * B + tid];
             bias[n0 + tid] = v;
         }
     }
     store_tile_dense<T, true>(eng, out, a.inner, a.hidden, m0, n0, static_cast<const T *>(nullptr), 0, 0, 0);
 }
 
-template <typename T, int PF>
+template <typename T, int B>
 __global__ void __launch_bounds__(kThreads, 2) gated_backward_kernel(GatedBackward<T> a, int dx_items, int dx_tiles, int dx_tiles_n, int dw_tiles, int dw_tiles_n) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
     T *const smem = reinterpret_cast<T *>(smem_raw);
     const int block = blockIdx.x;
-    if (block < dx_items) gated_dx_tile<T, PF>(a, block, dx_tiles, dx_tiles_n, smem);
-    else gated_dw_tile<T, PF>(a, block - dx_items, dw_tiles, dw_tiles_n, smem);
+    if (block < dx_items) gated_dx_tile<T, B>(a, block, dx_tiles, dx_tiles_n, smem);
+    else gated_dw_tile<T, B>(a, block - dx_items, dw_tiles, dw_tiles_n, smem);
 }
 
 // out[i] = sum over p < parts of src[p * stride + i], p ascending; up to five such sums in a launch.
@@ -373,49 +369,63 @@ ttamd_status launch_gated_forward_tiles(const GatedForward<T> &a, int device, hi
     }
 }
 
-// Reductions are cut into equal chunks where their tiles alone would load the CUs unevenly: of the numbers of chunks tried,
-// the pair that is done first by this estimate, in units of one k of a 64 x 64 tile (15 ns on a CU in f32, 30 in f64).  The
-// tiles are dealt to 256 CUs in order, dx's first; a tile costs its reduction and 70 units of first loads and stores; cut
-// reductions cost a launch (200) and the traffic of their parts.  Against whole reductions: 16 x 1024 x 4096 154 -> 46 us
-// forward and backward, 4096 x 256 x 512 134 -> 83; against one fixed rule (no chunk above the even share):
-// 4096 x 256 x 512 101 -> 83.
+// Reductions are cut into equal chunks where their tiles alone would load the CUs unevenly: of the tile sizes and numbers of
+// chunks tried, those that are done first by this estimate, in units of one k of a 64 x 64 tile (15 ns on a CU in f32, 30 in
+// f64).  The tiles are dealt to 256 CUs in order, dx's first; a tile costs its reduction and 70 units of first loads and
+// stores; a 128 x 128 tile (f32) costs 3.7 times as much a k; cut reductions cost a launch (200) and the traffic of their
+// parts.  Against whole reductions: 16 x 1024 x 4096 154 -> 46 us forward and backward, 4096 x 256 x 512 134 -> 73.
 GatedSplit plan_gated_split(size_t item, int64_t rows, int64_t inner, int64_t hidden, int64_t k) {
-    const int64_t dx = (rows + 63) / 64 * ((inner + 63) / 64), dw = 2 * ((inner + 63) / 64) * ((hidden + 63) / 64);
     const int64_t x_bytes = 2 * rows * inner * static_cast<int64_t>(item), w_bytes = 2 * inner * hidden * static_cast<int64_t>(item);
     constexpr int64_t kMostBytes = int64_t(64) << 20, kShortest = 192;
     const auto chunk_of = [](int64_t reduction, int n) { return ((reduction + n - 1) / n + 31) / 32 * 32; };  // (whole k tiles of either type)
     double best = 0;
-    int best_x = -1, best_w = 1;
-    for (int sx = 0; sx <= 32; sx = sx ? 2 * sx : 1) {  // 0: both reductions of a dx tile in one piece
-        if (sx > 1 && (chunk_of(k, sx) < kShortest || sx * x_bytes > kMostBytes)) break;
-        if (sx == 1 && x_bytes > kMostBytes) break;
-        const double lx = 70.0 + (sx ? static_cast<double>(chunk_of(k, sx)) : 2.0 * k);
-        const int64_t nx = dx * (sx ? 2 * sx : 1);
-        for (int sw = 1; sw <= 32; sw *= 2) {
-            if (sw > 1 && (chunk_of(rows, sw) < kShortest || sw * w_bytes > kMostBytes)) break;
-            const double lw = 70.0 + static_cast<double>(sw > 1 ? chunk_of(rows, sw) : rows);
-            const int64_t nw = dw * sw;
+    int best_b = 0, best_x = 0, best_w = 1;
+    for (int B = 64; B <= (item == 4 ? 128 : 64); B *= 2) {
+        const int64_t dx = (rows + B - 1) / B * ((inner + B - 1) / B), dw = 2 * ((inner + B - 1) / B) * ((hidden + B - 1) / B);
+        const double unit = B == 64 ? 1.0 : 3.7, once = B == 64 ? 70.0 : 160.0;
+        const double share = B == 64 && item == 4 ? 3 : 2;  // workgroups that a CU holds
+        for (int sx = 0; sx <= 32; sx = sx ? 2 * sx : 1) {  // 0: both reductions of a dx tile in one piece
+            if (sx > 0 && ((sx > 1 && chunk_of(k, sx) < kShortest) || sx * x_bytes > kMostBytes)) break;
+            const double lx = once + unit * (sx ? static_cast<double>(chunk_of(k, sx)) : 2.0 * k);
+            const int64_t nx = dx * (sx ? 2 * sx : 1);
             // CUs hold nx / 256 tiles of dx, the first nx % 256 of them one more; the weights' tiles go where there is room
             const double low = static_cast<double>(nx / 256) * lx, high = nx % 256 ? low + lx : low;
             const int64_t many = nx % 256, few = 256 - many;
-            double end = (nx * lx + nw * lw) / 256;
-            if (end < high) end = high;
-            for (int tries = 0; tries < 64; ++tries) {
-                const double a = std::floor((end - low) / lw + 1e-9), b = std::floor((end - high) / lw + 1e-9);
-                if (few * a + many * b >= nw) break;
-                const double next_low = low + (a + 1) * lw, next_high = high + (b + 1) * lw;
-                end = many && next_high < next_low ? next_high : next_low;
-            }
-            const double parts = (sx ? static_cast<double>(sx) * x_bytes : 0.0) + (sw > 1 ? static_cast<double>(sw) * w_bytes : 0.0);
-            if (parts > 0) end += 200 + 2 * parts / 4e12 / (item == 4 ? 15e-9 : 30e-9);
-            if (best_x < 0 || end < best) {
-                best = end;
-                best_x = sx;
-                best_w = sw;
+            for (int sw = 1; sw <= 32; sw *= 2) {
+                if (sw > 1 && (chunk_of(rows, sw) < kShortest || sw * w_bytes > kMostBytes)) break;
+                // (32-bit offsets: prefer pieces of rows that the tiles can reach)
+                if ((chunk_of(rows, sw) + 64) * (k > inner ? k : inner) * static_cast<int64_t>(item) > 0x7fffffffLL && 2 * sw <= 32 && 2 * sw * w_bytes <= kMostBytes) continue;
+                const double lw = once + unit * static_cast<double>(sw > 1 ? chunk_of(rows, sw) : rows);
+                const int64_t nw = dw * sw;
+                double end = (nx * lx + nw * lw) / 256;
+                if (end < high) end = high;
+                for (int tries = 0; tries < 64; ++tries) {
+                    const double a = std::floor((end - low) / lw + 1e-9), b = std::floor((end - high) / lw + 1e-9);
+                    if (few * a + many * b >= nw) break;
+                    const double next_low = low + (a + 1) * lw, next_high = high + (b + 1) * lw;
+                    end = many && next_high < next_low ? next_high : next_low;
+                }
+                // The workgroups of a CU share it: a dx tile proceeds at 1 / share of its rate while weights' tiles are left to
+                // fill the other places, and what is left of it then runs on after everything else has ended.
+                const double filled = (few * (share - nx / 256) + many * (share - nx / 256 - 1)) / share;
+                const double until = filled > 0 ? nw * lw / filled : share * lx;
+                if (nx < 256 * share && until < share * lx) {
+                    const double after = until + (nx / 256 + (many ? 1 : 0)) * (lx - until / share);
+                    if (end < after) end = after;
+                }
+                const double parts = (sx ? static_cast<double>(sx) * x_bytes : 0.0) + (sw > 1 ? static_cast<double>(sw) * w_bytes : 0.0);
+                if (parts > 0) end += 200 + 2 * parts / 4e12 / (item == 4 ? 15e-9 : 30e-9);
+                if (!best_b || end < best) {
+                    best = end;
+                    best_b = B;
+                    best_x = sx;
+                    best_w = sw;
+                }
             }
         }
     }
     GatedSplit s{};
+    s.tile = best_b;
     if (best_x > 0) {
         s.x_chunk = static_cast<int>(chunk_of(k, best_x));
         s.x_splits = static_cast<int>((k + s.x_chunk - 1) / s.x_chunk);
@@ -432,23 +442,30 @@ GatedSplit plan_gated_split(size_t item, int64_t rows, int64_t inner, int64_t hi
 
 template <typename T>
 ttamd_status launch_gated_backward_tiles(const GatedBackward<T> &a, int device, hipStream_t st) {
-    constexpr int BK = SmallTile<T>::BK, VK = Mfma<T>::VK;
+    constexpr int VK = Mfma<T>::VK;
     const GatedSplit &sp = a.split;
-    const int dx_n = (a.inner + 63) / 64, dx = (a.rows + 63) / 64 * dx_n, dx_items = dx * (sp.x_splits ? 2 * sp.x_splits : 1);
-    const int dw_n = (a.hidden + 63) / 64, dw = (a.inner + 63) / 64 * dw_n, dw_items = dw * (sp.w_splits ? 2 * sp.w_splits : 2);
-    const auto run = [&]<int PF>() -> ttamd_status {
-        using StK = Stager<T, 64, BK, true, VK, PF>;
-        using StM = Stager<T, 64, BK, false, VK, PF>;
-        constexpr size_t lds_k = TileEngine<T, 64, 64, BK, 2, 2, StK, StK>::kLdsBytes, lds_m = TileEngine<T, 64, 64, BK, 2, 2, StM, StM>::kLdsBytes;
+    const auto run = [&]<int B>() -> ttamd_status {
+        constexpr int BK = BackwardTile<T, B>::BK, PF = BackwardTile<T, B>::PF;
+        const int dx_n = (a.inner + B - 1) / B, dx = (a.rows + B - 1) / B * dx_n, dx_items = dx * (sp.x_splits ? 2 * sp.x_splits : 1);
+        const int dw_n = (a.hidden + B - 1) / B, dw = (a.inner + B - 1) / B * dw_n, dw_items = dw * (sp.w_splits ? 2 * sp.w_splits : 2);
+        using StK = Stager<T, B, BK, true, VK, PF>;
+        using StM = Stager<T, B, BK, false, VK, PF>;
+        constexpr size_t lds_k = TileEngine<T, B, B, BK, 2, 2, StK, StK>::kLdsBytes, lds_m = TileEngine<T, B, B, BK, 2, 2, StM, StM>::kLdsBytes;
         constexpr size_t lds = lds_k > lds_m ? lds_k : lds_m;
         static_assert(lds <= 48 * 1024, "within the default dynamic LDS limit");
-        gated_backward_kernel<T, PF><<<static_cast<unsigned>(dx_items + dw_items), kThreads, lds, st>>>(a, dx_items, dx, dx_n, dw, dw_n);
+        gated_backward_kernel<T, B><<<static_cast<unsigned>(dx_items + dw_items), kThreads, lds, st>>>(a, dx_items, dx, dx_n, dw, dw_n);
         TTAMD_HIP_CHECK(hipGetLastError());
         return TTAMD_OK;
     };
-    // two k tiles in flight: the smaller registers let a CU hold three workgroups (16 x 1024 x 4096: 50 -> 46 us; at most
-    // 1.5 % slower than four in flight where two workgroups a CU are all there are)
-    if (ttamd_status s = run.template operator()<2>()) return s;
+    if constexpr (sizeof(T) == 4) {
+        if (sp.tile == 128) {
+            if (ttamd_status s = run.template operator()<128>()) return s;
+        } else if (ttamd_status s = run.template operator()<64>()) {
+            return s;
+        }
+    } else {
+        if (ttamd_status s = run.template operator()<64>()) return s;
+    }
     PartSums<T> sums{};
     unsigned blocks = 0;
     const auto add = [&](int k, const T *src, T *out, int64_t n, int64_t stride, int parts) {
