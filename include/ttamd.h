@@ -353,7 +353,7 @@ ttamd_status ttamd_embedding_forward(int device, ttamd_dtype dtype, ttamd_dtype 
 /* Its gradient: grad_table[v, :] = scale * sum of grad_out[i, :] over the i with index[i] == v, for every v < vocab (zeros
  * where there is none); accumulate != 0: grad_table += that, rows without a position are left alone.  grad_out
  * [count, dim] and grad_table [vocab, dim] dense.  Sums run over the positions in groups whose order the indices fix, in
- * 64 bits. */
+ * 64 bits.  Up to 128 positions need no workspace. */
 ttamd_status ttamd_embedding_backward_workspace(ttamd_dtype dtype, int64_t count, int64_t vocab, int64_t dim, size_t *bytes);
 ttamd_status ttamd_embedding_backward(int device, ttamd_dtype dtype, ttamd_dtype index_dtype, int64_t count, int64_t vocab,
                                       int64_t dim, const void *grad_out, const void *index, double scale, int accumulate,

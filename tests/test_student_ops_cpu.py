@@ -40,10 +40,11 @@ def test_embedding_backward_refusals(tt):
     assert query(capi.I32, 4, 10, 8, C.byref(n)) == capi.ERR_UNSUPPORTED_DTYPE
     assert query(capi.F32, 4, 0, 8, C.byref(n)) == capi.ERR_INVALID_ARGUMENT
     assert query(capi.F32, 4, 10, 8, None) == capi.ERR_INVALID_ARGUMENT
-    assert query(capi.F32, 4, 10, 8, C.byref(n)) == capi.OK and n.value > 0
+    assert query(capi.F32, 4, 10, 8, C.byref(n)) == capi.OK and n.value == 0  # few positions need none
+    assert query(capi.F32, 400, 10, 8, C.byref(n)) == capi.OK and n.value > 0
     need = n.value
 
-    def call(index_dtype=capi.I32, count=4, dy=A, index=2 * A, grad=3 * A, ws=4 * A, size=need):
+    def call(index_dtype=capi.I32, count=400, dy=A, index=2 * A, grad=3 * A, ws=4 * A, size=need):
         return lib.ttamd_embedding_backward(0, capi.F32, index_dtype, count, 10, 8, dy, index, 1.0, 0, grad, ws, size, None)
 
     assert call(index_dtype=capi.F32) == capi.ERR_UNSUPPORTED_DTYPE

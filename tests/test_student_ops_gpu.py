@@ -98,7 +98,7 @@ def check_embedding_gradient(got, dy, ids, vocab, scale, dtype, before=None):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("index", [np.int32, np.int64])
-@pytest.mark.parametrize("count, vocab, dim", [(1, 1, 1), (1, 300, 8), (5, 3, 7), (16, 1, 4), (17, 1, 5), (257, 2, 3), (100, 1000, 333), (1000, 37, 130),
+@pytest.mark.parametrize("count, vocab, dim", [(1, 1, 1), (1, 300, 8), (5, 3, 7), (16, 1, 4), (17, 1, 5), (257, 2, 3), (100, 1000, 333), (1000, 37, 130), (64, 9, 30), (65, 40, 1), (128, 3, 257), (128, 70000, 8), (129, 50, 12),
                                                (4096, 600, 64), (3000, 140000, 12), (700, 513, 1028), (0, 9, 6), (5000, 1, 260)])
 def test_embedding_gradient(tt, dtype, index, count, vocab, dim):
     r = rng_of(count, vocab, dim)

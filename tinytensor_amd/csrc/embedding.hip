@@ -467,6 +467,61 @@ __global__ void __launch_bounds__(64 * kJoinWaves) embedding_join_kernel(SumArgs
     }
 }
 
+// ---- gradient of few positions: one launch -------------------------------------------------------------------------------
+// With kFew positions at most a wave holds every index in two registers a lane and finds the positions of a token by two
+// comparisons, so each wave sees to its kZeroRows rows of the table by itself: sums in the order of the positions, zeros where
+// there is none.  (17 positions, 1096 rows of 97 doubles: three launches and their workspace take the host 18 us, one 12.)
+constexpr int kFew = 128;
+template <typename T, int W, bool I64>
+__global__ void __launch_bounds__(64) embedding_few_kernel(SumArgs<T> a, const void *index, int count) {
+    const int lane = threadIdx.x;
+    int v[kFew / 64];
+#pragma unroll
+    for (int u = 0; u < kFew / 64; ++u) {
+        const int i = u * 64 + lane;
+        const int64_t x = i < count ? load_index<I64>(index, i) : -1;
+        v[u] = x >= 0 && x < a.vocab ? static_cast<int>(x) : -1;
+    }
+    const int64_t at = (static_cast<int64_t>(blockIdx.y) * 64 + lane) * W, col = at + W <= a.dim ? at : a.dim - W;
+    const bool live = at < a.dim;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kZeroRows, last = first + kZeroRows < a.vocab ? first + kZeroRows : a.vocab;
+    for (int64_t row = first; row < last; ++row) {
+        uint64_t with[kFew / 64], any = 0;
+#pragma unroll
+        for (int u = 0; u < kFew / 64; ++u) any |= with[u] = __ballot(v[u] == static_cast<int>(row));
+        if (!any) {
+            if (live && !a.accumulate) {
+#pragma unroll
+                for (int k = 0; k < W; ++k) a.grad[row * a.dim + col + k] = T(0);
+            }
+            continue;
+        }
+        double sum[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) sum[k] = 0;
+#pragma unroll
+        for (int u = 0; u < kFew / 64; ++u)
+            while (with[u]) {  // four rows in flight
+                T x[4][W];
+                const uint64_t four = with[u];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int p = with[u] ? __builtin_ctzll(with[u]) : __builtin_ctzll(four);
+                    with[u] &= with[u] - 1;
+                    load_row<T, W>(a.dy + static_cast<int64_t>(u * 64 + p) * a.dim + col, x[i]);
+                }
+                const int n = __popcll(four);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (i < n) {
+#pragma unroll
+                        for (int k = 0; k < W; ++k) sum[k] += static_cast<double>(x[i][k]);
+                    }
+            }
+        if (live) write_gradient<T, W>(a, row, col, sum);
+    }
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------------------
 struct BackwardPlan {
     int bucket_log, tokens, chunk;
@@ -520,6 +575,20 @@ ttamd_status launch_forward(int64_t count, int64_t vocab, int64_t dim, const voi
 template <typename T>
 ttamd_status launch_backward(int64_t count, int64_t vocab, int64_t dim, const void *grad_out, const void *index, bool index64, double scale,
                              int accumulate, void *grad, void *workspace, hipStream_t st) {
+    // (columns that two lanes write may not be added to what is there twice)
+    const bool vec = accumulate ? dim % Row<T>::W == 0 : dim >= Row<T>::W;
+    const int w = vec ? Row<T>::W : 1;
+    const int64_t slabs = (dim + 64 * w - 1) / (64 * w);
+    if (count <= kFew) {
+        const SumArgs<T> a{static_cast<const T *>(grad_out), static_cast<T *>(grad), nullptr, nullptr, nullptr, nullptr, nullptr, 0, dim, 0, scale,
+                           accumulate, nullptr, 0, 0, vocab};
+        const dim3 grid(static_cast<unsigned>((vocab + kZeroRows - 1) / kZeroRows), static_cast<unsigned>(slabs));
+        const auto run = [&](auto kernel) { kernel<<<grid, 64, 0, st>>>(a, index, static_cast<int>(count)); };
+        if (vec) index64 ? run(embedding_few_kernel<T, Row<T>::W, true>) : run(embedding_few_kernel<T, Row<T>::W, false>);
+        else index64 ? run(embedding_few_kernel<T, 1, true>) : run(embedding_few_kernel<T, 1, false>);
+        TTAMD_HIP_CHECK(hipGetLastError());
+        return TTAMD_OK;
+    }
     const BackwardPlan p = plan_backward(sizeof(T), count, vocab, dim);
     char *ws = static_cast<char *>(workspace);
     uint8_t *absent = accumulate ? nullptr : reinterpret_cast<uint8_t *>(ws + p.absent);
@@ -529,14 +598,9 @@ ttamd_status launch_backward(int64_t count, int64_t vocab, int64_t dim, const vo
     if (index64) embedding_order_kernel<true><<<1u << p.bucket_log, kOrderThreads, lds, st>>>(o);
     else embedding_order_kernel<false><<<1u << p.bucket_log, kOrderThreads, lds, st>>>(o);
     TTAMD_HIP_CHECK(hipGetLastError());
-    if (count == 0 && accumulate) return TTAMD_OK;
     const SumArgs<T> a{static_cast<const T *>(grad_out), static_cast<T *>(grad), reinterpret_cast<double *>(ws + p.partial), o.position,
                        o.token, o.total, reinterpret_cast<int4 *>(ws + p.crossing), p.chunks, dim, p.chunk, scale, accumulate,
                        absent, p.bucket_log, p.tokens, vocab};
-    // (columns that two lanes write may not be added to what is there twice)
-    const bool vec = accumulate ? dim % Row<T>::W == 0 : dim >= Row<T>::W;
-    const int w = vec ? Row<T>::W : 1;
-    const int64_t slabs = (dim + 64 * w - 1) / (64 * w);
     const int64_t fill = accumulate ? 0 : ((static_cast<int64_t>(p.tokens) << p.bucket_log) + kZeroRows * slabs - 1) / (kZeroRows * slabs);
     const dim3 grid(static_cast<unsigned>(p.chunks + fill), static_cast<unsigned>(slabs));
     // rows beyond half of the 256 MB Infinity Cache are loaded past it (65536 x 1024 f32: 216 -> 187 us in all; 8192 x 1024:
@@ -546,7 +610,6 @@ ttamd_status launch_backward(int64_t count, int64_t vocab, int64_t dim, const vo
     else if (vec) embedding_sum_kernel<T, Row<T>::W, false><<<grid, 64, 0, st>>>(a);
     else embedding_sum_kernel<T, 1, false><<<grid, 64, 0, st>>>(a);
     TTAMD_HIP_CHECK(hipGetLastError());
-    if (count == 0) return TTAMD_OK;
     const int64_t groups = (p.chunks + kJoinWaves - 1) / kJoinWaves;
     const dim3 join(static_cast<unsigned>(groups < 256 ? groups : 256), grid.y);
     if (vec) embedding_join_kernel<T, Row<T>::W><<<join, 64 * kJoinWaves, 0, st>>>(a);
@@ -615,7 +678,7 @@ ttamd_status ttamd_embedding_backward_workspace(ttamd_dtype dtype, int64_t count
         set_error("embedding_backward: bytes is NULL");
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
-    *bytes = plan_backward(dtype_size(dtype), count, vocab, dim).bytes;
+    *bytes = count <= kFew ? 0 : plan_backward(dtype_size(dtype), count, vocab, dim).bytes;
     return TTAMD_OK;
 }
 
@@ -627,7 +690,7 @@ ttamd_status ttamd_embedding_backward(int device, ttamd_dtype dtype, ttamd_dtype
     if (ttamd_status s = ttamd_embedding_backward_workspace(dtype, count, vocab, dim, &need)) return s;
     if (ttamd_status s = check_index_dtype(what, index_dtype)) return s;
     const size_t e = dtype_size(dtype);
-    if (!grad_table || !workspace || (count > 0 && (!index || !grad_out))) {
+    if (!grad_table || (need > 0 && !workspace) || (count > 0 && (!index || !grad_out))) {
         set_error("%s: NULL data pointer", what);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }

@@ -73,8 +73,28 @@ struct PrepareArgs {
 
 template <typename T>
 __device__ __forceinline__ void copy_tile(const CopyJob<T> &j, int block, T (*tile)[65]) {
+    using V = typename VecOf<T>::type;
+    typedef T near_t __attribute__((ext_vector_type(VecOf<T>::W), aligned(sizeof(T))));
+    constexpr int W = VecOf<T>::W, kVecs = 64 / W;
     const int tiles_n = static_cast<int>((j.dst_row + 63) / 64);
     const int64_t r0 = static_cast<int64_t>(block / tiles_n) * 64, c0 = static_cast<int64_t>(block % tiles_n) * 64;
+    if (j.s1 == 1) {  // rows in order: vectors, wherever the source's begin (dst_row is whole vectors)
+#pragma unroll
+        for (int i = threadIdx.x; i < 64 * kVecs; i += 256) {
+            const int64_t r = r0 + i / kVecs, c = c0 + i % kVecs * W;
+            if (r >= j.dst_rows || c >= j.dst_row) continue;
+            const T *src = j.src + r * j.s0 + c;
+            V v = {};
+            if (r < j.rows && c + W <= j.cols) {
+                v = *reinterpret_cast<const near_t *>(src);
+            } else if (r < j.rows) {
+#pragma unroll
+                for (int k = 0; k < W; ++k) v[k] = c + k < j.cols ? src[k] : T(0);
+            }
+            *reinterpret_cast<V *>(j.dst + r * j.dst_row + c) = v;
+        }
+        return;
+    }
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const bool by_rows = j.s0 < j.s1;  // lanes run along the rows (a transposed view) and the tile is turned in LDS
 #pragma unroll 4
@@ -192,6 +212,96 @@ __global__ void __launch_bounds__(256) gated_bias_kernel(const T *sums, int64_t 
     part[wave][lane] = v;
     __syncthreads();
     if (wave == 0 && c < hidden) out[c] = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+}
+
+// A few rows (a token or a handful while generating): bound by the weights, which are read once.  A workgroup owns 8 vectors of
+// columns of both weights and the whole reduction: lane group g of 128 takes every 128th row of the weights, so that its loads
+// are 128 neighbouring bytes and each feeds R rows of x out of LDS; the groups' sums are added by shuffles, then wave by
+// wave in order through LDS, and the same workgroup applies biases and activation: one launch.  Weights' rows may begin
+// anywhere; the last vector of a row is moved back to end with it (its first columns come out twice, the same).
+constexpr int kRowThreads = 1024, kRowLanes = 8, kRowGroups = kRowThreads / kRowLanes, kRowWaves = kRowThreads / 64;
+constexpr int kRowChunk = 1024;  // of the reduction whose x is in LDS at a time
+template <typename T>
+struct RowArgs {
+    const T *x, *wg, *wu, *bg, *bu;
+    int64_t x0, x1, wg_row, wu_row;
+    T *out, *gate, *up;
+    int rows, inner, hidden;  // rows: up to R
+};
+template <typename T, int R, int ACT>
+__global__ void __launch_bounds__(kRowThreads) gated_rows_kernel(RowArgs<T> a) {
+    constexpr int W = VecOf<T>::W;
+    typedef T near_t __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+    constexpr int kCols = kRowLanes * W;
+    __shared__ T xs[kRowChunk][R];
+    __shared__ T part[kRowWaves][2][R][kCols];
+    const int tid = threadIdx.x, lane = tid % kRowLanes, group = tid / kRowLanes;
+    const int c0 = blockIdx.x * kCols;
+    const int at = c0 + lane * W;
+    const int c = at + W <= a.hidden ? at : a.hidden - W;  // (lanes beyond the row repeat its last columns)
+    T g[R][W], u[R][W];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int k = 0; k < W; ++k) g[r][k] = u[r][k] = T(0);
+    for (int k0 = 0; k0 < a.inner; k0 += kRowChunk) {
+        const int n = a.inner - k0 < kRowChunk ? a.inner - k0 : kRowChunk;
+        if (k0) __syncthreads();
+        for (int i = tid; i < n * R; i += kRowThreads) {
+            const int r = i / n, k = i - r * n;
+            xs[k][r] = r < a.rows ? a.x[r * a.x0 + (k0 + k) * a.x1] : T(0);
+        }
+        __syncthreads();
+        const T *wg = a.wg + static_cast<int64_t>(k0) * a.wg_row + c, *wu = a.wu + static_cast<int64_t>(k0) * a.wu_row + c;
+#pragma unroll 4
+        for (int k = group; k < n; k += kRowGroups) {
+            const near_t p = *reinterpret_cast<const near_t *>(wg + k * a.wg_row), q = *reinterpret_cast<const near_t *>(wu + k * a.wu_row);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const T v = xs[k][r];
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    g[r][j] += v * p[j];
+                    u[r][j] += v * q[j];
+                }
+            }
+        }
+    }
+    const int wave = tid / 64;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+#pragma unroll
+            for (int d = kRowLanes; d < 64; d *= 2) {
+                g[r][j] += __shfl_xor(g[r][j], d, 64);
+                u[r][j] += __shfl_xor(u[r][j], d, 64);
+            }
+            if (tid % 64 < kRowLanes) {
+                part[wave][0][r][lane * W + j] = g[r][j];
+                part[wave][1][r][lane * W + j] = u[r][j];
+            }
+        }
+    __syncthreads();
+    for (int i = tid; i < a.rows * kCols; i += kRowThreads) {
+        const int r = i / kCols, k = i - r * kCols;
+        const int from = c0 + k / W * W;
+        const int col = (from + W <= a.hidden ? from : a.hidden - W) + k % W;  // the column that this place holds
+        T gv = T(0), uv = T(0);
+#pragma unroll
+        for (int w = 0; w < kRowWaves; ++w) {
+            gv += part[w][0][r][k];
+            uv += part[w][1][r][k];
+        }
+        if (a.bg) gv += a.bg[col];
+        if (a.bu) uv += a.bu[col];
+        const int64_t to = static_cast<int64_t>(r) * a.hidden + col;
+        if (a.gate) {
+            a.gate[to] = gv;
+            a.up[to] = uv;
+        }
+        a.out[to] = activate<T, ACT>(gv) * uv;
+    }
 }
 
 template <typename F>
@@ -330,12 +440,6 @@ bool row_vectors(const Operand<T> &m, int64_t cols) {
     constexpr int64_t W = VecOf<T>::W;
     return m.s1 == 1 && m.s0 % W == 0 && cols % W == 0 && !misaligned(m.data, 16);
 }
-// The same in either direction: what the separate products read with 16-byte loads.
-template <typename T>
-bool any_vectors(const Operand<T> &m) {
-    constexpr int64_t W = VecOf<T>::W;
-    return !misaligned(m.data, 16) && ((m.s1 == 1 && m.s0 % W == 0) || (m.s0 == 1 && m.s1 % W == 0));
-}
 template <typename T>
 CopyJob<T> copy_job(Operand<T> &m, int64_t rows, int64_t cols, int64_t dst_rows, int64_t dst_row, void *dst) {
     const int64_t blocks = (dst_rows + 63) / 64 * ((dst_row + 63) / 64);
@@ -371,18 +475,48 @@ struct Pass {
     void *stream;
 };
 
+// Up to 8 rows in one launch.  Against the separate products (three launches; f32, inputs in turn): 1 x 1024 x 4096 12.2 us
+// (a pass takes the host that long) against 18.0, 1 x 2048 x 8192 27.2 (4.9 TB/s) against 53, 8 x 2048 x 8192 41 against 52;
+// f64 1 x 1024 x 4096 15.5 against 18.1, but 4 x 2048 x 8192 64 against 55, so f64 takes 3 and 4 rows of small weights only.
+template <typename T>
+ttamd_status launch_rows(int act, const RowArgs<T> &a, int64_t rows, hipStream_t st) {
+    constexpr int kCols = kRowLanes * VecOf<T>::W;
+    const unsigned blocks = static_cast<unsigned>((a.hidden + kCols - 1) / kCols);
+    for_activation(act, [&]<int ACT>() {
+        if (rows > 4) {
+            if constexpr (sizeof(T) == 4) gated_rows_kernel<T, 8, ACT><<<blocks, kRowThreads, 0, st>>>(a);
+        } else if (rows > 2) {
+            gated_rows_kernel<T, 4, ACT><<<blocks, kRowThreads, 0, st>>>(a);
+        } else if (rows > 1) {
+            gated_rows_kernel<T, 2, ACT><<<blocks, kRowThreads, 0, st>>>(a);
+        } else {
+            gated_rows_kernel<T, 1, ACT><<<blocks, kRowThreads, 0, st>>>(a);
+        }
+    });
+    TTAMD_HIP_CHECK(hipGetLastError());
+    return TTAMD_OK;
+}
+
 template <typename T>
 ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, void *out, void *gate, void *up) {
     hipStream_t st = static_cast<hipStream_t>(p.stream);
     const int64_t rows = p.rows, inner = p.inner, hidden = p.hidden;
     const GatedSizes z = sizes_of(p.dtype, rows, inner, hidden, false);
     Operand<T> x = operand_of<T>(p.x), wg = operand_of<T>(p.wg), wu = operand_of<T>(p.wu);
+    const int64_t handful = z.item == 4 ? 8 : inner * hidden <= (1 << 20) ? 4 : 2;
+    if (rows <= handful && wg.s1 == 1 && wu.s1 == 1 && hidden >= z.vec) {
+        const RowArgs<T> a{x.data, wg.data, wu.data, static_cast<const T *>(gate_bias), static_cast<const T *>(up_bias), x.s0, x.s1, wg.s0, wu.s0,
+                           static_cast<T *>(out), static_cast<T *>(gate), static_cast<T *>(up), static_cast<int>(rows), static_cast<int>(inner), static_cast<int>(hidden)};
+        return launch_rows<T>(p.act, a, rows, st);
+    }
     PrepareArgs<T> prep{};
     // One grid of both products (gated_tiles.hip), unless it would be few tiles of a long reduction, which the separate
-    // products cut (128 x 1024 x 2048 f32: 64 tiles, 38 us against 28 in three launches; 256 x 1024 x 4096: 256 tiles, 38
-    // against 49), or the weights are beyond its reach.
-    const int64_t tiles = (rows + 63) / 64 * ((hidden + (z.item == 4 ? 63 : 31)) / (z.item == 4 ? 64 : 32));
-    const bool few = inner > 256 && (rows <= 32 || tiles < 96);
+    // products cut (f32, 64 x 128 tiles: 128 x 1024 x 2048, 64 tiles, 38 us against 28 in three launches; 256 x 1024 x 4096,
+    // 256 tiles, 38 against 49; f64, 64 x 64 tiles: 200 x 2001 x 1003, 128 tiles, 98 against 77; 256 x 1024 x 4096, 512
+    // tiles, 65 against 79), or the weights are beyond its reach.
+    const bool f32 = z.item == 4;
+    const int64_t tiles = (rows + 63) / 64 * ((hidden + (f32 ? 63 : 31)) / (f32 ? 64 : 32));
+    const bool few = inner > 256 && (rows <= 32 || tiles < (f32 ? 96 : 144));
     if (!few && within_reach(z.item, z.inner_row, z.hidden_row) && within_reach(z.item, kTileLines, z.inner_row) &&
         within_reach(z.item, kTileLines, z.hidden_row)) {
         const bool own = inner % z.vec == 0;  // (x's padding meets rows of zeros in the weights' copies)
@@ -395,12 +529,6 @@ ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, 
                                 static_cast<int>(z.hidden_row), static_cast<int>(hidden), p.act, static_cast<const T *>(gate_bias),
                                 static_cast<const T *>(up_bias), static_cast<T *>(out), static_cast<T *>(gate), static_cast<T *>(up)};
         return launch_gated_forward_tiles<T>(a, p.device, st);
-    }
-    if (rows >= 16) {
-        if (!any_vectors(x)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
-        if (!any_vectors(wg)) prep.copy[1] = copy_job(wg, inner, hidden, inner, z.hidden_row, p.ws + z.wg);
-        if (!any_vectors(wu)) prep.copy[2] = copy_job(wu, inner, hidden, inner, z.hidden_row, p.ws + z.wu);
-        if (ttamd_status s = launch_prepare(p.act, prep, st)) return s;
     }
     const ScratchLoan loan(p.ws + z.scratch, z.scratch_bytes);
     void *g = gate ? gate : p.ws + z.first, *u = gate ? up : p.ws + z.second;
@@ -451,11 +579,6 @@ ttamd_status backward(const Pass &p, const void *grad_out, const void *gate, con
                                  z.split, reinterpret_cast<T *>(p.ws + z.parts), reinterpret_cast<T *>(p.ws + z.parts) + z.split.x_parts,
                                  reinterpret_cast<T *>(p.ws + z.parts) + z.split.x_parts + z.split.w_parts};
         return launch_gated_backward_tiles<T>(a, p.device, st);
-    }
-    if (rows >= 16) {
-        if (!any_vectors(x)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
-        if (!any_vectors(wg)) prep.copy[1] = copy_job(wg, inner, hidden, inner, z.hidden_row, p.ws + z.wg);
-        if (!any_vectors(wu)) prep.copy[2] = copy_job(wu, inner, hidden, inner, z.hidden_row, p.ws + z.wu);
     }
     T *const sums = reinterpret_cast<T *>(p.ws + z.sums);
     if (dbg || dbu) prep.sums = sums;

@@ -175,8 +175,8 @@ gated_forward_kernel(GatedForward<T> a, int tiles_m, int tiles_n, int k_half) {
     }
 }
 
-// The backward pass's products as one grid of B x B tiles: first the tiles of dx = dg . Wg^T + du . Wu^T (two reductions into
-// the same accumulators), then those of dWg = x^T . dg and dWu = x^T . du, whose first rows of tiles also add up the vectors
+// The backward pass's products as one grid of B x B tiles: first the tiles of dx = dg . Wg^T + du . Wu^T (two reductions one
+// after the other), then those of dWg = x^T . dg and dWu = x^T . du, whose first rows of tiles also add up the vectors
 // of dg / du that they stage: the bias gradients.  At least two workgroups share a CU, and one's first loads and stores run
 // under the other's products; the long reductions of dx go first and the weights' tiles fill up beside them.
 template <typename T, int B>
@@ -198,10 +198,27 @@ __device__ __forceinline__ void gated_dx_tile(const GatedBackward<T> &a, int ite
     const int splits = a.split.x_splits;
     Engine eng;
     eng.init(tid);
+    // The first reduction's result is set aside and added at the end: as exact as two products added up, where one run of both
+    // through the accumulators would carry the roundings of twice the length.
+    typename Engine::M::acc_t first[Engine::NBM][Engine::NBN];
+#pragma unroll
+    for (int i = 0; i < Engine::NBM; ++i)
+#pragma unroll
+        for (int j = 0; j < Engine::NBN; ++j) first[i][j] = eng.acc[i][j];
 #pragma unroll 1
     for (int s = 0; s < 2; ++s) {
         if (splits && s != part / splits) continue;
-        if (s == 1 && !splits) __syncthreads();  // every wave has read the first reduction's last tile
+        if (s == 1 && !splits) {
+            __syncthreads();  // every wave has read the first reduction's last tile
+#pragma unroll
+            for (int i = 0; i < Engine::NBM; ++i)
+#pragma unroll
+                for (int j = 0; j < Engine::NBN; ++j) {
+                    first[i][j] = eng.acc[i][j];
+#pragma unroll
+                    for (int e = 0; e < Engine::M::NACC; ++e) eng.acc[i][j][e] = T(0);
+                }
+        }
         const int k0 = splits ? part % splits * a.split.x_chunk : 0;
         const int K = splits && a.k - k0 > a.split.x_chunk ? a.split.x_chunk : a.k - k0;
         const T *d = (s == 0 ? a.dg : a.du) + k0, *w = (s == 0 ? a.wg : a.wu) + k0;
@@ -211,6 +228,10 @@ __device__ __forceinline__ void gated_dx_tile(const GatedBackward<T> &a, int ite
         sb.init(w + static_cast<int64_t>(n0) * w_row, tid, a.inner - n0, w_row, 1, K);
         eng.run(sa, sb, smem, K, true);
     }
+#pragma unroll
+    for (int i = 0; i < Engine::NBM; ++i)
+#pragma unroll
+        for (int j = 0; j < Engine::NBN; ++j) eng.acc[i][j] += first[i][j];
     T *const out = splits ? a.x_part + static_cast<int64_t>(part) * a.rows * a.inner : a.dx;
     store_tile_dense<T, true>(eng, out, a.rows, a.inner, m0, n0, static_cast<const T *>(nullptr), 0, 0, 0);
 }
