@@ -911,6 +911,164 @@ inline auto linear_mse_head(const Tensor &input, const Tensor &weight, const Ten
                                 r.dx.data_ptr(), r.dW.data_ptr(), r.db ? r.db->data_ptr() : nullptr, nullptr));
     return r;
 }
+// ---- operators of a language-model student (include/ttamd.h): no counterpart in the reference, beside nn::Linear and
+// nn::mse_loss ----
+namespace detail {
+inline void check_floats(const char *what, const Tensor &first, std::initializer_list<const Tensor *> others) {
+    if (first.dtype() != kF32 && first.dtype() != kF64) throw TTException(std::string(what) + ": operands of one floating point dtype");
+    for (const Tensor *t : others) {
+        if (t && t->dtype() != first.dtype()) throw TTException(std::string(what) + ": operands of one floating point dtype");
+        if (t && !(t->device() == first.device())) throw TTException(std::string(what) + ": operands on one device");
+    }
+}
+inline auto indices(const char *what, const Tensor &t, Device device) -> Tensor {
+    if (t.dtype() == kF32 || t.dtype() == kF64 || t.dtype() == kBool) throw TTException(std::string(what) + ": indices are integers");
+    if (!(t.device() == device)) throw TTException(std::string(what) + ": operands on one device");
+    return (t.dtype() == kI32 || t.dtype() == kI64 ? t : t.to(kI32)).contiguous();
+}
+inline auto view2(const Tensor &t) -> ttamd_view2 { return {t.storage()->ptr_, t.offset(), {t.stride()[0], t.stride()[1]}}; }
+inline auto activation(const std::string &name) -> int {
+    const char *const names[] = {"silu", "gelu", "relu", "sigmoid"};
+    for (int i = 0; i < 4; ++i)
+        if (name == names[i]) return i;
+    throw TTException("gated_linear: unknown activation " + name);
+}
+}  // namespace detail
+
+// out[..., :] = scale * table[indices[..., ], :]; an index outside the table gives zeros.  The table may be any view.
+inline auto embedding(const Tensor &indices, const Tensor &table, double scale = 1.0) -> Tensor {
+    if (table.dim() != 2) throw TTException("embedding: the table must be 2-D");
+    detail::check_floats("embedding", table, {});
+    const Tensor idx = detail::indices("embedding", indices, table.device());
+    auto shape = indices.shape().to_vec();
+    shape.push_back(table.size(1));
+    const Tensor out = Tensor::empty(Shape(shape), table.dtype(), table.device());
+    const ttamd_view2 tv = detail::view2(table);
+    const void *first = static_cast<const char *>(tv.data) + tv.offset * static_cast<int64_t>(dtype_size(table.dtype()));
+    check(ttamd_embedding_forward(table.device().id, static_cast<ttamd_dtype>(table.dtype()), static_cast<ttamd_dtype>(idx.dtype()), idx.numel(),
+                                  table.size(0), table.size(1), idx.data_ptr(), first, tv.stride[0], tv.stride[1], scale, out.data_ptr(), nullptr));
+    return out;
+}
+
+// Gradient of embedding() with respect to its table, [vocab, dim]; into `add_to` (dense), added to what is there, when given.
+inline auto embedding_backward(const Tensor &grad_output, const Tensor &indices, int vocab, double scale = 1.0, const Tensor *add_to = nullptr)
+    -> Tensor {
+    auto shape = indices.shape().to_vec();
+    if (grad_output.dim() != static_cast<int>(shape.size()) + 1) throw TTException("embedding_backward: the gradient must hold a row an index");
+    const int dim = grad_output.size(grad_output.dim() - 1);
+    for (std::size_t i = 0; i < shape.size(); ++i)
+        if (grad_output.size(static_cast<int>(i)) != shape[i]) throw TTException("embedding_backward: the gradient must hold a row an index");
+    detail::check_floats("embedding_backward", grad_output, {add_to});
+    const Tensor idx = detail::indices("embedding_backward", indices, grad_output.device());
+    const Tensor dy = grad_output.contiguous();
+    if (add_to && (!add_to->is_contiguous() || add_to->dim() != 2 || add_to->size(0) != vocab || add_to->size(1) != dim))
+        throw TTException("embedding_backward: the tensor to add to must be dense, [vocab, dim]");
+    const Tensor out = add_to ? *add_to : Tensor::empty(Shape({vocab, dim}), dy.dtype(), dy.device());
+    const auto dt = static_cast<ttamd_dtype>(dy.dtype());
+    std::size_t bytes = 0;
+    check(ttamd_embedding_backward_workspace(dt, idx.numel(), vocab, dim, &bytes));
+    StorageAMD ws(bytes ? bytes : 1, dy.device().id);
+    check(ttamd_embedding_backward(dy.device().id, dt, static_cast<ttamd_dtype>(idx.dtype()), idx.numel(), vocab, dim, dy.data_ptr(), idx.data_ptr(), scale,
+                                   add_to != nullptr, out.data_ptr(), ws.ptr_, bytes, nullptr));
+    return out;
+}
+
+// The gated pair of Linear layers: act(input . w_gate + b_gate) * (input . w_up + b_up) for a 2-D input; gate and up are the
+// two products that gated_linear_backward() reads (`save`).
+struct GatedResult {
+    Tensor output;
+    std::optional<Tensor> gate, up;
+};
+inline auto gated_linear(const Tensor &input, const Tensor &w_gate, const Tensor &w_up, const Tensor *b_gate = nullptr, const Tensor *b_up = nullptr,
+                         const std::string &activation = "silu", bool save = false) -> GatedResult {
+    const int act = detail::activation(activation);
+    if (input.dim() != 2 || w_gate.dim() != 2 || !(w_gate.shape() == w_up.shape()) || input.size(1) != w_gate.size(0))
+        throw TTException("Invalid shape for matrix multiplication");
+    detail::check_floats("gated_linear", input, {&w_gate, &w_up, b_gate, b_up});
+    const int rows = input.size(0), inner = input.size(1), hidden = w_gate.size(1);
+    for (const Tensor *b : {b_gate, b_up})
+        if (b && (b->dim() != 1 || b->size(0) != hidden)) throw TTException("gated_linear: a bias holds an element a column");
+    std::optional<Tensor> bg, bu;
+    if (b_gate) bg = b_gate->contiguous();
+    if (b_up) bu = b_up->contiguous();
+    const auto dt = static_cast<ttamd_dtype>(input.dtype());
+    const auto fresh = [&] { return Tensor::empty(Shape({rows, hidden}), input.dtype(), input.device()); };
+    GatedResult r;
+    r.output = fresh();
+    if (save) {
+        r.gate = fresh();
+        r.up = fresh();
+    }
+    std::size_t bytes = 0;
+    check(ttamd_gated_linear_workspace(dt, rows, inner, hidden, 0, &bytes));
+    StorageAMD ws(bytes ? bytes : 1, input.device().id);
+    const ttamd_view2 x = detail::view2(input), g = detail::view2(w_gate), u = detail::view2(w_up);
+    check(ttamd_gated_linear_forward(input.device().id, dt, act, rows, inner, hidden, &x, &g, &u, bg ? bg->data_ptr() : nullptr,
+                                     bu ? bu->data_ptr() : nullptr, r.output.data_ptr(), save ? r.gate->data_ptr() : nullptr,
+                                     save ? r.up->data_ptr() : nullptr, ws.ptr_, bytes, nullptr));
+    return r;
+}
+
+struct GatedGrads {
+    Tensor dx, dw_gate, dw_up;
+    std::optional<Tensor> db_gate, db_up;
+};
+inline auto gated_linear_backward(const Tensor &grad_output, const Tensor &input, const Tensor &w_gate, const Tensor &w_up, const Tensor &gate,
+                                  const Tensor &up, const std::string &activation = "silu", bool bias_grad = false) -> GatedGrads {
+    const int act = detail::activation(activation);
+    if (input.dim() != 2 || w_gate.dim() != 2 || !(w_gate.shape() == w_up.shape()) || input.size(1) != w_gate.size(0))
+        throw TTException("Invalid shape for matrix multiplication");
+    detail::check_floats("gated_linear_backward", input, {&grad_output, &w_gate, &w_up, &gate, &up});
+    const int rows = input.size(0), inner = input.size(1), hidden = w_gate.size(1);
+    for (const Tensor *t : {&grad_output, &gate, &up})
+        if (t->dim() != 2 || t->size(0) != rows || t->size(1) != hidden) throw TTException("gated_linear_backward: grad_output, gate and up must be [rows, hidden]");
+    const Tensor dh = grad_output.contiguous(), g = gate.contiguous(), u = up.contiguous();
+    const auto fresh = [&](Shape s) { return Tensor::empty(s, input.dtype(), input.device()); };
+    GatedGrads r;
+    r.dx = fresh(Shape({rows, inner}));
+    r.dw_gate = fresh(Shape({inner, hidden}));
+    r.dw_up = fresh(Shape({inner, hidden}));
+    if (bias_grad) {
+        r.db_gate = fresh(Shape({hidden}));
+        r.db_up = fresh(Shape({hidden}));
+    }
+    const auto dt = static_cast<ttamd_dtype>(input.dtype());
+    std::size_t bytes = 0;
+    check(ttamd_gated_linear_workspace(dt, rows, inner, hidden, 1, &bytes));
+    StorageAMD ws(bytes ? bytes : 1, input.device().id);
+    const ttamd_view2 x = detail::view2(input), wg = detail::view2(w_gate), wu = detail::view2(w_up);
+    check(ttamd_gated_linear_backward(input.device().id, dt, act, rows, inner, hidden, dh.data_ptr(), &x, &wg, &wu, g.data_ptr(), u.data_ptr(),
+                                      r.dx.data_ptr(), r.dw_gate.data_ptr(), r.dw_up.data_ptr(), bias_grad ? r.db_gate->data_ptr() : nullptr,
+                                      bias_grad ? r.db_up->data_ptr() : nullptr, ws.ptr_, bytes, nullptr));
+    return r;
+}
+
+// Distillation from a teacher's top logits: the sum over rows of row_weight (none: 1 / rows) * temperature^2 * KL(teacher's
+// softmax over its slots || softmax of input), and its gradient with respect to input.
+struct DistillLoss {
+    Tensor loss, grad_input;
+};
+inline auto distill_loss(const Tensor &input, const Tensor &teacher_index, const Tensor &teacher_logit, double temperature = 1.0,
+                         const Tensor *row_weight = nullptr) -> DistillLoss {
+    if (input.dim() != 2 || teacher_logit.dim() != 2 || !(teacher_index.shape() == teacher_logit.shape()) || teacher_logit.size(0) != input.size(0))
+        throw TTException("distill_loss: input must be [rows, cols], teacher_index and teacher_logit [rows, top]");
+    detail::check_floats("distill_loss", input, {&teacher_logit, row_weight});
+    const int rows = input.size(0), cols = input.size(1), top = teacher_logit.size(1);
+    if (row_weight && (row_weight->dim() != 1 || row_weight->size(0) != rows)) throw TTException("distill_loss: row_weight must hold an element a row");
+    const Tensor idx = detail::indices("distill_loss", teacher_index, input.device()), logit = teacher_logit.contiguous(), z = input.contiguous();
+    std::optional<Tensor> w;
+    if (row_weight) w = row_weight->contiguous();
+    DistillLoss r;
+    r.loss = Tensor::empty(Shape({1}), input.dtype(), input.device());
+    r.grad_input = Tensor::empty(Shape({rows, cols}), input.dtype(), input.device());
+    const auto dt = static_cast<ttamd_dtype>(input.dtype());
+    std::size_t bytes = 0;
+    check(ttamd_distill_loss_workspace(dt, rows, cols, top, &bytes));
+    StorageAMD ws(bytes ? bytes : 1, input.device().id);
+    check(ttamd_distill_loss(input.device().id, dt, static_cast<ttamd_dtype>(idx.dtype()), rows, cols, top, z.data_ptr(), cols, idx.data_ptr(),
+                             logit.data_ptr(), w ? w->data_ptr() : nullptr, temperature, r.loss.data_ptr(), r.grad_input.data_ptr(), ws.ptr_, bytes, nullptr));
+    return r;
+}
 }  // namespace nn
 
 }  // namespace tt_amd
