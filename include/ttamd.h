@@ -338,10 +338,11 @@ ttamd_status ttamd_linear_mse_head(int device, ttamd_dtype dtype, int64_t rows, 
 
 /* ---- operators of a language-model student: tokens in, a gated block, a teacher's logits as the target ----------------
  * No counterpart in the reference; they stand beside nn::Linear (nn/linear.cpp:42-50) and nn::mse_loss
- * (nn/loss.cpp:69-72).  f32 / f64.  Results are dense row-major and may not overlap an operand.  A `workspace` is device
- * memory of the size that the matching _workspace call names (host arithmetic only), the caller's own for the call: calls
- * that may run at the same time, and graphs that may be replayed at the same time, need one each.  Nothing is kept in it
- * between calls.  Only kernels are enqueued (no memset or copy nodes).  Results are the same bits on every call. */
+ * (nn/loss.cpp:69-72).  f32 / f64.  Results are dense row-major and may not overlap an operand or one another.  A
+ * `workspace` is device memory of the size that the matching _workspace call names (host arithmetic only; where it names 0,
+ * NULL will do), aligned to 16 bytes and the caller's own for the call: calls that may run at the same time, and graphs
+ * that may be replayed at the same time, need one each.  Nothing is kept in it between calls.  Only kernels are enqueued
+ * (no memset or copy nodes).  Results are the same bits on every call. */
 
 /* Rows of a table by token: out[i, :] = scale * table[index[i], :] for i < count, out dense [count, dim].  index: dense,
  * i32 or i64.  table: element (v, d) at table[v * row_stride + d * col_stride], strides >= 0 (a transposed weight is read

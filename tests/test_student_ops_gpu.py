@@ -454,7 +454,7 @@ def distill_data(r, rows, cols, top, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows, cols, top", [(1, 1, 1), (3, 2, 2), (5, 3, 1), (4, 10, 4), (130, 10, 10), (7, 17, 5), (3, 64, 8), (9, 65, 33), (2, 257, 64),
                                              (5, 1000, 100), (3, 1024, 7), (3, 1025, 64), (2, 2051, 300), (6, 4096, 64), (3, 8191, 1), (2, 8200, 1024),
-                                             (2, 16390, 16), (1, 33001, 128), (3, 65537, 70), (2, 98305, 33), (1, 131073, 64), (140, 5000, 12), (2, 200003, 9),
+                                             (2, 16390, 16), (1, 33001, 128), (3, 65537, 70), (2, 98305, 33), (2, 90000, 1024), (1, 150001, 300), (1, 131073, 64), (140, 5000, 12), (2, 200003, 9),
                                              (300, 2000, 3), (0, 8, 2), (2, 3, 300),
                                              (5, 1, 1024), (3, 70, 1000), (4, 2, 65), (3, 64, 64), (3, 63, 257), (2, 1024, 256), (2, 900, 257)])
 def test_distill_loss(tt, dtype, rows, cols, top):
@@ -489,8 +489,28 @@ def test_distill_loss_many_long_rows(tt, dtype, rows, cols):
     assert abs(loss.to_numpy()[0] - want) <= U[dtype] * (sum(each[of[i]][3] * float(w[i]) for i in range(rows)) + abs(want))
 
 
+def test_distill_loss_of_millions_of_rows(tt):
+    """More rows than one launch takes."""
+    rows, cols = (1 << 21) + 37, 3
+    r = rng_of(rows)
+    z, t = r.normal(0, 1, (rows, cols)).astype(np.float32), r.normal(0, 1, (rows, 2)).astype(np.float32)
+    ids = np.stack([r.integers(0, cols, rows), r.integers(-1, cols, rows)], 1).astype(np.int32)
+    T = tt.Tensor.from_numpy
+    w = np.full(rows, 1.0, np.float32)
+    _, got = tt.distill_loss(T(z), T(ids), T(t), row_weight=T(w))
+    q = np.exp(z.astype(np.float64))
+    q /= q.sum(1, keepdims=True)
+    p = np.where(ids >= 0, np.exp(t.astype(np.float64)), 0)
+    p /= p.sum(1, keepdims=True)
+    for k in range(2):
+        ok = ids[:, k] >= 0
+        q[np.flatnonzero(ok), ids[ok, k]] -= p[ok, k]
+    # (exponentials of arguments up to 12: 52 u, the sums and quotients of three and two terms some ten more, twice)
+    assert np.max(np.abs(got.to_numpy() - q)) <= 150 * U[np.float32]
+
+
 # sizes of every way through the operator: tiny rows, a wave, workgroups of several sizes, rows cut into parts
-MASK_SIZES = [(6, 12), (6, 300), (6, 3001), (6, 20000), (150, 9000), (130, 70001)]
+MASK_SIZES = [(6, 12), (6, 300), (6, 3001), (6, 20000), (150, 9000), (6, 90001), (130, 70001)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -47,7 +47,7 @@ struct DistillArgs {
     const T *weight;      // [rows] or null: 1 / rows
     T *grad;              // [rows, cols]
     double *row_loss;     // [rows] scratch
-    int64_t rows;
+    int64_t rows, row0;   // row0: first row of the launch
     int cols, top, index64;
     double temperature;
     T c;                  // factor of exp_scaled: log2(e) / T for float, 1 / T for double
@@ -55,12 +55,14 @@ struct DistillArgs {
 };
 
 // What a row's slots come to, in LDS.  p is 0 in a slot that does not count: an index outside the columns, a logit of -inf.
+// The arrays are padded to whole vectors with slots of no column.
 template <typename T>
 struct Slots {
     T *p, *z;
     int *index;
-    static size_t bytes(int64_t top) { return (static_cast<size_t>(top) * (2 * sizeof(T) + sizeof(int)) + 15) / 16 * 16; }
-    __device__ __forceinline__ Slots(void *lds, int top) : p(static_cast<T *>(lds)), z(p + top), index(reinterpret_cast<int *>(z + top)) {}
+    static constexpr __host__ __device__ int64_t padded(int64_t top) { return (top + 3) / 4 * 4; }
+    static size_t bytes(int64_t top) { return static_cast<size_t>(padded(top)) * (2 * sizeof(T) + sizeof(int)); }
+    __device__ __forceinline__ Slots(void *lds, int top) : p(static_cast<T *>(lds)), z(p + padded(top)), index(reinterpret_cast<int *>(z + padded(top))) {}
 };
 
 template <typename T>
@@ -83,15 +85,17 @@ __device__ __forceinline__ int slot_index(const DistillArgs<T> &a, int64_t row, 
     return i >= 0 && i < a.cols ? static_cast<int>(i) : -1;
 }
 
-// One wave reads the row's slots into `s` (probabilities, student logits, indices); false when none counts, and the row
-// then contributes nothing.
-template <typename T>
-__device__ __forceinline__ bool read_slots(const DistillArgs<T> &a, int64_t row, int lane, const Slots<T> &s) {
+// The slots in three steps, each lane with every BT-th of them, between the row's own reductions: what the indices, the
+// teacher's and the student's logits are (returns the lane's largest teacher logit, NaN if one is NaN); the exponentials
+// (returns their sum); the probabilities (returns T^2 sum_j p_j (log p_j - log q_j) with log q_j = (z_j - m) / T - log(total),
+// terms and sum in 64 bits).
+template <typename T, int BT>
+__device__ __forceinline__ T slots_read(const DistillArgs<T> &a, int64_t row, const Slots<T> &s) {
     const T *zr = a.z + row * a.z_row;
     T most = Num<T>::neg_inf();
     bool nan = false;
-    for (int j = lane; j < a.top; j += 64) {
-        const int i = slot_index(a, row, j);
+    for (int j = threadIdx.x; j < Slots<T>::padded(a.top); j += BT) {
+        const int i = j < a.top ? slot_index(a, row, j) : -1;
         const T t = i >= 0 ? a.teacher[row * a.top + j] : Num<T>::neg_inf();
         s.index[j] = i;
         s.p[j] = t;
@@ -99,38 +103,74 @@ __device__ __forceinline__ bool read_slots(const DistillArgs<T> &a, int64_t row,
         most = Num<T>::max_(most, t);
         nan = nan || t != t;
     }
-    most = wave_max(most);
-    if (most == Num<T>::neg_inf() && !__any(nan)) return false;
+    return __any(nan) ? T(__builtin_nan("")) : wave_max(most);
+}
+template <typename T, int BT>
+__device__ __forceinline__ T slots_exp(const DistillArgs<T> &a, const Slots<T> &s, T most) {
     T sum = T(0);
-    for (int j = lane; j < a.top; j += 64) {
+    for (int j = threadIdx.x; j < Slots<T>::padded(a.top); j += BT) {
         const T e = s.index[j] >= 0 ? Num<T>::exp_scaled(s.p[j] - most, a.c) : T(0);
         s.p[j] = e;
         sum += e;
     }
-    sum = wave_sum(sum);
-    for (int j = lane; j < a.top; j += 64) s.p[j] /= sum;
-    return true;
+    return wave_sum(sum);
 }
-
-// One wave: T^2 sum_j p_j (log p_j - log q_j), log q_j = (z_j - m) / T - log(total); terms and sum in 64 bits.
-template <typename T>
-__device__ __forceinline__ double slots_loss(const DistillArgs<T> &a, int lane, const Slots<T> &s, T most, T total) {
+template <typename T, int BT>
+__device__ __forceinline__ double slots_loss(const DistillArgs<T> &a, const Slots<T> &s, T sum, T most, T total) {
     const double inv = 1.0 / a.temperature, log_total = log(static_cast<double>(total));
-    double sum = 0;
-    for (int j = lane; j < a.top; j += 64) {
-        const double p = s.p[j];
-        if (p != 0.0) sum += p * (log(p) - ((static_cast<double>(s.z[j]) - static_cast<double>(most)) * inv - log_total));  // (p = 0: the term is 0 whatever q is)
+    double loss = 0;
+    for (int j = threadIdx.x; j < Slots<T>::padded(a.top); j += BT) {
+        const T pj = s.p[j] / sum;
+        s.p[j] = pj;
+        const double p = s.index[j] >= 0 ? static_cast<double>(pj) : 0.0;
+        if (p != 0.0) loss += p * (log(p) - ((static_cast<double>(s.z[j]) - static_cast<double>(most)) * inv - log_total));  // (p = 0: the term is 0 whatever q is)
     }
-    return a.temperature * a.temperature * wave_sum(sum);
+    return a.temperature * a.temperature * wave_sum(loss);
 }
 
-// p summed over the slots with slot j's index (a teacher may name a column twice), in slot order.
-template <typename T>
-__device__ __forceinline__ T slot_share(const Slots<T> &s, int top, int j) {
-    const int i = s.index[j];
-    T sum = T(0);
-    for (int k = 0; k < top; ++k) sum += s.index[k] == i ? s.p[k] : T(0);
-    return sum;
+// The waves' values put together: largest (a NaN among them wins) or sum, in wave order.  `lds`: a place a wave.
+template <typename T, int NW, bool MAX>
+__device__ __forceinline__ T join_waves(const T *lds) {
+    T r = lds[0];
+    bool nan = r != r;
+#pragma unroll
+    for (int i = 1; i < NW; ++i) {
+        if constexpr (MAX) {
+            nan = nan || lds[i] != lds[i];
+            r = Num<T>::max_(r, lds[i]);
+        } else {
+            r += lds[i];
+        }
+    }
+    return MAX && nan ? T(__builtin_nan("")) : r;
+}
+
+// The teacher's columns of the gradient, over its bulk: w T (q - the p of all slots with this column, which a teacher may name
+// twice).  Neighbouring lanes share a slot (as many as there are lanes for it, up to 16): each adds up a stretch of the
+// slots, four a step, and the stretches are added in a fixed tree.
+template <typename T, int BT>
+__device__ __forceinline__ void write_slots(const DistillArgs<T> &a, const Slots<T> &s, T *grad, T most, T f, T wt, int c0, int c1, int c2) {
+    typedef int idx4 __attribute__((ext_vector_type(4)));
+    typedef T val4 __attribute__((ext_vector_type(4), aligned(16)));
+    const int padded = static_cast<int>(Slots<T>::padded(a.top));
+    int share = 1;
+    while (share < 16 && 2 * share * a.top <= BT) share *= 2;
+    const int stretch = (padded / 4 + share - 1) / share * 4, part = threadIdx.x & (share - 1);
+    const int k0 = part * stretch, k1 = k0 + stretch < padded ? k0 + stretch : padded;
+    for (int j0 = 0; j0 < a.top; j0 += BT / share) {  // (every lane takes part in the shuffles)
+        const int j = j0 + threadIdx.x / share;
+        const int i = j < a.top ? s.index[j] : -1;
+        T sum = T(0);
+        for (int k = k0; k < k1; k += 4) {
+            const idx4 at = *reinterpret_cast<const idx4 *>(s.index + k);
+            const val4 p = *reinterpret_cast<const val4 *>(s.p + k);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum += at[u] == i ? p[u] : T(0);
+        }
+        for (int d = 1; d < share; d *= 2) sum += __shfl_xor(sum, d, 64);
+        // columns of this workgroup: [c0, c1) and those from c2 on
+        if (part == 0 && i >= 0 && ((i >= c0 && i < c1) || i >= c2)) grad[i] = Num<T>::exp_scaled(s.z[j] - most, a.c) * f - wt * sum;
+    }
 }
 
 template <typename T, int BT, bool MAX>
@@ -175,10 +215,11 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int l
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     lds_t *const more = reinterpret_cast<lds_t *>(smem);  // [lds_vecs][BT]
     const Slots<T> slots(smem + static_cast<size_t>(lds_vecs) * BT * sizeof(lds_t), a.top);
-    __shared__ T red[2][BT / 64];
-    __shared__ int counts;
-    const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid % 64;
+    constexpr int NW = BT / 64;
+    __shared__ T red[4][NW];
+    __shared__ double loss_of[NW];
+    const int64_t row = a.row0 + blockIdx.x;
+    const int tid = threadIdx.x, wave = tid / 64;
     const T *zr = a.z + row * a.z_row;
     T *gr = a.grad + row * a.cols;
     const int nvec = a.cols / W, tail = nvec * W + tid;
@@ -187,10 +228,8 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int l
         empty_row<T, BT>(a, row);
         return;
     }
-    if (tid < 64) {  // (while the other waves request the row; with the vectors already held it would run out of registers)
-        const bool on = read_slots(a, row, lane, slots);
-        if (tid == 0) counts = on;
-    }
+    // (before the row is held: with the vectors in registers the longest rows would run out of them)
+    const T tmost_wave = slots_read<T, BT>(a, row, slots);
     // Every lane requests its vectors before any is used.  A place behind the row's end repeats the last vector and is set
     // to -inf afterwards, which leaves the maximum alone and adds 0 to the sum: a branch around each load would wait for
     // each load.  (A row shorter than a vector comes here for its many slots; it requests its first column for nothing.)
@@ -233,7 +272,13 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int l
             most = Num<T>::max_(most, held[i][k]);
         }
     }
-    most = block_reduce<T, BT, true>(most, red[0]);
+    most = wave_max(most);
+    if (tid % 64 == 0) {
+        red[0][wave] = most;
+        red[1][wave] = tmost_wave;
+    }
+    __syncthreads();
+    most = join_waves<T, NW, true>(red[0]);
     T total = T(0);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -258,11 +303,15 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int l
     }
     last = tail < a.cols ? Num<T>::exp_scaled(last - most, a.c) : T(0);
     total += last;
-    total = block_reduce<T, BT, false>(total, red[1]);
-    if (!counts) {
+    total = wave_sum(total);
+    if (tid % 64 == 0) red[2][wave] = total;
+    __syncthreads();
+    const T tmost = join_waves<T, NW, true>(red[1]);
+    if (tmost == Num<T>::neg_inf()) {  // (no slot counts; the same for the whole workgroup)
         empty_row<T, BT>(a, row);
         return;
     }
+    total = join_waves<T, NW, false>(red[2]);
     const T wt = w * static_cast<T>(a.temperature), f = wt / total;
     const auto put = [&](int v, V x) {
         if constexpr (NT) __builtin_nontemporal_store(x, &reinterpret_cast<V *>(gr)[v]);
@@ -287,22 +336,22 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int l
         put(v, x);
     }
     if (tail < a.cols) gr[tail] = last * f;
-    if (tid < 64) {
-        const double loss = slots_loss(a, lane, slots, most, total);
-        if (tid == 0) a.row_loss[row] = static_cast<double>(w) * loss;
-    }
+    const T tsum_wave = slots_exp<T, BT>(a, slots, tmost);  // (now that the row's vectors have left the registers)
+    if (tid % 64 == 0) red[3][wave] = tsum_wave;
+    __syncthreads();
+    const double loss = slots_loss<T, BT>(a, slots, join_waves<T, NW, false>(red[3]), most, total);
+    if (tid % 64 == 0) loss_of[wave] = loss;
     __syncthreads();  // the gradient's bulk comes first, the teacher's columns are written over it
-    for (int j = tid; j < a.top; j += BT)
-        if (slots.index[j] >= 0)
-            gr[slots.index[j]] = Num<T>::exp_scaled(slots.z[j] - most, a.c) * f - wt * slot_share(slots, a.top, j);
+    if (tid == 0) a.row_loss[row] = static_cast<double>(w) * join_waves<double, NW, false>(loss_of);
+    write_slots<T, BT>(a, slots, gr, most, f, wt, 0, a.cols, a.cols);
 }
 
-// Short rows: G lanes own a row, E columns each (lane l: columns l, l + G, ..), up to 4 G slots.  Everything stays in
+// Short rows: G lanes own a row, E columns each (lane l: columns l, l + G, ..), up to 64 slots.  Everything stays in
 // registers; the slots go round the group one by one and the lane that holds a slot's column takes its share off.
 template <typename T, int G, int E>
 __global__ void __launch_bounds__(256) distill_short_kernel(DistillArgs<T> a) {
-    constexpr int S = 4;  // slots a lane
-    const int64_t row_of = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / G;
+    constexpr int S = 64 / G;  // slots a lane
+    const int64_t row_of = a.row0 + (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / G;
     const bool live = row_of < a.rows;
     const int64_t row = live ? row_of : a.rows - 1;  // (every lane takes part in the shuffles)
     const int lane = threadIdx.x % G;
@@ -443,42 +492,51 @@ __global__ void __launch_bounds__(kPartThreads) distill_part_kernel(DistillArgs<
 template <typename T>
 __global__ void __launch_bounds__(kPartThreads) distill_join_kernel(DistillArgs<T> a, const PartSums<T> *parts) {
     using V = typename Num<T>::vec_t;
-    constexpr int W = Num<T>::W;
+    constexpr int W = Num<T>::W, NW = kPartThreads / 64;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const Slots<T> slots(smem, a.top);
-    __shared__ T red[2][kPartThreads / 64];
-    __shared__ int counts;
+    __shared__ T red[4][NW];
+    __shared__ double loss_of[NW];
     const int64_t row = blockIdx.y;
-    const int tid = threadIdx.x, lane = tid % 64;
+    const int tid = threadIdx.x, wave = tid / 64;
     const T *zr = a.z + row * a.z_row;
     T *gr = a.grad + row * a.cols;
     const int nvec = a.cols / W, first = blockIdx.x * (kPartThreads * kPartVecs) + tid;
     const int tail = nvec * W + tid;
     const T w = a.weight ? a.weight[row] : a.uniform_weight;
-    const bool mine = blockIdx.x == 0;
+    const bool mine = blockIdx.x == 0;  // the row's loss and its columns behind the last whole vector
     V x[kPartVecs];
-    T last = Num<T>::neg_inf();
-    if (w != T(0)) {
+    T last = Num<T>::neg_inf(), most = Num<T>::neg_inf(), total = T(0), tmost = Num<T>::neg_inf(), tsum = T(0);
+    if (w != T(0)) {  // (the same for the whole workgroup)
 #pragma unroll
         for (int i = 0; i < kPartVecs; ++i) {
             const int v = first + i * kPartThreads;
             x[i] = reinterpret_cast<const V *>(zr)[v < nvec ? v : nvec - 1];
         }
         if (mine && tail < a.cols) last = zr[tail];
-        if (tid < 64) {
-            const bool on = read_slots(a, row, lane, slots);
-            if (tid == 0) counts = on;
-        }
-    }
-    T most = Num<T>::neg_inf(), total = T(0);
-    if (w != T(0)) {
         const PartSums<T> *own = parts + row * gridDim.x;
         for (int i = tid; i < static_cast<int>(gridDim.x); i += kPartThreads) most = Num<T>::max_(most, own[i].most);
-        most = block_reduce<T, kPartThreads, true>(most, red[0]);
+        most = wave_max(most);
+        tmost = slots_read<T, kPartThreads>(a, row, slots);
+        if (tid % 64 == 0) {
+            red[0][wave] = most;
+            red[1][wave] = tmost;
+        }
+        __syncthreads();
+        most = join_waves<T, NW, true>(red[0]);
+        tmost = join_waves<T, NW, true>(red[1]);
         for (int i = tid; i < static_cast<int>(gridDim.x); i += kPartThreads) total += own[i].total * Num<T>::exp_scaled(own[i].most - most, a.c);
-        total = block_reduce<T, kPartThreads, false>(total, red[1]);
+        total = wave_sum(total);
+        tsum = slots_exp<T, kPartThreads>(a, slots, tmost);
+        if (tid % 64 == 0) {
+            red[2][wave] = total;
+            red[3][wave] = tsum;
+        }
+        __syncthreads();
+        total = join_waves<T, NW, false>(red[2]);
+        tsum = join_waves<T, NW, false>(red[3]);
     }
-    const bool on = w != T(0) && counts;  // (counts: written before the reductions' barriers)
+    const bool on = w != T(0) && tmost != Num<T>::neg_inf();
     const T wt = w * static_cast<T>(a.temperature), f = wt / total;
 #pragma unroll
     for (int i = 0; i < kPartVecs; ++i) {
@@ -488,18 +546,16 @@ __global__ void __launch_bounds__(kPartThreads) distill_join_kernel(DistillArgs<
         if (v < nvec) reinterpret_cast<V *>(gr)[v] = x[i];
     }
     if (mine && tail < a.cols) gr[tail] = on ? Num<T>::exp_scaled(last - most, a.c) * f : T(0);
-    if (mine && tid < 64) {
-        const double loss = on ? slots_loss(a, lane, slots, most, total) : 0.0;
-        if (tid == 0) a.row_loss[row] = on ? static_cast<double>(w) * loss : 0.0;
+    if (!on) {
+        if (mine && tid == 0) a.row_loss[row] = 0.0;
+        return;
     }
-    if (!on) return;
+    const double loss = slots_loss<T, kPartThreads>(a, slots, tsum, most, total);
+    if (tid % 64 == 0) loss_of[wave] = loss;
     __syncthreads();  // the bulk first, then the teacher's columns that lie in this part
-    const int c0 = blockIdx.x * (kPartThreads * kPartVecs * W), c1 = c0 + kPartThreads * kPartVecs * W;
-    for (int j = tid; j < a.top; j += kPartThreads) {
-        const int c = slots.index[j];
-        if (c >= 0 && (c >= nvec * W ? mine : c >= c0 && c < c1))
-            gr[c] = Num<T>::exp_scaled(slots.z[j] - most, a.c) * f - wt * slot_share(slots, a.top, j);
-    }
+    if (mine && tid == 0) a.row_loss[row] = static_cast<double>(w) * join_waves<double, NW, false>(loss_of);
+    const int c0 = blockIdx.x * (kPartThreads * kPartVecs * W), c1 = c0 + kPartThreads * kPartVecs * W, whole = nvec * W;
+    write_slots<T, kPartThreads>(a, slots, gr, most, f, wt, c0, c1 < whole ? c1 : whole, mine ? whole : a.cols);
 }
 
 // loss = sum of the rows' losses: a lane adds every 1024th, the lanes are added in a fixed order.
@@ -518,16 +574,18 @@ size_t part_offset(int64_t rows) { return (static_cast<size_t>(rows) * sizeof(do
 int64_t parts_of(size_t item, int64_t rows, int64_t cols) {
     const int64_t vec = 16 / static_cast<int64_t>(item), per = kPartThreads * kPartVecs * vec;
     const int64_t row_bytes = cols * static_cast<int64_t>(item);
-    return rows <= 128 && row_bytes > 32768 ? (cols + per - 1) / per : 0;
+    // (a third launch must pay: 16 x 131072 f32 21 us against 24 with a workgroup a row, 64 x 131072 21 against 33, 1 x 131072
+    // f64 20 against 68; but 64 x 65000 f32 21 against 17, 200 x 131072 57 against 54)
+    return rows <= 128 && row_bytes > 320 * 1024 ? (cols + per - 1) / per : 0;
 }
 
 template <typename T>
-ttamd_status launch_rows(const DistillArgs<T> &a, void *parts, hipStream_t st) {
+ttamd_status launch_some_rows(const DistillArgs<T> &a, int64_t rows, void *parts, hipStream_t st) {
     const size_t slots = Slots<T>::bytes(a.top);
     if (a.cols <= 64 && a.top <= 64) {
-        distill_short_kernel<T, 16, 4><<<static_cast<unsigned>((a.rows + 15) / 16), 256, 0, st>>>(a);
-    } else if (a.cols <= 1024 && a.top <= 256) {
-        distill_short_kernel<T, 64, 16><<<static_cast<unsigned>((a.rows + 3) / 4), 256, 0, st>>>(a);
+        distill_short_kernel<T, 16, 4><<<static_cast<unsigned>((rows + 15) / 16), 256, 0, st>>>(a);
+    } else if (a.cols <= 1024 && a.top <= 32) {  // (the slots go one by one: 4096 x 1000 f32 17 us with 16 of them, with 64 29 against 24)
+        distill_short_kernel<T, 64, 16><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(a);
     } else if (const int64_t n = parts_of(sizeof(T), a.rows, a.cols)) {
         const dim3 grid(static_cast<unsigned>(n), static_cast<unsigned>(a.rows));
         distill_part_kernel<T><<<grid, kPartThreads, 0, st>>>(a, static_cast<PartSums<T> *>(parts));
@@ -542,7 +600,7 @@ ttamd_status launch_rows(const DistillArgs<T> &a, void *parts, hipStream_t st) {
             const size_t lds = static_cast<size_t>(lds_vecs) * threads * 16 + slots;
             if (lds > 48 * 1024)
                 TTAMD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-            kernel<<<static_cast<unsigned>(a.rows), threads, lds, st>>>(a, static_cast<int>(lds_vecs));
+            kernel<<<static_cast<unsigned>(rows), threads, lds, st>>>(a, static_cast<int>(lds_vecs));
             return TTAMD_OK;
         };
         // The smallest form that keeps the row: small workgroups share a CU and one's loads run under another's stores
@@ -563,6 +621,15 @@ ttamd_status launch_rows(const DistillArgs<T> &a, void *parts, hipStream_t st) {
         if (ttamd_status s = beyond ? pick.template operator()<true>() : pick.template operator()<false>()) return s;
     }
     TTAMD_HIP_CHECK(hipGetLastError());
+    return TTAMD_OK;
+}
+
+// A launch holds fewer than 2^32 lanes: rows beyond kLaunchRows go to launches of their own.
+constexpr int64_t kLaunchRows = int64_t(1) << 21;
+template <typename T>
+ttamd_status launch_rows(DistillArgs<T> a, void *parts, hipStream_t st) {
+    for (a.row0 = 0; a.row0 < a.rows; a.row0 += kLaunchRows)
+        if (ttamd_status s = launch_some_rows(a, a.rows - a.row0 < kLaunchRows ? a.rows - a.row0 : kLaunchRows, parts, st)) return s;
     return TTAMD_OK;
 }
 
@@ -598,8 +665,8 @@ ttamd_status check_distill_shape(ttamd_dtype dtype, int64_t rows, int64_t cols, 
         set_error("distill_loss: floating point dtypes only");
         return TTAMD_ERR_UNSUPPORTED_DTYPE;
     }
-    if (rows < 0 || cols < 1 || top < 1 || rows > 0x7fffffffLL || cols > 0x3fffffffLL || top > kMaxTop) {
-        set_error("distill_loss: rows %lld, cols %lld, top %lld: fewer than 2^31 rows, 1 to 2^30 - 1 columns, 1 to %d teacher slots",
+    if (rows < 0 || cols < 1 || top < 1 || rows > 0x7fffffffLL || cols > 0x3fffffffLL || rows * cols > int64_t(1) << 40 || top > kMaxTop) {
+        set_error("distill_loss: rows %lld, cols %lld, top %lld: fewer than 2^31 rows, 1 to 2^30 - 1 columns, 2^40 elements at most, 1 to %d teacher slots",
                   static_cast<long long>(rows), static_cast<long long>(cols), static_cast<long long>(top), kMaxTop);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
@@ -648,8 +715,8 @@ ttamd_status ttamd_distill_loss(int device, ttamd_dtype dtype, ttamd_dtype index
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
     if (misaligned(input, e) || misaligned(teacher_logit, e) || misaligned(row_weight, e) || misaligned(loss_out, e) ||
-        misaligned(grad_input_out, e) || misaligned(teacher_index, ie) || misaligned(workspace, sizeof(double))) {
-        set_error("distill_loss: pointers must be aligned to the element size, the workspace to 8 bytes");
+        misaligned(grad_input_out, e) || misaligned(teacher_index, ie) || misaligned(workspace, 16)) {
+        set_error("distill_loss: pointers must be aligned to the element size, the workspace to 16 bytes");
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
     if (workspace_bytes < need) {

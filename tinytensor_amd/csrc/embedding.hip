@@ -694,8 +694,8 @@ ttamd_status ttamd_embedding_backward(int device, ttamd_dtype dtype, ttamd_dtype
         set_error("%s: NULL data pointer", what);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
-    if (misaligned(grad_out, e) || misaligned(grad_table, e) || misaligned(index, dtype_size(index_dtype)) || misaligned(workspace, sizeof(double))) {
-        set_error("%s: pointers must be aligned to the element size, the workspace to 8 bytes", what);
+    if (misaligned(grad_out, e) || misaligned(grad_table, e) || misaligned(index, dtype_size(index_dtype)) || (need > 0 && misaligned(workspace, 16))) {
+        set_error("%s: pointers must be aligned to the element size, the workspace to 16 bytes", what);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
     if (workspace_bytes < need) {
