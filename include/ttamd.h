@@ -354,7 +354,7 @@ ttamd_status ttamd_embedding_forward(int device, ttamd_dtype dtype, ttamd_dtype 
 /* Its gradient: grad_table[v, :] = scale * sum of grad_out[i, :] over the i with index[i] == v, for every v < vocab (zeros
  * where there is none); accumulate != 0: grad_table += that, rows without a position are left alone.  grad_out
  * [count, dim] and grad_table [vocab, dim] dense.  Sums run over the positions in groups whose order the indices fix, in
- * 64 bits.  Up to 128 positions need no workspace. */
+ * 64 bits.  Up to 128 positions need no workspace.  Beyond 2^17 rows of the table, count * vocab <= 2^48. */
 ttamd_status ttamd_embedding_backward_workspace(ttamd_dtype dtype, int64_t count, int64_t vocab, int64_t dim, size_t *bytes);
 ttamd_status ttamd_embedding_backward(int device, ttamd_dtype dtype, ttamd_dtype index_dtype, int64_t count, int64_t vocab,
                                       int64_t dim, const void *grad_out, const void *index, double scale, int accumulate,
@@ -363,7 +363,7 @@ ttamd_status ttamd_embedding_backward(int device, ttamd_dtype dtype, ttamd_dtype
 /* The gated pair of Linear layers of a feed-forward block: g = x . Wg + bg, u = x . Wu + bu, out = act(g) * u.
  * input [rows, inner], gate_weight and up_weight [inner, hidden]: any non-negative strides, read in place.  gate_bias,
  * up_bias: dense [hidden], each may be NULL.  out [rows, hidden].  gate_out / up_out: both or neither; they receive g and
- * u, what the backward pass reads.  gelu is the exact (erf) form. */
+ * u, what the backward pass reads.  gelu is the exact (erf) form.  rows <= 2^28, inner and hidden <= 2^26, strides <= 2^32. */
 typedef enum ttamd_activation { TTAMD_ACT_SILU = 0, TTAMD_ACT_GELU = 1, TTAMD_ACT_RELU = 2, TTAMD_ACT_SIGMOID = 3 } ttamd_activation;
 ttamd_status ttamd_gated_linear_workspace(ttamd_dtype dtype, int64_t rows, int64_t inner, int64_t hidden, int backward,
                                           size_t *bytes);

@@ -40,6 +40,11 @@ def test_embedding_backward_refusals(tt):
     assert query(capi.I32, 4, 10, 8, C.byref(n)) == capi.ERR_UNSUPPORTED_DTYPE
     assert query(capi.F32, 4, 0, 8, C.byref(n)) == capi.ERR_INVALID_ARGUMENT
     assert query(capi.F32, 4, 10, 8, None) == capi.ERR_INVALID_ARGUMENT
+    # a long list of positions of a huge table, which would keep the device busy for minutes
+    assert query(capi.F32, 1 << 30, 1 << 28, 1, C.byref(n)) == capi.ERR_INVALID_ARGUMENT
+    assert query(capi.F32, (1 << 20) + 1, 1 << 28, 1, C.byref(n)) == capi.ERR_INVALID_ARGUMENT
+    assert query(capi.F32, 1 << 20, 1 << 28, 1, C.byref(n)) == capi.OK
+    assert query(capi.F32, (1 << 31) - 1, 1 << 17, 1, C.byref(n)) == capi.OK
     assert query(capi.F32, 4, 10, 8, C.byref(n)) == capi.OK and n.value == 0  # few positions need none
     assert query(capi.F32, 400, 10, 8, C.byref(n)) == capi.OK and n.value > 0
     need = n.value
@@ -59,6 +64,10 @@ def test_gated_linear_refusals(tt):
     assert lib.ttamd_gated_linear_workspace(capi.I64, 3, 8, 8, 0, C.byref(n)) == capi.ERR_UNSUPPORTED_DTYPE
     assert lib.ttamd_gated_linear_workspace(capi.F32, 3, 0, 8, 0, C.byref(n)) == capi.ERR_INVALID_ARGUMENT
     assert lib.ttamd_gated_linear_workspace(capi.F32, 3, 8, 8, 0, None) == capi.ERR_INVALID_ARGUMENT
+    for big in (((1 << 28) + 1, 1, 1), (1, (1 << 26) + 1, 1), (1, 1, (1 << 26) + 1), (1 << 28, 1 << 13, 1), (1, 1 << 26, 1 << 15)):
+        assert lib.ttamd_gated_linear_workspace(capi.F32, *big, 1, C.byref(n)) == capi.ERR_INVALID_ARGUMENT, big
+    for large in ((1 << 28, 1, 1), (1, 1 << 26, 1), (1, 1, 1 << 26)):
+        assert lib.ttamd_gated_linear_workspace(capi.F32, *large, 1, C.byref(n)) == capi.OK, large
     assert lib.ttamd_gated_linear_workspace(capi.F32, 3, 8, 8, 1, C.byref(n)) == capi.OK
 
     def forward(dtype=capi.F32, act=0, rows=3, x=view(capi), wg=view(capi), wu=view(capi), out=2 * A, gate=None, up=None, ws=3 * A, size=1 << 30):
@@ -66,7 +75,7 @@ def test_gated_linear_refusals(tt):
 
     assert forward(dtype=capi.I32) == capi.ERR_UNSUPPORTED_DTYPE
     for kw in (dict(act=4), dict(act=-1), dict(rows=-1), dict(x=None), dict(wg=view(capi, data=None)), dict(wu=view(capi, offset=-1)),
-               dict(wu=view(capi, stride=(8, -1))), dict(x=view(capi, data=A + 2)), dict(out=None), dict(out=A + 1), dict(gate=4 * A),
+               dict(wu=view(capi, stride=(8, -1))), dict(x=view(capi, stride=((1 << 32) + 1, 1))), dict(x=view(capi, data=A + 2)), dict(out=None), dict(out=A + 1), dict(gate=4 * A),
                dict(up=4 * A), dict(ws=3 * A + 4)):
         assert forward(**kw) == capi.ERR_INVALID_ARGUMENT, kw
 

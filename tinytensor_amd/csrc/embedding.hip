@@ -678,6 +678,12 @@ ttamd_status ttamd_embedding_backward_workspace(ttamd_dtype dtype, int64_t count
         set_error("embedding_backward: bytes is NULL");
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
+    // Each of vocab / kOrderTokens workgroups looks at every index: half a second's work at this bound.
+    if (count > kFew && vocab > (1 << 17) && count > (int64_t(1) << 48) / vocab) {
+        set_error("embedding_backward: %lld positions of a table of %lld rows: beyond 2^17 rows, positions x rows up to 2^48",
+                  static_cast<long long>(count), static_cast<long long>(vocab));
+        return TTAMD_ERR_INVALID_ARGUMENT;
+    }
     *bytes = count <= kFew ? 0 : plan_backward(dtype_size(dtype), count, vocab, dim).bytes;
     return TTAMD_OK;
 }

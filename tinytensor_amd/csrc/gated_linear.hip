@@ -395,10 +395,11 @@ ttamd_status check_gated(const char *what, ttamd_dtype dtype, int64_t rows, int6
         set_error("%s: floating point dtypes only", what);
         return TTAMD_ERR_UNSUPPORTED_DTYPE;
     }
-    constexpr int64_t most = int64_t(1) << 30;  // (and below 2^40 elements a matrix: every size in bytes fits 64 bits)
-    if (rows < 0 || inner < 1 || hidden < 1 || rows > most || inner > most || hidden > most || rows * inner > most << 10 ||
-        rows * hidden > most << 10 || inner * hidden > most << 10) {
-        set_error("%s: rows %lld, inner %lld, hidden %lld: rows from 0, the others from 1, up to 2^30 each and 2^40 elements a matrix", what,
+    // (a launch holds fewer than 2^32 lanes, and every size in bytes fits 64 bits)
+    constexpr int64_t most_rows = int64_t(1) << 28, most_cols = int64_t(1) << 26, most = int64_t(1) << 40;
+    if (rows < 0 || inner < 1 || hidden < 1 || rows > most_rows || inner > most_cols || hidden > most_cols || rows * inner > most ||
+        rows * hidden > most || inner * hidden > most) {
+        set_error("%s: rows %lld, inner %lld, hidden %lld: rows from 0 to 2^28, the others from 1 to 2^26, 2^40 elements a matrix", what,
                   static_cast<long long>(rows), static_cast<long long>(inner), static_cast<long long>(hidden));
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
@@ -416,8 +417,9 @@ ttamd_status check_view(const char *what, const char *name, const ttamd_view2 *v
         set_error("%s: NULL view or data of %s", what, name);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
-    if (v->offset < 0 || v->stride[0] < 0 || v->stride[1] < 0 || misaligned(v->data, item)) {
-        set_error("%s: %s: negative offset or stride, or a pointer off the element size", what, name);
+    constexpr int64_t most = int64_t(1) << 32;  // (reaches are computed in 64 bits)
+    if (v->offset < 0 || v->stride[0] < 0 || v->stride[1] < 0 || v->stride[0] > most || v->stride[1] > most || misaligned(v->data, item)) {
+        set_error("%s: %s: a negative offset, a stride outside 0 to 2^32, or a pointer off the element size", what, name);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
     return TTAMD_OK;
