@@ -489,6 +489,42 @@ def test_distill_loss_many_long_rows(tt, dtype, rows, cols):
     assert abs(loss.to_numpy()[0] - want) <= U[dtype] * (sum(each[of[i]][3] * float(w[i]) for i in range(rows)) + abs(want))
 
 
+def test_distill_loss_from_two_threads(tt):
+    """Calls that want different amounts of LDS of one kernel, from two threads with a stream each: the results of calls alone."""
+    import ctypes
+    import threading
+    r = rng_of("threads")
+    T, capi, lib = tt.Tensor.from_numpy, tt._capi, tt._capi.lib
+    rows, calls, failed = 140, [], []
+    for cols, top in ((66000, 5), (90000, 900)):     # 1024 lanes with 16 vectors each, and 1 or 6 vectors of LDS
+        z, ids, t = distill_data(r, rows, cols, top, np.float32)
+        ops = [T(z), T(ids.astype(np.int32)), T(t)]
+        want = [x.to_numpy() for x in tt.distill_loss(*ops)]
+        size = ctypes.c_size_t()
+        assert lib.ttamd_distill_loss_workspace(capi.F32, rows, cols, top, ctypes.byref(size)) == capi.OK
+        outs = [tt.Tensor.empty((1,), capi.F32), tt.Tensor.empty((rows, cols), capi.F32), tt.Tensor.empty((size.value // 4,), capi.F32)]
+        stream = tt.graph.Stream(non_blocking=True)
+        z, ids, t, loss, grad, ws = (x.storage.ptr for x in ops + outs)
+        args = (0, capi.F32, capi.I32, rows, cols, top, z, cols, ids, t, None, 1.0, loss, grad, ws, size.value, stream.handle)
+        calls.append((ops, outs, want, stream, args))
+
+    def work(args):
+        for _ in range(20):
+            if lib.ttamd_distill_loss(*args) != capi.OK:
+                failed.append(capi.last_error())
+
+    threads = [threading.Thread(target=work, args=(c[-1],)) for c in calls]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed, failed
+    for ops, (loss, grad, _), want, stream, _ in calls:
+        stream.synchronize()
+        assert np.array_equal(loss.to_numpy(), want[0]) and np.array_equal(grad.to_numpy(), want[1])
+        stream.close()
+
+
 def test_distill_loss_of_millions_of_rows(tt):
     """More rows than one launch takes."""
     rows, cols = (1 << 21) + 37, 3
@@ -507,6 +543,17 @@ def test_distill_loss_of_millions_of_rows(tt):
         q[np.flatnonzero(ok), ids[ok, k]] -= p[ok, k]
     # (exponentials of arguments up to 12: 52 u, the sums and quotients of three and two terms some ten more, twice)
     assert np.max(np.abs(got.to_numpy() - q)) <= 150 * U[np.float32]
+    # the loss of rows at the launches' ends, with all the others masked
+    some = np.array([0, 5, (1 << 21) - 1, 1 << 21, (1 << 21) + 1, rows - 2, rows - 1])
+    w[:] = 0
+    w[some] = 1
+    loss, _ = tt.distill_loss(T(z), T(ids), T(t), row_weight=T(w))
+    want, _, _, rel = distill_reference(z[some], ids[some], t[some], 1.0, np.ones(len(some)))
+    assert abs(loss.to_numpy()[0] - want) <= U[np.float32] * (rel + 2 * abs(want))
+    w[:] = 0
+    w[some] = 1 / 64
+    half, _ = tt.distill_loss(T(z), T(ids), T(t), row_weight=T(w))
+    assert half.to_numpy()[0] == loss.to_numpy()[0] / 64
 
 
 # sizes of every way through the operator: tiny rows, a wave, workgroups of several sizes, rows cut into parts

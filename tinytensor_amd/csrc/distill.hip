@@ -46,7 +46,7 @@ struct DistillArgs {
     const T *teacher;     // [rows, top]
     const T *weight;      // [rows] or null: 1 / rows
     T *grad;              // [rows, cols]
-    double *row_loss;     // [rows] scratch
+    double *row_loss;     // [rows] scratch, or a place for the four rows of a wave (narrow)
     int64_t rows, row0;   // row0: first row of the launch
     int cols, top, index64;
     double temperature;
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DistillArgs<T> a) {
     const int lane = threadIdx.x % G;
     const T *zr = a.z + row * a.z_row;
     const T w = a.weight ? a.weight[row] : a.uniform_weight;
-    T e[E], zs[S], p[S];
+    T e[E], zs[S], t[S], p[S];
     int index[S];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -370,14 +370,16 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DistillArgs<T> a) {
     for (int s = 0; s < S; ++s) {
         const int j = lane + s * G;
         index[s] = -1;
-        p[s] = Num<T>::neg_inf();
+        t[s] = Num<T>::neg_inf();
         if (j < a.top) {
             index[s] = slot_index(a, row, j);
-            if (index[s] >= 0) p[s] = a.teacher[row * a.top + j];
+            if (index[s] >= 0) t[s] = a.teacher[row * a.top + j];
         }
+        zs[s] = T(0);
+        if (s * G >= a.top) continue;  // (no lane has a slot here)
         zs[s] = zr[index[s] >= 0 ? index[s] : 0];
-        tmost = Num<T>::max_(tmost, p[s]);
-        nan |= p[s] != p[s];
+        tmost = Num<T>::max_(tmost, t[s]);
+        nan |= t[s] != t[s];
     }
     T most = Num<T>::neg_inf();
 #pragma unroll
@@ -400,7 +402,9 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DistillArgs<T> a) {
     }
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        p[s] = index[s] >= 0 ? Num<T>::exp_scaled(p[s] - tmost, a.c) : T(0);
+        p[s] = T(0);
+        if (s * G >= a.top) continue;
+        if (index[s] >= 0) p[s] = Num<T>::exp_scaled(t[s] - tmost, a.c);
         ptotal += p[s];
     }
 #pragma unroll
@@ -409,13 +413,17 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DistillArgs<T> a) {
         ptotal += __shfl_xor(ptotal, d, G);
     }
     const bool on = w != T(0) && (tmost != Num<T>::neg_inf() || nan);
-    const double inv = 1.0 / a.temperature, log_total = log(static_cast<double>(total));
+    // log p_j - log q_j = ((t_j - tmost) - (z_j - most)) / T + log(total / ptotal): one logarithm in 64 bits for the whole row
+    // instead of one a slot
+    const double inv = 1.0 / a.temperature, shift = log(static_cast<double>(total) / static_cast<double>(ptotal));
     double loss = 0;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
+        if (s * G >= a.top) continue;
         p[s] /= ptotal;
         const double pj = index[s] >= 0 ? static_cast<double>(p[s]) : 0.0;
-        if (pj != 0.0) loss += pj * (log(pj) - ((static_cast<double>(zs[s]) - static_cast<double>(most)) * inv - log_total));
+        if (pj != 0.0)
+            loss += pj * (((static_cast<double>(t[s]) - static_cast<double>(tmost)) - (static_cast<double>(zs[s]) - static_cast<double>(most))) * inv + shift);
     }
 #pragma unroll
     for (int d = G / 2; d > 0; d /= 2) loss += __shfl_xor(loss, d, G);
@@ -433,13 +441,17 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DistillArgs<T> a) {
             for (int i = 0; i < E; ++i) share[i] += c == lane + i * G ? pk : T(0);
         }
     }
+    // the rows of a wave are added up here (its first row lives if any does)
+    double own = live && on ? static_cast<double>(w) * a.temperature * a.temperature * loss : 0.0;
+#pragma unroll
+    for (int d = G; d < 64; d *= 2) own += __shfl_xor(own, d, 64);
     if (!live) return;
+    if (threadIdx.x % 64 == 0) a.row_loss[row / (64 / G)] = own;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         const int c = lane + i * G;
         if (c < a.cols) a.grad[row * a.cols + c] = on ? e[i] * f - wt * share[i] : T(0);
     }
-    if (lane == 0) a.row_loss[row] = on ? static_cast<double>(w) * a.temperature * a.temperature * loss : 0.0;
 }
 
 // Few long rows: a workgroup has a part of a row, kPartVecs vectors a lane.  The first kernel leaves the part's largest
@@ -558,12 +570,14 @@ __global__ void __launch_bounds__(kPartThreads) distill_join_kernel(DistillArgs<
     write_slots<T, kPartThreads>(a, slots, gr, most, f, wt, c0, c1 < whole ? c1 : whole, mine ? whole : a.cols);
 }
 
-// loss = sum of the rows' losses: a lane adds every 1024th, the lanes are added in a fixed order.
+// loss = sum of the rows' losses (or of what the rows of a wave came to: `n` of them): a lane adds every 1024th, the lanes are
+// added in a fixed order.
 template <typename T>
-__global__ void __launch_bounds__(1024) distill_sum_kernel(const double *row_loss, int64_t rows, T *out) {
+__global__ void __launch_bounds__(1024) distill_sum_kernel(const double *row_loss, int64_t n, T *out) {
     __shared__ double red[16];
     double v = 0;
-    for (int64_t r = threadIdx.x; r < rows; r += 1024) v += row_loss[r];
+#pragma unroll 8
+    for (int64_t r = threadIdx.x; r < n; r += 1024) v += row_loss[r];
     v = block_reduce<double, 1024, false>(v, red);
     if (threadIdx.x == 0) out[0] = static_cast<T>(v);
 }
@@ -579,10 +593,13 @@ int64_t parts_of(size_t item, int64_t rows, int64_t cols) {
     return rows <= 128 && row_bytes > 320 * 1024 ? (cols + per - 1) / per : 0;
 }
 
+// Rows of a few columns: 16 lanes each, four to a wave.
+bool narrow(int64_t cols, int64_t top) { return cols <= 64 && top <= 64; }
+
 template <typename T>
 ttamd_status launch_some_rows(const DistillArgs<T> &a, int64_t rows, void *parts, hipStream_t st) {
     const size_t slots = Slots<T>::bytes(a.top);
-    if (a.cols <= 64 && a.top <= 64) {
+    if (narrow(a.cols, a.top)) {
         distill_short_kernel<T, 16, 4><<<static_cast<unsigned>((rows + 15) / 16), 256, 0, st>>>(a);
     } else if (a.cols <= 1024 && a.top <= 32) {  // (the slots go one by one: 4096 x 1000 f32 17 us with 16 of them, with 64 29 against 24)
         distill_short_kernel<T, 64, 16><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(a);
@@ -598,8 +615,10 @@ ttamd_status launch_some_rows(const DistillArgs<T> &a, int64_t rows, void *parts
             int64_t lds_vecs = left > 0 ? (left + threads - 1) / threads : 0;
             if (lds_vecs > kLdsVecs) lds_vecs = kLdsVecs;
             const size_t lds = static_cast<size_t>(lds_vecs) * threads * 16 + slots;
+            // (the limit of the largest call, whichever comes first: calls of other threads may be between their two steps)
+            const size_t most = static_cast<size_t>(kLdsVecs) * threads * 16 + Slots<T>::bytes(kMaxTop);
             if (lds > 48 * 1024)
-                TTAMD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
+                TTAMD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most)));
             kernel<<<static_cast<unsigned>(rows), threads, lds, st>>>(a, static_cast<int>(lds_vecs));
             return TTAMD_OK;
         };
@@ -655,7 +674,8 @@ ttamd_status launch_distill(int64_t rows, int64_t cols, int64_t top, const void 
         a.uniform_weight = static_cast<T>(1.0 / static_cast<double>(rows));
         if (ttamd_status s = launch_rows(a, static_cast<char *>(workspace) + part_offset(rows), st)) return s;
     }
-    distill_sum_kernel<T><<<1, 1024, 0, st>>>(static_cast<const double *>(workspace), rows, static_cast<T *>(loss_out));
+    const int64_t sums = narrow(cols, top) ? (rows + 3) / 4 : rows;
+    distill_sum_kernel<T><<<1, 1024, 0, st>>>(static_cast<const double *>(workspace), sums, static_cast<T *>(loss_out));
     TTAMD_HIP_CHECK(hipGetLastError());
     return TTAMD_OK;
 }
