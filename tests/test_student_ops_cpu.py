@@ -107,7 +107,58 @@ def test_distill_loss_refusals(tt):
                dict(weight=A + 1), dict(ws=A + 4), dict(grad=A), dict(grad=A + 4 * 16)):
         assert call(**kw) == capi.ERR_INVALID_ARGUMENT, kw
     call(grad=A)
-    assert b"over the logits" in lib.ttamd_last_error_string()
+    assert b"the gradient shares memory with the logits" in lib.ttamd_last_error_string()
+
+
+def test_shared_memory_is_refused(tt):
+    """A result over an operand or another result; what only lies between an operand's rows, or next to it, is left alone."""
+    capi, lib = tt._capi, tt._capi.lib
+
+    def shared(status):
+        return status == capi.ERR_INVALID_ARGUMENT and b"shares memory with" in lib.ttamd_last_error_string()
+
+    # table: rows of 32 bytes, 64 apart (10 of them); out: 128 bytes
+    assert shared(embed(tt, rs=16, out=2 * A + 9 * 64 + 28)) and not shared(embed(tt, rs=16, out=2 * A + 9 * 64 + 32))
+    assert shared(embed(tt, rs=16, out=2 * A - 124)) and not shared(embed(tt, rs=16, out=2 * A - 128))
+    assert shared(embed(tt, count=1, rs=16, out=2 * A + 28)) and not shared(embed(tt, count=1, rs=16, out=2 * A + 32))
+    assert shared(embed(tt, count=1, rs=16, out=2 * A + 36))
+    assert shared(embed(tt, out=A + 12)) and not shared(embed(tt, out=A + 16))                  # over the indices, behind them
+    # columns 64 bytes apart, rows neighbours (a transposed view): 10 x 4 bytes in each
+    assert shared(embed(tt, count=1, dim=2, rs=1, cs=16, out=2 * A + 36)) and not shared(embed(tt, count=1, dim=2, rs=1, cs=16, out=2 * A + 40))
+    assert shared(embed(tt, count=1, dim=2, rs=1, cs=16, out=2 * A + 100)) and not shared(embed(tt, count=1, dim=2, rs=1, cs=16, out=2 * A + 104))
+    assert shared(embed(tt, rs=0, cs=0, out=2 * A)) and not shared(embed(tt, rs=0, cs=0, out=2 * A + 4))
+    assert shared(embed(tt, vocab=1 << 28, rs=1 << 32, out=2 * A + (9 << 34)))                  # (a reach of 2^62 bytes)
+
+    def scatter(dy=A, index=2 * A, grad=3 * A, ws=4 * A):
+        return lib.ttamd_embedding_backward(0, capi.F32, capi.I32, 400, 10, 8, dy, index, 1.0, 0, grad, ws, A, None)
+
+    assert not shared(scatter())
+    for kw in (dict(grad=A), dict(grad=2 * A), dict(ws=A), dict(ws=2 * A), dict(ws=3 * A), dict(grad=A + 399 * 32)):
+        assert shared(scatter(**kw)), kw
+
+    def forward(out=2 * A, gate=3 * A, up=4 * A, ws=5 * A, bg=6 * A, bu=None):
+        return lib.ttamd_gated_linear_forward(0, capi.F32, 0, 3, 8, 8, view(capi), view(capi, 7 * A), view(capi, 8 * A, 1), bg, bu, out, gate, up, ws, A, None)
+
+    assert not shared(forward())
+    for kw in (dict(out=A), dict(out=7 * A), dict(out=8 * A + 4), dict(out=3 * A), dict(gate=4 * A), dict(up=A), dict(ws=A), dict(ws=2 * A), dict(out=6 * A),
+               dict(bu=2 * A)):
+        assert shared(forward(**kw)), kw
+
+    def backward(dx=2 * A, dwg=3 * A, dwu=4 * A, dbg=9 * A, dbu=10 * A, ws=5 * A):
+        return lib.ttamd_gated_linear_backward(0, capi.F32, 0, 3, 8, 8, 6 * A, view(capi), view(capi, 7 * A), view(capi, 8 * A), 11 * A, 12 * A, dx, dwg, dwu, dbg,
+                                               dbu, ws, A, None)
+
+    assert not shared(backward())
+    for kw in (dict(dx=A), dict(dx=6 * A), dict(dx=11 * A), dict(dx=12 * A), dict(dwg=7 * A), dict(dwu=8 * A), dict(dwg=4 * A), dict(dbg=10 * A), dict(dbu=A),
+               dict(ws=9 * A), dict(ws=A)):
+        assert shared(backward(**kw)), kw
+
+    def distill(z=A, stride=16, index=2 * A, logit=3 * A, weight=None, loss=4 * A, grad=5 * A, ws=6 * A):
+        return lib.ttamd_distill_loss(0, capi.F32, capi.I64, 3, 8, 2, z, stride, index, logit, weight, 1.0, loss, grad, ws, A, None)
+
+    assert not shared(distill()) and not shared(distill(loss=A + 32))                           # (between two rows of logits)
+    for kw in (dict(loss=A + 64), dict(grad=2 * A), dict(grad=3 * A), dict(loss=5 * A), dict(ws=A), dict(ws=5 * A), dict(weight=4 * A)):
+        assert shared(distill(**kw)), kw
 
 
 class _Memory:

@@ -7,6 +7,8 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
+#include <utility>
 
 #include "ttamd.h"
 
@@ -35,11 +37,17 @@ inline size_t dtype_size(ttamd_dtype dt) {
 }
 
 inline bool misaligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
-// Whether two byte ranges share a byte.
-inline bool overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return a_bytes > 0 && b_bytes > 0 && x < y + b_bytes && y < x + a_bytes;
-}
+// A matrix in memory, for check_disjoint: element (r, c) at data[r * s0 + c * s1].
+struct Extent {
+    const char *name;
+    const void *data;
+    int64_t rows, cols, s0, s1;
+    size_t item;
+};
+inline Extent dense_extent(const char *name, const void *data, int64_t n, size_t item) { return {name, data, 1, n, n, 1, item}; }
+// TTAMD_ERR_INVALID_ARGUMENT when a result (dense, rows of one) shares memory with an operand or with another result.  What is
+// NULL or empty shares nothing; rows of an operand whose elements lie apart count as whole.
+ttamd_status check_disjoint(const char *what, std::initializer_list<Extent> results, std::initializer_list<Extent> operands);
 
 #define TTAMD_HIP_CHECK(expr)                                                                  \
     do {                                                                                       \

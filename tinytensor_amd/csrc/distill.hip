@@ -743,10 +743,12 @@ ttamd_status ttamd_distill_loss(int device, ttamd_dtype dtype, ttamd_dtype index
         set_error("distill_loss: workspace of %zu bytes, %zu needed", workspace_bytes, need);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
-    if (rows > 0 && overlap(input, static_cast<size_t>((rows - 1) * input_row_stride + cols) * e, grad_input_out, static_cast<size_t>(rows * cols) * e)) {
-        set_error("distill_loss: the gradient may not be written over the logits");
-        return TTAMD_ERR_INVALID_ARGUMENT;
-    }
+    if (ttamd_status s = check_disjoint("distill_loss",
+                                        {dense_extent("the gradient", grad_input_out, rows * cols, e), dense_extent("the loss", loss_out, 1, e),
+                                         dense_extent("the workspace", workspace, static_cast<int64_t>(need), 1)},
+                                        {{"the logits", input, rows, cols, input_row_stride, 1, e}, dense_extent("teacher_index", teacher_index, rows * top, ie),
+                                         dense_extent("teacher_logit", teacher_logit, rows * top, e), dense_extent("row_weight", row_weight, rows, e)}))
+        return s;
     if (ttamd_status s = use_device(device)) return s;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == TTAMD_F32)

@@ -664,6 +664,9 @@ ttamd_status ttamd_embedding_forward(int device, ttamd_dtype dtype, ttamd_dtype 
         set_error("%s: pointers must be aligned to the element size", what);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
+    if (ttamd_status s = check_disjoint(what, {dense_extent("the result", out, count * dim, e)},
+                                        {{"the table", table, vocab, dim, row_stride, col_stride, e}, dense_extent("the indices", index, count, dtype_size(index_dtype))}))
+        return s;
     if (ttamd_status s = use_device(device)) return s;
     if (count == 0) return TTAMD_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -708,6 +711,9 @@ ttamd_status ttamd_embedding_backward(int device, ttamd_dtype dtype, ttamd_dtype
         set_error("%s: workspace of %zu bytes, %zu needed", what, workspace_bytes, need);
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
+    if (ttamd_status s = check_disjoint(what, {dense_extent("the gradient", grad_table, vocab * dim, e), dense_extent("the workspace", workspace, static_cast<int64_t>(need), 1)},
+                                        {dense_extent("grad_out", grad_out, count * dim, e), dense_extent("the indices", index, count, dtype_size(index_dtype))}))
+        return s;
     if (ttamd_status s = use_device(device)) return s;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const bool i64 = index_dtype == TTAMD_I64;

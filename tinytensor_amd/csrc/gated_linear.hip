@@ -617,6 +617,10 @@ ttamd_status backward(const Pass &p, const void *grad_out, const void *gate, con
     return TTAMD_OK;
 }
 
+Extent extent_of(const char *name, const ttamd_view2 &v, int64_t rows, int64_t cols, size_t item) {
+    return {name, v.data ? static_cast<const char *>(v.data) + v.offset * static_cast<int64_t>(item) : nullptr, rows, cols, v.stride[0], v.stride[1], item};
+}
+
 ttamd_status check_workspace(const char *what, const void *workspace, size_t given, size_t needed) {
     if (workspace && !misaligned(workspace, 16) && given >= needed) return TTAMD_OK;
     set_error("%s: workspace %p of %zu bytes: %zu are needed, aligned to 16", what, workspace, given, needed);
@@ -665,8 +669,18 @@ ttamd_status ttamd_gated_linear_forward(int device, ttamd_dtype dtype, int activ
             set_error("%s: pointers must be aligned to the element size", what);
             return TTAMD_ERR_INVALID_ARGUMENT;
         }
-    if (work)
-        if (ttamd_status s = check_workspace(what, workspace, workspace_bytes, sizes_of(dtype, rows, inner, hidden, false).bytes)) return s;
+    if (work) {
+        const size_t need = sizes_of(dtype, rows, inner, hidden, false).bytes;
+        if (ttamd_status s = check_workspace(what, workspace, workspace_bytes, need)) return s;
+        const int64_t n = rows * hidden;
+        if (ttamd_status s = check_disjoint(what,
+                                            {dense_extent("out", out, n, item), dense_extent("gate_out", gate_out, n, item), dense_extent("up_out", up_out, n, item),
+                                             dense_extent("the workspace", workspace, static_cast<int64_t>(need), 1)},
+                                            {extent_of("input", *input, rows, inner, item), extent_of("gate weight", *gate_weight, inner, hidden, item),
+                                             extent_of("up weight", *up_weight, inner, hidden, item), dense_extent("gate_bias", gate_bias, hidden, item),
+                                             dense_extent("up_bias", up_bias, hidden, item)}))
+            return s;
+    }
     if (ttamd_status s = use_device(device)) return s;
     if (!work) return TTAMD_OK;
     const Pass p{device, activation, dtype, rows, inner, hidden, *input, *gate_weight, *up_weight, static_cast<char *>(workspace), stream};
@@ -697,8 +711,20 @@ ttamd_status ttamd_gated_linear_backward(int device, ttamd_dtype dtype, int acti
             set_error("%s: pointers must be aligned to the element size", what);
             return TTAMD_ERR_INVALID_ARGUMENT;
         }
-    if (work)
-        if (ttamd_status s = check_workspace(what, workspace, workspace_bytes, sizes_of(dtype, rows, inner, hidden, true).bytes)) return s;
+    size_t need = 0;
+    if (work) {
+        need = sizes_of(dtype, rows, inner, hidden, true).bytes;
+        if (ttamd_status s = check_workspace(what, workspace, workspace_bytes, need)) return s;
+    }
+    const int64_t n = rows * hidden, w = inner * hidden;
+    if (ttamd_status s = check_disjoint(what,
+                                        {dense_extent("grad_input", grad_input, rows * inner, item), dense_extent("grad_gate_weight", grad_gate_weight, w, item),
+                                         dense_extent("grad_up_weight", grad_up_weight, w, item), dense_extent("grad_gate_bias", grad_gate_bias, hidden, item),
+                                         dense_extent("grad_up_bias", grad_up_bias, hidden, item), dense_extent("the workspace", workspace, static_cast<int64_t>(need), 1)},
+                                        {dense_extent("grad_out", grad_out, n, item), extent_of("input", *input, rows, inner, item),
+                                         extent_of("gate weight", *gate_weight, inner, hidden, item), extent_of("up weight", *up_weight, inner, hidden, item),
+                                         dense_extent("gate", gate, n, item), dense_extent("up", up, n, item)}))
+        return s;
     if (ttamd_status s = use_device(device)) return s;
     const Pass p{device, activation, dtype, rows, inner, hidden, *input, *gate_weight, *up_weight, static_cast<char *>(workspace), stream};
     return dtype == TTAMD_F32 ? backward<float>(p, grad_out, gate, up, grad_input, grad_gate_weight, grad_up_weight, grad_gate_bias, grad_up_bias)

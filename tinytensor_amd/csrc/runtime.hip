@@ -154,6 +154,40 @@ ttamd_status use_device(int device) {
     return TTAMD_OK;
 }
 
+// Whether bytes [p, p + n) meet one of the matrix's rows.
+static bool touches(const void *p, size_t n, Extent e) {
+    if (!p || n == 0 || !e.data || e.rows < 1 || e.cols < 1) return false;
+    if (e.rows == 1) e.s0 = 0;
+    if (e.cols == 1) e.s1 = 0;
+    if (e.s0 < e.s1) {
+        std::swap(e.s0, e.s1);
+        std::swap(e.rows, e.cols);
+    }
+    typedef __int128 wide;
+    const wide item = static_cast<wide>(e.item), pitch = e.s0 * item, len = ((e.cols - 1) * static_cast<wide>(e.s1) + 1) * item;
+    const wide first = static_cast<wide>(reinterpret_cast<uintptr_t>(p)) - static_cast<wide>(reinterpret_cast<uintptr_t>(e.data));
+    const wide last = first + static_cast<wide>(n);
+    if (last <= 0 || first >= (e.rows - 1) * pitch + len) return false;
+    if (e.rows == 1 || pitch <= len) return true;
+    const wide row = first < len ? 0 : (first - len) / pitch + 1;  // the first that ends behind the range's beginning
+    return row < e.rows && row * pitch < last;
+}
+
+ttamd_status check_disjoint(const char *what, std::initializer_list<Extent> results, std::initializer_list<Extent> operands) {
+    const auto refuse = [&](const Extent &r, const Extent &o) {
+        set_error("%s: %s shares memory with %s", what, r.name, o.name);
+        return TTAMD_ERR_INVALID_ARGUMENT;
+    };
+    for (const Extent *r = results.begin(); r != results.end(); ++r) {
+        const size_t n = static_cast<size_t>(r->rows * r->cols) * r->item;
+        for (const Extent &o : operands)
+            if (touches(r->data, n, o)) return refuse(*r, o);
+        for (const Extent *o = r + 1; o != results.end(); ++o)
+            if (touches(r->data, n, *o)) return refuse(*r, *o);
+    }
+    return TTAMD_OK;
+}
+
 static thread_local void *t_lent = nullptr;
 static thread_local size_t t_lent_bytes = 0;
 static thread_local bool t_loan = false;
