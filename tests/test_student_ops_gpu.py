@@ -463,6 +463,25 @@ def test_distill_loss(tt, dtype, rows, cols, top):
     check_distill(tt, z, ids, t, 1.0 if cols % 2 else 2.5, None, dtype, index=np.int32 if top % 2 else np.int64)
 
 
+@pytest.mark.parametrize("dtype", [np.float32, np.float64])
+@pytest.mark.parametrize("rows, cols, top", [(r, 40, 3) for r in (1, 3, 4, 5, 63, 64, 65)] + [(r, 700, 20) for r in (1, 2, 8, 9, 16, 17)] +
+                         [(1, 700, 40), (2, 700, 40), (1, 50003, 70), (1, 90001, 70)])
+def test_distill_loss_of_one_workgroup_or_more(tt, dtype, rows, cols, top):
+    """Row counts on both sides of what one workgroup takes (it adds the loss up itself), with rows that do not count."""
+    r = rng_of(rows, cols, top, "one")
+    z, ids, t = distill_data(r, rows, cols, top, dtype)
+    check_distill(tt, z, ids, t, 2.0, None, dtype)
+    if rows > 1:
+        ids[rows - 1] = -1                              # nothing in the last row, and no weight for the first
+        w = r.random(rows).astype(dtype)
+        w[0] = 0
+        check_distill(tt, z, ids, t, 1.0, w, dtype)
+    else:
+        check_distill(tt, z, ids, t, 1.0, np.zeros(1, dtype), dtype)
+        ids[0] = -1
+        check_distill(tt, z, ids, t, 1.0, None, dtype)
+
+
 @pytest.mark.parametrize("dtype, rows, cols", [(np.float32, 140, 60001), (np.float32, 130, 98309), (np.float32, 140, 131072), (np.float32, 129, 200003),
                                                (np.float64, 131, 65538), (np.float64, 129, 100001), (np.float32, 1600, 33000), (np.float32, 400, 131071),
                                                (np.float64, 700, 37001), (np.float32, 15000, 3501)])

@@ -46,7 +46,8 @@ struct DistillArgs {
     const T *teacher;     // [rows, top]
     const T *weight;      // [rows] or null: 1 / rows
     T *grad;              // [rows, cols]
-    double *row_loss;     // [rows] scratch, or a place for the four rows of a wave (narrow)
+    double *row_loss;     // [rows] scratch, or a place for the four rows of a wave
+    T *loss;              // a launch of one workgroup writes the loss itself; null: distill_sum_kernel does
     int64_t rows, row0;   // row0: first row of the launch
     int cols, top, index64;
     double temperature;
@@ -186,6 +187,13 @@ __device__ __forceinline__ T block_reduce(T v, T *lds) {
     return r;
 }
 
+// One lane leaves a row's loss (the whole loss where there is one row).
+template <typename T>
+__device__ __forceinline__ void leave_loss(const DistillArgs<T> &a, int64_t row, double loss) {
+    if (a.loss) a.loss[0] = static_cast<T>(loss);
+    else a.row_loss[row] = loss;
+}
+
 // A row that weighs nothing, or whose slots are all empty: no loss, a gradient of zeros.
 template <typename T, int BT>
 __device__ __forceinline__ void empty_row(const DistillArgs<T> &a, int64_t row) {
@@ -198,7 +206,7 @@ __device__ __forceinline__ void empty_row(const DistillArgs<T> &a, int64_t row) 
     for (int k = 0; k < W; ++k) zero[k] = T(0);
     for (int v = threadIdx.x; v < nvec; v += BT) reinterpret_cast<V *>(gr)[v] = zero;
     for (int i = nvec * W + threadIdx.x; i < a.cols; i += BT) gr[i] = T(0);
-    if (threadIdx.x == 0) a.row_loss[row] = 0.0;
+    if (threadIdx.x == 0) leave_loss(a, row, 0.0);
 }
 
 // A workgroup a row.  The row is requested once and stays: NV vectors of it in every lane's registers, `lds_vecs` more in
@@ -342,16 +350,17 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int l
     const double loss = slots_loss<T, BT>(a, slots, join_waves<T, NW, false>(red[3]), most, total);
     if (tid % 64 == 0) loss_of[wave] = loss;
     __syncthreads();  // the gradient's bulk comes first, the teacher's columns are written over it
-    if (tid == 0) a.row_loss[row] = static_cast<double>(w) * join_waves<double, NW, false>(loss_of);
+    if (tid == 0) leave_loss(a, row, static_cast<double>(w) * join_waves<double, NW, false>(loss_of));
     write_slots<T, BT>(a, slots, gr, most, f, wt, 0, a.cols, a.cols);
 }
 
 // Short rows: G lanes own a row, E columns each (lane l: columns l, l + G, ..), up to 64 slots.  Everything stays in
 // registers; the slots go round the group one by one and the lane that holds a slot's column takes its share off.
-template <typename T, int G, int E>
-__global__ void __launch_bounds__(256) distill_short_kernel(DistillArgs<T> a) {
+template <typename T, int G, int E, int BT>
+__global__ void __launch_bounds__(BT) distill_short_kernel(DistillArgs<T> a) {
+    __shared__ double of_wave[BT / 64];
     constexpr int S = 64 / G;  // slots a lane
-    const int64_t row_of = a.row0 + (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / G;
+    const int64_t row_of = a.row0 + (static_cast<int64_t>(blockIdx.x) * BT + threadIdx.x) / G;
     const bool live = row_of < a.rows;
     const int64_t row = live ? row_of : a.rows - 1;  // (every lane takes part in the shuffles)
     const int lane = threadIdx.x % G;
@@ -445,12 +454,21 @@ __global__ void __launch_bounds__(256) distill_short_kernel(DistillArgs<T> a) {
     double own = live && on ? static_cast<double>(w) * a.temperature * a.temperature * loss : 0.0;
 #pragma unroll
     for (int d = G; d < 64; d *= 2) own += __shfl_xor(own, d, 64);
-    if (!live) return;
-    if (threadIdx.x % 64 == 0) a.row_loss[row / (64 / G)] = own;
+    if (live) {
+        if (threadIdx.x % 64 == 0 && !a.loss) a.row_loss[row / (64 / G)] = own;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const int c = lane + i * G;
-        if (c < a.cols) a.grad[row * a.cols + c] = on ? e[i] * f - wt * share[i] : T(0);
+        for (int i = 0; i < E; ++i) {
+            const int c = lane + i * G;
+            if (c < a.cols) a.grad[row * a.cols + c] = on ? e[i] * f - wt * share[i] : T(0);
+        }
+    }
+    if (!a.loss) return;  // (one workgroup: its waves' sums in order)
+    if (threadIdx.x % 64 == 0) of_wave[threadIdx.x / 64] = own;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double sum = 0;
+        for (int w = 0; w < static_cast<int>(blockDim.x / 64); ++w) sum += of_wave[w];
+        a.loss[0] = static_cast<T>(sum);
     }
 }
 
@@ -593,16 +611,32 @@ int64_t parts_of(size_t item, int64_t rows, int64_t cols) {
     return rows <= 128 && row_bytes > 320 * 1024 ? (cols + per - 1) / per : 0;
 }
 
-// Rows of a few columns: 16 lanes each, four to a wave.
-bool narrow(int64_t cols, int64_t top) { return cols <= 64 && top <= 64; }
+// Rows of a few columns: 16 lanes each, four to a wave.  Rows of up to 1024 columns: a wave each (the slots go one by one:
+// 4096 x 1000 f32 17 us with 16 of them, with 64 29 against 24).  0: others.
+int short_lanes(int64_t cols, int64_t top) { return cols <= 64 && top <= 64 ? 16 : cols <= 1024 && top <= 32 ? 64 : 0; }
+
+// Whether one workgroup has all rows: it adds up the loss too, which spares the second launch (64 x 60, 16 x 1000 and 1 x 30000
+// f32 13.5 us a call against 15.7, host side included).  In f64 a CU's exponentials take longer: 8 x 1000 15.3 against 15.7,
+// but 16 x 1000 24.9 against 15.8.
+bool one_workgroup(size_t item, int64_t rows, int64_t cols, int64_t top) {
+    const int lanes = short_lanes(cols, top);
+    return lanes ? rows * lanes <= (lanes == 64 && item == 8 ? 512 : 1024) : rows == 1 && parts_of(item, rows, cols) == 0;
+}
+
+template <typename T, int G, int E>
+void launch_short(const DistillArgs<T> &a, int64_t rows, hipStream_t st) {
+    if (a.loss) distill_short_kernel<T, G, E, 1024><<<1, static_cast<unsigned>((rows * G + 63) / 64 * 64), 0, st>>>(a);
+    else distill_short_kernel<T, G, E, 256><<<static_cast<unsigned>((rows + 256 / G - 1) / (256 / G)), 256, 0, st>>>(a);
+}
 
 template <typename T>
 ttamd_status launch_some_rows(const DistillArgs<T> &a, int64_t rows, void *parts, hipStream_t st) {
     const size_t slots = Slots<T>::bytes(a.top);
-    if (narrow(a.cols, a.top)) {
-        distill_short_kernel<T, 16, 4><<<static_cast<unsigned>((rows + 15) / 16), 256, 0, st>>>(a);
-    } else if (a.cols <= 1024 && a.top <= 32) {  // (the slots go one by one: 4096 x 1000 f32 17 us with 16 of them, with 64 29 against 24)
-        distill_short_kernel<T, 64, 16><<<static_cast<unsigned>((rows + 3) / 4), 256, 0, st>>>(a);
+    const int lanes = short_lanes(a.cols, a.top);
+    if (lanes == 16) {
+        launch_short<T, 16, 4>(a, rows, st);
+    } else if (lanes == 64) {
+        launch_short<T, 64, 16>(a, rows, st);
     } else if (const int64_t n = parts_of(sizeof(T), a.rows, a.cols)) {
         const dim3 grid(static_cast<unsigned>(n), static_cast<unsigned>(a.rows));
         distill_part_kernel<T><<<grid, kPartThreads, 0, st>>>(a, static_cast<PartSums<T> *>(parts));
@@ -656,8 +690,10 @@ template <typename T>
 ttamd_status launch_distill(int64_t rows, int64_t cols, int64_t top, const void *input, int64_t input_row_stride, const void *index,
                             bool index64, const void *teacher, const void *weight, double temperature, void *loss_out, void *grad_out,
                             void *workspace, hipStream_t st) {
+    const bool one = rows > 0 && one_workgroup(sizeof(T), rows, cols, top);
     if (rows > 0) {
         DistillArgs<T> a{};
+        a.loss = one ? static_cast<T *>(loss_out) : nullptr;
         a.z = static_cast<const T *>(input);
         a.z_row = input_row_stride;
         a.index = index;
@@ -674,7 +710,8 @@ ttamd_status launch_distill(int64_t rows, int64_t cols, int64_t top, const void 
         a.uniform_weight = static_cast<T>(1.0 / static_cast<double>(rows));
         if (ttamd_status s = launch_rows(a, static_cast<char *>(workspace) + part_offset(rows), st)) return s;
     }
-    const int64_t sums = narrow(cols, top) ? (rows + 3) / 4 : rows;
+    if (one) return TTAMD_OK;
+    const int64_t sums = short_lanes(cols, top) == 16 ? (rows + 3) / 4 : rows;
     distill_sum_kernel<T><<<1, 1024, 0, st>>>(static_cast<const double *>(workspace), sums, static_cast<T *>(loss_out));
     TTAMD_HIP_CHECK(hipGetLastError());
     return TTAMD_OK;
