@@ -363,7 +363,7 @@ ttamd_status ttamd_embedding_backward(int device, ttamd_dtype dtype, ttamd_dtype
 /* The gated pair of Linear layers of a feed-forward block: g = x . Wg + bg, u = x . Wu + bu, out = act(g) * u.
  * input [rows, inner], gate_weight and up_weight [inner, hidden]: any non-negative strides, read in place.  gate_bias,
  * up_bias: dense [hidden], each may be NULL.  out [rows, hidden].  gate_out / up_out: both or neither; they receive g and
- * u, what the backward pass reads.  gelu is the exact (erf) form.  rows <= 2^28, inner and hidden <= 2^26, strides <= 2^32. */
+ * u, what the backward pass reads.  gelu is the exact (erf) form.  rows, inner and hidden <= 2^26, strides <= 2^32. */
 typedef enum ttamd_activation { TTAMD_ACT_SILU = 0, TTAMD_ACT_GELU = 1, TTAMD_ACT_RELU = 2, TTAMD_ACT_SIGMOID = 3 } ttamd_activation;
 ttamd_status ttamd_gated_linear_workspace(ttamd_dtype dtype, int64_t rows, int64_t inner, int64_t hidden, int backward,
                                           size_t *bytes);

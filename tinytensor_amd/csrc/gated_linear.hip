@@ -50,16 +50,18 @@ __global__ void __launch_bounds__(256) gated_product_kernel(const T *gate, const
 // What a pass needs before its products, in one launch: the gradients of the two products' results, and copies of operands
 // whose rows are no whole aligned vectors.
 //   dg = dh * u * act'(g), du = dh * act(g): dense dh, g, u [rows, hidden] in, rows of d_row elements out (a multiple of the
-//   vector; zeros behind the columns).  A workgroup has 64 vectors of columns and kSlopeRows rows, a wave every fourth of
+//   vector; zeros behind the columns).  A workgroup has 64 vectors of columns and slope_rows rows, a wave every fourth of
 //   them; with `sums` it also leaves its rows' column sums, the bias gradients' parts: sums[row block][2][d_row].
+//   slope_rows: kSlopeRows with sums (their parts are read again), else kFewSlopeRows: more waves with fewer loads one after
+//   the other (1024 x 784 x 1024 f32 forward and backward 107 -> 103 us; 4 or 16 rows 104).
 //   A copy: element (r, c) of any view to dst[r * dst_row + c], zeros from (rows, cols) to (dst_rows, dst_row).
-constexpr int kSlopeRows = 32, kCopies = 3;
+constexpr int kSlopeRows = 32, kFewSlopeRows = 8, kCopies = 3;
 template <typename T>
 struct CopyJob {
     const T *src;
     int64_t s0, s1, rows, cols, dst_rows, dst_row;
     T *dst;
-    int blocks;  // 64 x 64 tiles of dst; 0: nothing to copy
+    int blocks;  // tiles of dst, copy_rows() x 64; 0: nothing to copy
 };
 template <typename T>
 struct PrepareArgs {
@@ -67,9 +69,13 @@ struct PrepareArgs {
     T *dg, *du, *sums;
     int64_t rows, d_row;
     int hidden;
-    int slope_blocks, slope_blocks_n;  // workgroups of the gradients; of them side by side
+    int slope_rows, slope_blocks, slope_blocks_n;  // rows a workgroup; workgroups of the gradients; of them side by side
     CopyJob<T> copy[kCopies];
 };
+
+// Rows of a tile: rows in order go by vectors, one to three a lane; others are turned in LDS.
+template <typename T>
+__host__ __device__ constexpr int copy_rows(const CopyJob<T> &j) { return j.s1 == 1 ? 16 : 64; }
 
 template <typename T>
 __device__ __forceinline__ void copy_tile(const CopyJob<T> &j, int block, T (*tile)[65]) {
@@ -77,10 +83,10 @@ __device__ __forceinline__ void copy_tile(const CopyJob<T> &j, int block, T (*ti
     typedef T near_t __attribute__((ext_vector_type(VecOf<T>::W), aligned(sizeof(T))));
     constexpr int W = VecOf<T>::W, kVecs = 64 / W;
     const int tiles_n = static_cast<int>((j.dst_row + 63) / 64);
-    const int64_t r0 = static_cast<int64_t>(block / tiles_n) * 64, c0 = static_cast<int64_t>(block % tiles_n) * 64;
+    const int64_t r0 = static_cast<int64_t>(block / tiles_n) * copy_rows(j), c0 = static_cast<int64_t>(block % tiles_n) * 64;
     if (j.s1 == 1) {  // rows in order: vectors, wherever the source's begin (dst_row is whole vectors)
 #pragma unroll
-        for (int i = threadIdx.x; i < 64 * kVecs; i += 256) {
+        for (int i = threadIdx.x; i < 16 * kVecs; i += 256) {
             const int64_t r = r0 + i / kVecs, c = c0 + i % kVecs * W;
             if (r >= j.dst_rows || c >= j.dst_row) continue;
             const T *src = j.src + r * j.s0 + c;
@@ -133,14 +139,14 @@ __global__ void __launch_bounds__(256) gated_prepare_kernel(PrepareArgs<T> a) {
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int row_block = block / a.slope_blocks_n, col_block = block - row_block * a.slope_blocks_n;
     const int64_t c = (static_cast<int64_t>(col_block) * 64 + lane) * W;
-    const int64_t r0 = static_cast<int64_t>(row_block) * kSlopeRows;
+    const int64_t r0 = static_cast<int64_t>(row_block) * a.slope_rows;
     T sg[W], su[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) sg[k] = su[k] = T(0);
     if (c < a.d_row) {
         const bool whole = c + W <= a.hidden;
 #pragma unroll 2
-        for (int i = wave; i < kSlopeRows; i += 4) {
+        for (int i = wave; i < a.slope_rows; i += 4) {
             if (r0 + i >= a.rows) break;
             const int64_t at = (r0 + i) * a.hidden + c;
             T d[W], g[W], u[W];
@@ -396,10 +402,10 @@ ttamd_status check_gated(const char *what, ttamd_dtype dtype, int64_t rows, int6
         return TTAMD_ERR_UNSUPPORTED_DTYPE;
     }
     // (a launch holds fewer than 2^32 lanes, and every size in bytes fits 64 bits)
-    constexpr int64_t most_rows = int64_t(1) << 28, most_cols = int64_t(1) << 26, most = int64_t(1) << 40;
-    if (rows < 0 || inner < 1 || hidden < 1 || rows > most_rows || inner > most_cols || hidden > most_cols || rows * inner > most ||
+    constexpr int64_t most_lines = int64_t(1) << 26, most = int64_t(1) << 40;
+    if (rows < 0 || inner < 1 || hidden < 1 || rows > most_lines || inner > most_lines || hidden > most_lines || rows * inner > most ||
         rows * hidden > most || inner * hidden > most) {
-        set_error("%s: rows %lld, inner %lld, hidden %lld: rows from 0 to 2^28, the others from 1 to 2^26, 2^40 elements a matrix", what,
+        set_error("%s: rows %lld, inner %lld, hidden %lld: rows from 0, the others from 1, up to 2^26 each and 2^40 elements a matrix", what,
                   static_cast<long long>(rows), static_cast<long long>(inner), static_cast<long long>(hidden));
         return TTAMD_ERR_INVALID_ARGUMENT;
     }
@@ -444,8 +450,8 @@ bool row_vectors(const Operand<T> &m, int64_t cols) {
 }
 template <typename T>
 CopyJob<T> copy_job(Operand<T> &m, int64_t rows, int64_t cols, int64_t dst_rows, int64_t dst_row, void *dst) {
-    const int64_t blocks = (dst_rows + 63) / 64 * ((dst_row + 63) / 64);
-    const CopyJob<T> j{m.data, m.s0, m.s1, rows, cols, dst_rows, dst_row, static_cast<T *>(dst), static_cast<int>(blocks)};
+    CopyJob<T> j{m.data, m.s0, m.s1, rows, cols, dst_rows, dst_row, static_cast<T *>(dst), 0};
+    j.blocks = static_cast<int>((dst_rows + copy_rows(j) - 1) / copy_rows(j) * ((dst_row + 63) / 64));
     m = {static_cast<const T *>(dst), dst_row, 1};
     return j;
 }
@@ -564,7 +570,8 @@ ttamd_status backward(const Pass &p, const void *grad_out, const void *gate, con
         prep.d_row = z.hidden_row;
         prep.hidden = static_cast<int>(hidden);
         prep.slope_blocks_n = static_cast<int>((z.hidden_row / z.vec + 63) / 64);
-        prep.slope_blocks = static_cast<int>((rows + kSlopeRows - 1) / kSlopeRows) * prep.slope_blocks_n;
+        prep.slope_rows = kFewSlopeRows;
+        prep.slope_blocks = static_cast<int>((rows + kFewSlopeRows - 1) / kFewSlopeRows) * prep.slope_blocks_n;
     }
     // One grid of all three products (gated_tiles.hip) unless rows or weights are beyond its reach.
     const int64_t piece = z.split.w_splits ? z.split.w_chunk : rows;  // rows under a tile of a weight's gradient
@@ -583,7 +590,11 @@ ttamd_status backward(const Pass &p, const void *grad_out, const void *gate, con
         return launch_gated_backward_tiles<T>(a, p.device, st);
     }
     T *const sums = reinterpret_cast<T *>(p.ws + z.sums);
-    if (dbg || dbu) prep.sums = sums;
+    if (dbg || dbu) {
+        prep.sums = sums;
+        prep.slope_rows = kSlopeRows;
+        prep.slope_blocks = static_cast<int>((rows + kSlopeRows - 1) / kSlopeRows) * prep.slope_blocks_n;
+    }
     if (ttamd_status s = launch_prepare(p.act, prep, st)) return s;
     if (dbg || dbu) {
         gated_bias_kernel<T><<<dim3(static_cast<unsigned>((hidden + 63) / 64), 2), 256, 0, st>>>(
