@@ -302,6 +302,25 @@ def test_gated_linear_views(tt, dtype, rows, form):
     check_gated(tt, dtype, "silu", x, wg, wu, bg, None, tx, twg, twu, dh=dh)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, inner, hidden", [(n, *s) for s in ((1, 2), (7, 3), (16, 31), (17, 33), (250, 64), (1003, 130))
+                                                 for n in (3, 5, 8, 15, 16, 17, 31, 33, 64, 100, 250)] + [(5, 300, 8200), (17, 300, 8200), (33, 300, 8200)])
+def test_gated_linear_blocks_of_rows(tt, dtype, rows, inner, hidden):
+    """Row counts, reductions and widths around the blocks of 16 and 32 rows, 8 or 16 k and 32 columns; operands are cut out of
+    buffers of NaN, which nothing may reach."""
+    T = tt.Tensor
+    r = rng_of(rows, inner, hidden, "rows")
+    x, wg, wu, bg, bu, _ = gated_data(r, dtype, rows, inner, hidden)
+
+    def inside(a):
+        b = np.full((a.shape[0] + 2, a.shape[1] + 3), np.nan, dtype)
+        b[1:-1, 1:-2] = a
+        t = T.from_numpy(b)
+        return T(t.storage, t.dtype, a.shape, (b.shape[1], 1), b.shape[1] + 1)
+
+    check_gated(tt, dtype, "gelu" if rows % 2 else "silu", x, wg, wu, bg if rows % 3 else None, bu, inside(x), inside(wg), inside(wu))
+
+
 def test_gated_linear_beyond_32_bit_offsets(tt):
     """Matrices of more than 2^31 bytes, and rows that lie that far apart: whole numbers, so every sum is exact."""
     r = rng_of(31)

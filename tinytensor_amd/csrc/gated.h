@@ -81,6 +81,10 @@ struct GatedBackward {
     GatedSplit split;
     T *x_part, *w_part, *b_part;        // [2 x_splits][rows, inner], [w_splits][2][inner, hidden], [w_splits][2][hidden]
 };
+// A block of rows: k and w_cols are the true sizes, rows begin anywhere, hidden >= 2.  The estimate is its time in us.
+double few_rows_estimate(size_t item, int64_t rows, int64_t inner, int64_t hidden);
+template <typename T>
+ttamd_status launch_gated_few_rows(const GatedForward<T> &a, int device, hipStream_t st);
 template <typename T>
 ttamd_status launch_gated_forward_tiles(const GatedForward<T> &a, int device, hipStream_t st);
 template <typename T>

@@ -483,18 +483,16 @@ struct Pass {
     void *stream;
 };
 
-// Up to 8 rows in one launch.  Against the separate products (three launches; f32, inputs in turn): 1 x 1024 x 4096 12.2 us
-// (a pass takes the host that long) against 18.0, 1 x 2048 x 8192 27.2 (4.9 TB/s) against 53, 8 x 2048 x 8192 41 against 52;
-// f64 1 x 1024 x 4096 15.5 against 18.1, but 4 x 2048 x 8192 64 against 55, so f64 takes 3 and 4 rows of small weights only.
+// Up to 4 rows (f32; 2 f64) in one launch: 1 x 2048 x 2048 f32 13.2 us against 18.3 on the matrix cores
+// (gated_few_kernel), 4 x 4000 x 512 27 against 33, f64 2 x 2048 x 2048 16.6 against 22.2; f32 of more columns only 1 row (1 x 2048 x 8192
+// 22.6 against 21.6, 4.9 TB/s; 4 x 2048 x 8192 28.9 against 22).
 template <typename T>
 ttamd_status launch_rows(int act, const RowArgs<T> &a, int64_t rows, hipStream_t st) {
     constexpr int kCols = kRowLanes * VecOf<T>::W;
     const unsigned blocks = static_cast<unsigned>((a.hidden + kCols - 1) / kCols);
     for_activation(act, [&]<int ACT>() {
-        if (rows > 4) {
-            if constexpr (sizeof(T) == 4) gated_rows_kernel<T, 8, ACT><<<blocks, kRowThreads, 0, st>>>(a);
-        } else if (rows > 2) {
-            gated_rows_kernel<T, 4, ACT><<<blocks, kRowThreads, 0, st>>>(a);
+        if (rows > 2) {
+            if constexpr (sizeof(T) == 4) gated_rows_kernel<T, 4, ACT><<<blocks, kRowThreads, 0, st>>>(a);
         } else if (rows > 1) {
             gated_rows_kernel<T, 2, ACT><<<blocks, kRowThreads, 0, st>>>(a);
         } else {
@@ -511,7 +509,9 @@ ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, 
     const int64_t rows = p.rows, inner = p.inner, hidden = p.hidden;
     const GatedSizes z = sizes_of(p.dtype, rows, inner, hidden, false);
     Operand<T> x = operand_of<T>(p.x), wg = operand_of<T>(p.wg), wu = operand_of<T>(p.wu);
-    const int64_t handful = z.item == 4 ? 8 : inner * hidden <= (1 << 20) ? 4 : 2;
+    const bool f32 = z.item == 4;
+    const bool in_order = x.s1 == 1 && wg.s1 == 1 && wu.s1 == 1;
+    const int64_t handful = f32 ? (hidden <= 4096 ? 4 : 1) : 2;
     if (rows <= handful && wg.s1 == 1 && wu.s1 == 1 && hidden >= z.vec) {
         const RowArgs<T> a{x.data, wg.data, wu.data, static_cast<const T *>(gate_bias), static_cast<const T *>(up_bias), x.s0, x.s1, wg.s0, wu.s0,
                            static_cast<T *>(out), static_cast<T *>(gate), static_cast<T *>(up), static_cast<int>(rows), static_cast<int>(inner), static_cast<int>(hidden)};
@@ -522,11 +522,24 @@ ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, 
     // products cut (f32, 64 x 128 tiles: 128 x 1024 x 2048, 64 tiles, 38 us against 28 in three launches; 256 x 1024 x 4096,
     // 256 tiles, 38 against 49; f64, 64 x 64 tiles: 200 x 2001 x 1003, 128 tiles, 98 against 77; 256 x 1024 x 4096, 512
     // tiles, 65 against 79), or the weights are beyond its reach.
-    const bool f32 = z.item == 4;
     const int64_t tiles = (rows + 63) / 64 * ((hidden + (f32 ? 63 : 31)) / (f32 ? 64 : 32));
-    const bool few = inner > 256 && (rows <= 32 || tiles < (f32 ? 96 : 144));
-    if (!few && within_reach(z.item, z.inner_row, z.hidden_row) && within_reach(z.item, kTileLines, z.inner_row) &&
-        within_reach(z.item, kTileLines, z.hidden_row)) {
+    const bool cut = inner > 256 && (rows <= 32 || tiles < (f32 ? 96 : 144));
+    const bool tiled = !cut && within_reach(z.item, z.inner_row, z.hidden_row) && within_reach(z.item, kTileLines, z.inner_row) &&
+                       within_reach(z.item, kTileLines, z.hidden_row);
+    if (rows <= 256 && in_order && hidden >= 2) {
+        // What the others take, in us: a round of tiles (0.034 a k) and a copy launch where an operand needs one, or two
+        // products and the launch behind them.
+        const bool copies = !row_vectors(x, inner) || !row_vectors(wg, hidden) || !row_vectors(wu, hidden);
+        const double others = tiled ? static_cast<double>((tiles + 255) / 256 * inner) * 0.034 + (copies ? 11 : 3)
+                                    : 17 + 0.0035 * static_cast<double>(inner) + 4e-6 * static_cast<double>(rows * inner) * static_cast<double>(hidden) / (f32 ? 153 : 73);
+        if (few_rows_estimate(z.item, rows, inner, hidden) < others) {
+            const GatedForward<T> a{x.data, wg.data, wu.data, x.s0, wg.s0, wu.s0, static_cast<int>(rows), static_cast<int>(inner), static_cast<int>(hidden),
+                                    static_cast<int>(hidden), p.act, static_cast<const T *>(gate_bias), static_cast<const T *>(up_bias),
+                                    static_cast<T *>(out), static_cast<T *>(gate), static_cast<T *>(up)};
+            return launch_gated_few_rows<T>(a, p.device, st);
+        }
+    }
+    if (tiled) {
         const bool own = inner % z.vec == 0;  // (x's padding meets rows of zeros in the weights' copies)
         const auto far = [&](const Operand<T> &w) { return !own || !row_vectors(w, hidden) || !within_reach(z.item, inner, w.s0); };
         if (!row_vectors(x, inner) || !within_reach(z.item, kTileLines, x.s0)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);

@@ -1,13 +1,14 @@
 // gated_tiles.hip — the gated pair of Linear layers on the matrix cores: both products of the forward pass with their
-// activation as one grid, and the three products of the backward pass as one grid (gfx950).
+// activation as one grid, and the three products of the backward pass as one grid; the forward pass of a few rows (gfx950).
 //
-// Built from the tile engine of mfma_core.h.  Operands here are row-major with 16-byte aligned rows of whole 16-byte
+// The grids are built from the tile engine of mfma_core.h.  Operands here are row-major with 16-byte aligned rows of whole 16-byte
 // vectors; gated_linear.hip sees to that (it copies what is not) and picks between these kernels and separate products.
 #include "gated.h"
 #include "mfma_core.h"
 
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 namespace ttamd {
 namespace {
@@ -329,6 +330,157 @@ __global__ void __launch_bounds__(256) gated_add_parts_kernel(PartSums<T> a) {
     }
 }
 
+// A block of rows (a batch of requests in step, a short prompt): too few for tiles of 64 rows, more than the vector units
+// want.  A workgroup owns 32 columns of both weights and 16 or 32 rows, and its NW waves share out the reduction in groups of
+// 64 / MB x VK k, every NW-th to a wave: a lane loads 16 bytes of a row of x and the rows of the weights that meet them,
+// straight into the registers that the matrix instructions read (lane group h of a group takes k = VK h .. VK h + VK - 1, of
+// x and weights alike, so the order inside a group does not matter).  Weights are read once, there is no barrier until the end;
+// the waves' sums are added up through LDS in wave order, and the same lanes apply biases and activation: one launch.
+// Columns behind the last are moved back onto it (they come out twice, the same); rows behind the last repeat it and are dropped.
+// Bound: HBM with 16 rows (16 x 2048 x 8192 f32 22.6 us, 5.9 TB/s with what the caches keep; separate products 48; 8 x 2048 x
+// 8192 22 against 36 on the vector units), the matrix cores next to it with 32 (32 x 2048 x 8192 32 us against 75;
+// 64 x 2048 x 2048 20 against 47; f64 33 x 2048 x 2048 23 against 52).
+// Blocks of 16 x 16 f32: half the matrix instructions' time of 32 x 32 for up to 16 rows.
+struct Mfma16 {
+    static constexpr int MB = 16, VK = 4, NACC = 4;
+    using acc_t = float __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ acc_t mma(float a, float b, acc_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ int acc_row(int e, int lane) { return 4 * (lane / 16) + e; }
+};
+template <typename T, class MI, int RB>
+struct FewShape {
+    static constexpr int CB = 32 / MI::MB;                  // blocks of columns: neighbouring columns of a lane
+    static constexpr int E = RB * CB * MI::NACC;            // elements a lane and matrix
+    static constexpr int NW = E * sizeof(T) > 64 ? 8 : 16;  // 128 KB of parts
+    static constexpr size_t kLds = static_cast<size_t>(NW) * 2 * E * 64 * sizeof(T);
+    static constexpr int kRows = RB * MI::MB;
+};
+
+template <typename T, class MI, int RB, int ACT>
+__global__ void __launch_bounds__((FewShape<T, MI, RB>::NW * 64)) gated_few_kernel(GatedForward<T> a) {
+    using S = FewShape<T, MI, RB>;
+    constexpr int MB = MI::MB, VK = MI::VK, CB = S::CB, E = S::E, NW = S::NW, kGroup = 64 / MB * VK;
+    typedef T xvec_t __attribute__((ext_vector_type(VK), aligned(sizeof(T))));
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem_raw[];
+    T *const part = reinterpret_cast<T *>(smem_raw);  // [NW][2][E][64]
+    const int tid = threadIdx.x, lane = tid % 64, l = lane % MB, h = lane / MB;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int c0 = blockIdx.x * 32, m0 = blockIdx.y * S::kRows;
+    const auto col_of = [&](int place, int cb) {  // the column that a lane's place holds
+        const int at = c0 + place * CB;
+        return (at + CB <= a.hidden ? at : a.hidden - CB) + cb;
+    };
+    const T *xr[RB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+        const int m = m0 + r * MB + l;
+        xr[r] = a.x + (m < a.rows ? m : a.rows - 1) * a.x_row + h * VK;
+    }
+    const T *wg = a.wg + h * VK * a.wg_row + col_of(l, 0), *wu = a.wu + h * VK * a.wu_row + col_of(l, 0);
+    typename MI::acc_t acc[2][RB][CB];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+#pragma unroll
+                for (int e = 0; e < MI::NACC; ++e) acc[m][r][c][e] = T(0);
+    typedef T wvec_t __attribute__((ext_vector_type(CB), aligned(sizeof(T))));
+    xvec_t x[RB];
+    wvec_t w[2][VK];
+    const auto load = [&](int64_t k) {
+#pragma unroll
+        for (int r = 0; r < RB; ++r) x[r] = *reinterpret_cast<const xvec_t *>(xr[r] + k);
+#pragma unroll
+        for (int j = 0; j < VK; ++j) {
+            w[0][j] = *reinterpret_cast<const wvec_t *>(wg + (k + j) * a.wg_row);
+            w[1][j] = *reinterpret_cast<const wvec_t *>(wu + (k + j) * a.wu_row);
+        }
+    };
+    const auto multiply = [&] {
+#pragma unroll
+        for (int j = 0; j < VK; ++j)
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int c = 0; c < CB; ++c) acc[m][r][c] = MI::mma(x[r][j], w[m][j][c], acc[m][r][c]);
+    };
+    // A wave's next group is requested once the last one has been multiplied; the other waves' loads fill the time.  (Two to
+    // four groups in flight a wave: 32 x 2048 x 8192 f32 42 us instead of 29.)
+    const int groups = a.k / kGroup;
+    if (wave < groups) {
+        load(static_cast<int64_t>(wave) * kGroup);
+        int g = wave;
+        for (; g + NW < groups; g += NW) {
+            multiply();
+            __builtin_amdgcn_sched_barrier(0);
+            load(static_cast<int64_t>(g + NW) * kGroup);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        multiply();
+    }
+    if (groups * kGroup < a.k && wave == groups % NW) {  // the last k, one by one; zeros on both sides behind them
+        const int k = groups * kGroup;
+#pragma unroll
+        for (int j = 0; j < VK; ++j) {
+            const bool in = k + h * VK + j < a.k;
+#pragma unroll
+            for (int r = 0; r < RB; ++r) x[r][j] = in ? xr[r][k + j] : T(0);
+            const wvec_t zero = {};
+            w[0][j] = in ? *reinterpret_cast<const wvec_t *>(wg + (k + j) * a.wg_row) : zero;
+            w[1][j] = in ? *reinterpret_cast<const wvec_t *>(wu + (k + j) * a.wu_row) : zero;
+        }
+        multiply();
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+#pragma unroll
+                for (int e = 0; e < MI::NACC; ++e) part[((wave * 2 + m) * E + (r * CB + c) * MI::NACC + e) * 64 + lane] = acc[m][r][c][e];
+    __syncthreads();
+#pragma unroll
+    for (int e = wave; e < E; e += NW) {
+        const int r = e / (CB * MI::NACC), c = e / MI::NACC % CB;
+        const int row = m0 + r * MB + MI::acc_row(e % MI::NACC, lane), col = col_of(l, c);
+        T g = T(0), u = T(0);
+#pragma unroll
+        for (int v = 0; v < NW; ++v) {
+            g += part[((v * 2 + 0) * E + e) * 64 + lane];
+            u += part[((v * 2 + 1) * E + e) * 64 + lane];
+        }
+        if (a.gate_bias) g += a.gate_bias[col];
+        if (a.up_bias) u += a.up_bias[col];
+        if (row >= a.rows) continue;
+        const int64_t to = static_cast<int64_t>(row) * a.hidden + col;
+        if (a.gate) {
+            a.gate[to] = g;
+            a.up[to] = u;
+        }
+        a.out[to] = activate<T, ACT>(g) * u;
+    }
+}
+
+template <typename T, class MI, int RB, int ACT>
+ttamd_status run_few(const GatedForward<T> &a, int device, hipStream_t st) {
+    using S = FewShape<T, MI, RB>;
+    static_assert(S::kLds <= 160 * 1024, "LDS of a CU");
+    auto kernel = gated_few_kernel<T, MI, RB, ACT>;
+    static std::atomic<bool> configured[kMaxDevices] = {};
+    if (!configured[device].load(std::memory_order_acquire)) {
+        TTAMD_HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kLds)));
+        configured[device].store(true, std::memory_order_release);
+    }
+    kernel<<<dim3(static_cast<unsigned>((a.hidden + 31) / 32), static_cast<unsigned>((a.rows + S::kRows - 1) / S::kRows)), S::NW * 64, S::kLds, st>>>(a);
+    TTAMD_HIP_CHECK(hipGetLastError());
+    return TTAMD_OK;
+}
+
 template <typename T, int BM, int BN, int BK, int WGM, int WGN, int PF, int HALVES>
 ttamd_status run_forward(const GatedForward<T> &a, int device, hipStream_t st) {
     using StA = Stager<T, BM, BK, true, Mfma<T>::VK, PF>;
@@ -360,6 +512,32 @@ bool halves_match(int k, int bk) {
 }
 
 }  // namespace
+
+// 16 rows a workgroup while each finds a CU of its own, else 32 (32 x 4000 x 512 f32 28 us against 50; 32 x 2048 x 8192 46
+// against 29).
+static int few_rows_blocks(int64_t rows, int64_t hidden) { return rows <= 16 || (rows + 15) / 16 * ((hidden + 31) / 32) <= 256 ? 1 : 2; }
+
+double few_rows_estimate(size_t item, int64_t rows, int64_t inner, int64_t hidden) {
+    const int blocks = few_rows_blocks(rows, hidden);
+    const int64_t rounds = ((rows + 16 * blocks - 1) / (16 * blocks) * ((hidden + 31) / 32) + 255) / 256;
+    const double a_k = item == 4 ? (blocks == 1 ? 7.5e-3 : 13e-3) : (blocks == 1 ? 9e-3 : 17e-3);
+    return static_cast<double>(rounds) * (a_k * static_cast<double>(inner) + 3);
+}
+
+template <typename T>
+ttamd_status launch_gated_few_rows(const GatedForward<T> &a, int device, hipStream_t st) {
+    const auto run = [&]<class MI, int RB>() -> ttamd_status {
+        switch (a.act) {
+        case kSilu: return run_few<T, MI, RB, kSilu>(a, device, st);
+        case kGelu: return run_few<T, MI, RB, kGelu>(a, device, st);
+        case kRelu: return run_few<T, MI, RB, kRelu>(a, device, st);
+        default: return run_few<T, MI, RB, kSigmoid>(a, device, st);
+        }
+    };
+    using MI = std::conditional_t<sizeof(T) == 4, Mfma16, Mfma<T>>;
+    static_assert(MI::MB == 16);
+    return few_rows_blocks(a.rows, a.hidden) == 1 ? run.template operator()<MI, 1>() : run.template operator()<MI, 2>();
+}
 
 // The tile whose workgroups, dealt to 256 CUs, are done first: workgroups of the fullest CU x tile area / the share of the
 // peak that the tile reaches (measured at inner = 1024: f32 64 x 128 0.83, 128 x 128 0.84 alone on its CU and 0.90 from two
@@ -507,6 +685,8 @@ ttamd_status launch_gated_backward_tiles(const GatedBackward<T> &a, int device, 
     return TTAMD_OK;
 }
 
+template ttamd_status launch_gated_few_rows<float>(const GatedForward<float> &, int, hipStream_t);
+template ttamd_status launch_gated_few_rows<double>(const GatedForward<double> &, int, hipStream_t);
 template ttamd_status launch_gated_forward_tiles<float>(const GatedForward<float> &, int, hipStream_t);
 template ttamd_status launch_gated_forward_tiles<double>(const GatedForward<double> &, int, hipStream_t);
 template ttamd_status launch_gated_backward_tiles<float>(const GatedBackward<float> &, int, hipStream_t);
