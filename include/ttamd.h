@@ -338,7 +338,7 @@ ttamd_status ttamd_linear_mse_head(int device, ttamd_dtype dtype, int64_t rows, 
 
 /* ---- operators of a language-model student: tokens in, a gated block, a teacher's logits as the target ----------------
  * No counterpart in the reference; they stand beside nn::Linear (nn/linear.cpp:42-50) and nn::mse_loss
- * (nn/loss.cpp:69-72).  f32 / f64.  Results are dense row-major and may not overlap an operand or one another.  A
+ * (nn/loss.cpp:69-72).  f32 / f64.  Results are dense row-major; one that shares memory with an operand or another is refused.  A
  * `workspace` is device memory of the size that the matching _workspace call names (host arithmetic only; where it names 0,
  * NULL will do), aligned to 16 bytes and the caller's own for the call: calls that may run at the same time, and graphs
  * that may be replayed at the same time, need one each.  Nothing is kept in it between calls.  Only kernels are enqueued

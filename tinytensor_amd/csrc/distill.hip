@@ -213,8 +213,8 @@ __device__ __forceinline__ void empty_row(const DistillArgs<T> &a, int64_t row) 
 // the lane's own places in LDS, and only what is beyond both is read again for the sum and for the gradient (a row of
 // 131072 floats just fits: 24 vectors in registers, 8 in LDS).  Columns behind the row's last whole vector go one by one.
 // NT: loads and stores that leave the caches alone, for matrices that would not stay in them anyway.
-// Traffic is the floor's, read once and written once: 2048 x 32000 f32 with 64 slots 97 us (5.4 TB/s; a copy of 2 GiB
-// reaches 4.9), 4096 x 131072 842 us (5.1 TB/s); as three reads and a write these took 199 and 1641 us.
+// Traffic is the floor's, read once and written once: 2048 x 32000 f32 with 64 slots 94 us (5.6 TB/s; a copy of 2 GiB
+// reaches 4.9), 4096 x 131072 880 us (4.9 TB/s); as three reads and a write these took 199 and 1641 us.
 template <typename T, int BT, int NV, bool NT>
 __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int lds_vecs) {
     using V = typename Num<T>::vec_t;
