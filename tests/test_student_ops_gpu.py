@@ -120,6 +120,23 @@ def test_embedding_gradient(tt, dtype, index, count, vocab, dim):
     assert np.array_equal(acc.to_numpy()[n == 0], before[n == 0])
 
 
+@pytest.mark.parametrize("vocab", [130560, 130561, 130817, 131071, 131072, 131073, 262144])
+@pytest.mark.parametrize("index", [np.int32, np.int64])
+def test_embedding_gradient_fullest_buckets(tt, vocab, index):
+    """Vocabularies whose buckets hold as many tokens as the counters have room for, or one fewer or more; first and last token."""
+    count, dim = 6000, 5
+    r = rng_of(vocab, 17)
+    ids = r.integers(0, vocab, count)
+    ids[:700] = 256 * r.integers(0, vocab // 256, 700) + 3  # more positions of one bucket than a wave lists
+    ids[700:710], ids[710:720], ids[720:725], ids[725:730] = 0, vocab - 1, -1, vocab
+    ids = ids.astype(index)
+    dy = r.integers(-8, 9, (count, dim)).astype(np.float32)  # whole numbers: the sums are exact
+    out, intact = framed(tt, (vocab, dim), np.float32)
+    tt.embedding_backward(tt.Tensor.from_numpy(dy), tt.Tensor.from_numpy(ids), vocab, out=out)
+    assert np.array_equal(out.to_numpy().astype(np.float64), embedding_gradient(dy, ids, vocab, 1.0)[0])
+    assert intact()
+
+
 @pytest.mark.parametrize("pattern", ["one", "blocks", "bucket", "borders"])
 def test_embedding_gradient_runs(tt, pattern):
     """Runs of equal tokens that fill, end at, cross and span the groups that are added up together."""

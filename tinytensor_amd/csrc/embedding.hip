@@ -103,7 +103,9 @@ struct OrderArgs {
 
 constexpr int kBatch = 8;  // loads of 64 indices in flight: with one at a time a scan of 60000 indices took 27 us of waiting
 
-constexpr int kListed = 256;  // positions of its bucket that a wave keeps in LDS; a wave that finds more reads its share again
+constexpr int kListed = 252;  // positions of its bucket that a wave keeps in LDS; a wave that finds more reads its share again
+// Counters, lists and the waves' sums together stay within the 64 KB that a launch may have without raising a limit.
+static_assert(kOrderWaves * (kOrderTokens * sizeof(int32_t) + kListed * sizeof(int2) + 2 * sizeof(int32_t)) <= 64 * 1024, "LDS of the order kernel");
 
 // The next kBatch x 64 positions of a wave's share: lane l's u-th token is that of position i0 + 64 u + l; -1 where there is
 // none, or where the index names no row.
