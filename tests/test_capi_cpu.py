@@ -130,3 +130,20 @@ def test_variant_names_without_gpu(tt):
     assert variant(capi.U8, 1, 64, 64, 8, (0, 64, 1), (0, 8, 1)) == "simt_u8_128x16"
     assert variant(capi.BOOL, 1, 64, 64, 64, (0, 64, 1), (0, 64, 1)) == "invalid"
     assert variant(capi.F32, 0, 64, 64, 64, (0, 64, 1), (0, 64, 1)) == "empty"
+
+
+@pytest.mark.parametrize("code", ["F32", "F64"])
+def test_thin_kernels_leave_what_a_launch_cannot_hold(tt, code):
+    """A workgroup of 1024 lanes for every 16 columns or rows: 2^32 lanes, one more than a launch holds, from 2^26 - 15 on."""
+    capi = tt._capi
+    lib, dtype = capi.lib, getattr(capi, code)
+
+    def variant(N, K, M):
+        a, b = capi.View3(), capi.View3()
+        a.data, b.data = 256, 256
+        a.stride[:], b.stride[:] = (0, 0, 1), (0, M, 1)  # (one row for all)
+        return lib.ttamd_batched_matmul_variant(dtype, 1, N, K, M, C.byref(a), C.byref(b)).decode()
+
+    edge = (1 << 26) - 16
+    assert variant(1, 8, edge).startswith("thin") and not variant(1, 8, edge + 1).startswith("thin")
+    assert variant(edge, 64, 10).startswith("thin") and not variant(edge + 1, 64, 10).startswith("thin")

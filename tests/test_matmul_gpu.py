@@ -355,6 +355,14 @@ def test_variant_selection(tt):
     assert be.batched_matmul_variant(i32, i32) == "simt_i32_64x64"
 
 
+def test_one_row_of_2_to_the_26_columns(tt):
+    """More strips of 16 columns than a launch of the thin kernel holds."""
+    T = tt.Tensor
+    row = np.random.default_rng(4).integers(-9, 10, (2, 1 << 26)).astype(np.float32)
+    got = tt.matmul(T.from_numpy(np.array([[2.0, -1.0]], np.float32)), T.from_numpy(row)).to_numpy()
+    assert np.array_equal(got, 2 * row[:1] - row[1:])
+
+
 @pytest.mark.parametrize("dtype", [np.float32, np.float64])
 def test_empty_and_degenerate_shapes(tt, dtype):
     code = tt._capi.F32 if dtype == np.float32 else tt._capi.F64

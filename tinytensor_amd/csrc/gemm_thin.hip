@@ -714,8 +714,11 @@ ttamd_status launch_linear_mse_head(int device, int64_t rows, int64_t in_feature
 ttamd_status launch_gemm_thin(ttamd_dtype dt, const GemmArgs &g, int device, hipStream_t stream, const char **variant,
                               bool variant_only, bool *handled, bool fixed_scratch) {
     *handled = false;
+    // Grid limits, a launch's lanes in the first dimension (fewer than 2^32) among them: anything beyond goes to the general kernels.
+    constexpr int kMostStrips = (1 << 22) - 1;
+    static_assert(kMostStrips * int64_t(64) * kThinWaves < int64_t(1) << 32, "lanes of a row of workgroups");
     if ((dt == TTAMD_F32 || dt == TTAMD_F64) && g.K <= 16 && g.N >= 16 && static_cast<int64_t>(g.M) * g.N >= kThinKMinOutput &&
-        g.batch <= 65535 && (g.M + 255) / 256 <= 65535) {  // (grid limits: anything beyond goes to the general kernels)
+        g.batch <= 65535 && (g.M + 255) / 256 <= 65535 && (g.N + int64_t(15)) / 16 <= kMostStrips) {
         *handled = true;
         *variant = dt == TTAMD_F32 ? "thin_f32_k16" : "thin_f64_k16";
         if (variant_only) return TTAMD_OK;
@@ -730,7 +733,7 @@ ttamd_status launch_gemm_thin(ttamd_dtype dt, const GemmArgs &g, int device, hip
     const int vec_len = dt == TTAMD_F32 ? 4 : 2;
     const bool rows_vec = g.a_sk == 1 && g.K % vec_len == 0 && g.a_sm % vec_len == 0 && g.a_sb % vec_len == 0;
     const int max_k = (rows_vec ? 4 : 2) * kThinWaves * 16 * vec_len;
-    const bool thin = g.N <= 16 && g.K >= kThinMinK && g.K <= max_k;
+    const bool thin = g.N <= 16 && g.K >= kThinMinK && g.K <= max_k && (g.M + int64_t(15)) / 16 <= kMostStrips;
     // A small output with a long reduction: on 64 x 64 tiles it would have a few tiles, split k over workgroups and add
     // the parts in a second kernel.  As 16 x 16 blocks it fills the chip in one round of workgroups (two fit a CU).
     const bool small = g.N > 16 && g.K >= kSmallMinK && g.K <= max_k && blocks <= kSmallMaxBlocks;
