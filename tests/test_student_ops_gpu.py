@@ -378,6 +378,30 @@ def test_gated_linear_beyond_32_bit_offsets(tt):
     assert np.array_equal(got[1].to_numpy(), host.T @ pg) and np.array_equal(got[2].to_numpy(), host.T @ pu)
 
 
+def test_gated_linear_largest_grids(tt):
+    """Sizes whose workgroups one launch cannot hold: the copy of 2^26 rows of 257 elements (an overlapping view: element (r, c) is
+    base[r + c]), and 2^26 columns of doubles for one row.  Whole numbers, so every sum is exact."""
+    T = tt.Tensor
+    r = rng_of(53)
+    rows, inner = 1 << 26, 257
+    base = r.integers(-1, 2, rows + inner).astype(np.float32)
+    x = T(T.from_numpy(base).storage, tt._capi.F32, (rows, inner), (1, 1), 0)
+    wg, wu = (r.integers(-1, 2, (inner, 1)).astype(np.float32) for _ in range(2))
+    try:
+        got = tt.gated_linear(x, T.from_numpy(wg), T.from_numpy(wu), activation="relu").to_numpy()[:, 0]
+        some = np.unique(np.concatenate([np.arange(0, rows, 40009), r.integers(0, rows, 3000), np.arange(64), rows - 1 - np.arange(64)]))
+        part = base[some[:, None] + np.arange(inner)]
+        assert np.array_equal(got[some], np.maximum(part @ wg, 0)[:, 0] * (part @ wu)[:, 0])
+        del x, got
+        hidden = 1 << 26
+        w = r.integers(-3, 4, (2, hidden)).astype(np.float64)
+        gate, up = (T.from_numpy(w[i:i + 1]) for i in range(2))
+        got = tt.gated_linear(T.from_numpy(np.array([[3.0]])), gate, up, activation="relu").to_numpy()
+        assert np.array_equal(got[0], np.maximum(3 * w[0], 0) * (3 * w[1]))
+    finally:
+        tt._capi.lib.ttamd_empty_cache(0)  # (70 GB of workspace)
+
+
 def test_gated_linear_shapes(tt):
     r = rng_of(11)
     x, wg, wu, bg, bu, _ = gated_data(r, np.float32, 24, 40, 36)

@@ -71,6 +71,7 @@ struct PrepareArgs {
     int hidden;
     int slope_rows, slope_blocks, slope_blocks_n;  // rows a workgroup; workgroups of the gradients; of them side by side
     CopyJob<T> copy[kCopies];
+    unsigned first;  // number of the launch's first workgroup (launch_prepare)
 };
 
 // Rows of a tile: rows in order go by vectors, one to three a lane; others are turned in LDS.
@@ -123,19 +124,20 @@ __global__ void __launch_bounds__(256) gated_prepare_kernel(PrepareArgs<T> a) {
     typedef T near_t __attribute__((ext_vector_type(VecOf<T>::W), aligned(sizeof(T))));
     constexpr int W = VecOf<T>::W;
     __shared__ T lds[64][65];
-    int block = blockIdx.x;
-    if (block >= a.slope_blocks) {
-        block -= a.slope_blocks;
+    unsigned job = a.first + blockIdx.x;
+    if (job >= static_cast<unsigned>(a.slope_blocks)) {
+        job -= a.slope_blocks;
 #pragma unroll
         for (int k = 0; k < kCopies; ++k) {
-            if (block < a.copy[k].blocks) {
-                copy_tile(a.copy[k], block, lds);
+            if (job < static_cast<unsigned>(a.copy[k].blocks)) {
+                copy_tile(a.copy[k], static_cast<int>(job), lds);
                 return;
             }
-            block -= a.copy[k].blocks;
+            job -= a.copy[k].blocks;
         }
         return;
     }
+    const int block = static_cast<int>(job);
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int row_block = block / a.slope_blocks_n, col_block = block - row_block * a.slope_blocks_n;
     const int64_t c = (static_cast<int64_t>(col_block) * 64 + lane) * W;
@@ -401,7 +403,9 @@ ttamd_status check_gated(const char *what, ttamd_dtype dtype, int64_t rows, int6
         set_error("%s: floating point dtypes only", what);
         return TTAMD_ERR_UNSUPPORTED_DTYPE;
     }
-    // (a launch holds fewer than 2^32 lanes, and every size in bytes fits 64 bits)
+    // Every size in bytes fits 64 bits, and a launch fewer than 2^32 lanes: launch_prepare goes in runs, launch_rows is left to
+    // narrower layers, and the operands, results and workspace of a call that 288 GB hold keep a grid of tiles (64 x 64 results and 256
+    // lanes at least) below 2^24 workgroups.
     constexpr int64_t most_lines = int64_t(1) << 26, most = int64_t(1) << 40;
     if (rows < 0 || inner < 1 || hidden < 1 || rows > most_lines || inner > most_lines || hidden > most_lines || rows * inner > most ||
         rows * hidden > most || inner * hidden > most) {
@@ -464,9 +468,15 @@ template <typename T>
 ttamd_status launch_prepare(int act, const PrepareArgs<T> &a, hipStream_t st) {
     int64_t blocks = a.slope_blocks;
     for (const CopyJob<T> &j : a.copy) blocks += j.blocks;
-    if (blocks == 0) return TTAMD_OK;
-    for_activation(act, [&]<int ACT>() { gated_prepare_kernel<T, ACT><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a); });
-    TTAMD_HIP_CHECK(hipGetLastError());
+    // A launch holds fewer than 2^32 lanes; copies of more than 2^32 elements have more (2^26 rows of 257 f32: 2^22 x 5 workgroups).
+    constexpr int64_t kRun = int64_t(1) << 23;
+    PrepareArgs<T> run = a;
+    for (int64_t at = 0; at < blocks; at += kRun) {
+        run.first = static_cast<unsigned>(at);
+        const unsigned n = static_cast<unsigned>(blocks - at < kRun ? blocks - at : kRun);
+        for_activation(act, [&]<int ACT>() { gated_prepare_kernel<T, ACT><<<n, 256, 0, st>>>(run); });
+        TTAMD_HIP_CHECK(hipGetLastError());
+    }
     return TTAMD_OK;
 }
 
@@ -512,7 +522,9 @@ ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, 
     const bool f32 = z.item == 4;
     const bool in_order = x.s1 == 1 && wg.s1 == 1 && wu.s1 == 1;
     const int64_t handful = f32 ? (hidden <= 4096 ? 4 : 1) : 2;
-    if (rows <= handful && wg.s1 == 1 && wu.s1 == 1 && hidden >= z.vec) {
+    // (a launch of 2^32 lanes, f64 from 2^26 - 15 columns on, is one too many)
+    const bool in_a_launch = (hidden + kRowLanes * z.vec - 1) / (kRowLanes * z.vec) * kRowThreads < int64_t(1) << 32;
+    if (rows <= handful && wg.s1 == 1 && wu.s1 == 1 && hidden >= z.vec && in_a_launch) {
         const RowArgs<T> a{x.data, wg.data, wu.data, static_cast<const T *>(gate_bias), static_cast<const T *>(up_bias), x.s0, x.s1, wg.s0, wu.s0,
                            static_cast<T *>(out), static_cast<T *>(gate), static_cast<T *>(up), static_cast<int>(rows), static_cast<int>(inner), static_cast<int>(hidden)};
         return launch_rows<T>(p.act, a, rows, st);
