@@ -390,7 +390,9 @@ ttamd_status ttamd_gated_linear_backward(int device, ttamd_dtype dtype, int acti
  * input: rows of cols elements, input_row_stride >= cols apart; teacher_index (i32 / i64) and teacher_logit: dense
  * [rows, top], 1 <= top <= 1024.  A slot whose index lies outside the columns is padding; one whose logit is -inf has
  * p = 0; an index may come twice.  row_weight: dense [rows] or NULL (1 / rows each: the mean).  A row of weight 0, or
- * without a slot that counts, adds nothing and has a gradient of zeros, whatever its logits are. */
+ * without a slot that counts, adds nothing and has a gradient of zeros, whatever its logits are.  A row's sum of
+ * exponentials is in the dtype over at most 128 terms one after another, then in 64 bits, as the loss is: its accuracy does not
+ * depend on the number of columns. */
 ttamd_status ttamd_distill_loss_workspace(ttamd_dtype dtype, int64_t rows, int64_t cols, int64_t top, size_t *bytes);
 ttamd_status ttamd_distill_loss(int device, ttamd_dtype dtype, ttamd_dtype index_dtype, int64_t rows, int64_t cols, int64_t top,
                                 const void *input, int64_t input_row_stride, const void *teacher_index,

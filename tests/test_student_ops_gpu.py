@@ -639,6 +639,45 @@ def test_distill_loss_of_millions_of_rows(tt):
 MASK_SIZES = [(6, 12), (6, 300), (6, 3001), (6, 20000), (150, 9000), (6, 90001), (130, 70001)]
 
 
+@pytest.mark.parametrize("rows, cols, large, low", [(130, (1 << 22) + 3, 1 << 16, 18.2), (1, (1 << 27) + 5, 1 << 12, 24.1)])
+def test_distill_sums_over_millions_of_columns(tt, rows, cols, large, low):
+    """`large` logits of 0 and millions of logits whose exponential 2^-low is too small to count beside what a lane has added up in
+    32 bits, but which together are 2e-4 and 2e-3 of the sum.  Rows of weight 0 hold whatever the memory held."""
+    T, u = tt.Tensor, U[np.float32]
+    z = np.full(cols, -low * np.log(2), np.float32)
+    z[:large] = 0
+    ids, t_logit = np.array([5, 70000, cols - 1]), np.array([1.0, 0.5, -1.0], np.float32)
+    where = sorted({0, rows // 2, rows - 1})
+    weight = np.zeros(rows, np.float32)
+    weight[where] = [0.25, 0.5, 1.0][:len(where)]
+    whole, one = T.empty((rows, cols), tt._capi.F32), T.from_numpy(z)
+    for r in where:
+        T(whole.storage, whole.dtype, (cols,), (1,), r * cols).assign(one)
+    loss, grad = tt.distill_loss(whole, T.from_numpy(np.tile(ids, (rows, 1))), T.from_numpy(np.tile(t_logit, (rows, 1))), row_weight=T.from_numpy(weight))
+    small = float(z[-1])
+    log_total = np.log(large + (cols - large) * np.exp(small))
+    p = np.exp(t_logit.astype(np.float64))
+    p /= p.sum()
+    lq = z[ids].astype(np.float64) - log_total
+    # Relative roundings: an exponential 4 |x| + 4; the sum 3 a vector, 8 vectors kept in LDS (the ones before them add up exactly),
+    # 10 of the tree, a conversion, or 16 and 10 of a part, a product: below 32;
+    # the quotient, the factor and the product 4 more; p of 3 slots 4 |t| + 4 each, 3 for their sum, the quotient, the weight: below 40.
+    q_tol = lambda x: (4 * np.abs(x) + 4 + 32 + 4) * u  # noqa: E731
+    for r in where:
+        w = float(weight[r])
+        got = T(grad.storage, grad.dtype, (cols,), (1,), r * cols).contiguous().to_numpy().astype(np.float64)
+        for j, i in enumerate(ids):
+            q = np.exp(lq[j])
+            assert abs(got[i] - w * (q - p[j])) <= w * (q * q_tol(z[i]) + 40 * u * p[j])
+        got = np.delete(got, ids)
+        for part, x in ((got[:large - 1], 0.0), (got[large - 1:], small)):
+            assert np.all(np.abs(part - w * np.exp(x - log_total)) <= w * np.exp(x - log_total) * q_tol(x))
+    terms = p * (np.log(p) - lq)
+    want = weight.sum(dtype=np.float64) * terms.sum()
+    tol = weight.sum(dtype=np.float64) * u * ((p * (np.abs(np.log(p) - lq) + 1)).sum() * 40 + 32) + 4 * u * abs(want)
+    assert abs(loss.to_numpy()[0] - want) <= tol
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows, cols", MASK_SIZES)
 def test_distill_masks(tt, dtype, rows, cols):

@@ -117,8 +117,8 @@ __device__ __forceinline__ T slots_exp(const DistillArgs<T> &a, const Slots<T> &
     return wave_sum(sum);
 }
 template <typename T, int BT>
-__device__ __forceinline__ double slots_loss(const DistillArgs<T> &a, const Slots<T> &s, T sum, T most, T total) {
-    const double inv = 1.0 / a.temperature, log_total = log(static_cast<double>(total));
+__device__ __forceinline__ double slots_loss(const DistillArgs<T> &a, const Slots<T> &s, T sum, T most, double total) {
+    const double inv = 1.0 / a.temperature, log_total = log(total);
     double loss = 0;
     for (int j = threadIdx.x; j < Slots<T>::padded(a.top); j += BT) {
         const T pj = s.p[j] / sum;
@@ -224,8 +224,8 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int l
     lds_t *const more = reinterpret_cast<lds_t *>(smem);  // [lds_vecs][BT]
     const Slots<T> slots(smem + static_cast<size_t>(lds_vecs) * BT * sizeof(lds_t), a.top);
     constexpr int NW = BT / 64;
-    __shared__ T red[4][NW];
-    __shared__ double loss_of[NW];
+    __shared__ T red[3][NW];
+    __shared__ double total_of[NW], loss_of[NW];
     const int64_t row = a.row0 + blockIdx.x;
     const int tid = threadIdx.x, wave = tid / 64;
     const T *zr = a.z + row * a.z_row;
@@ -287,40 +287,49 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int l
     }
     __syncthreads();
     most = join_waves<T, NW, true>(red[0]);
-    T total = T(0);
+    // What is kept on the chip is added up in T, up to 128 exponentials a lane (vector by vector first, the 24-vector form would spill
+    // five registers more: 4096 x 131072 f32 880 us against 868); what is beyond in 64 bits, for a lane may have 2^18 vectors there and
+    // a running sum in 32 would round that often (2^22 columns, some large, the others just too small to count beside them: 2e-4 of
+    // the sum was lost).
+    T near = T(0);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             held[i][k] = Num<T>::exp_scaled(held[i][k] - most, a.c);
-            total += held[i][k];
+            near += held[i][k];
         }
     for (int v = NV * BT + tid; v < lds_end; v += BT) {
         lds_t x = more[v - NV * BT];
+        T sum = T(0);
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             x[k] = Num<T>::exp_scaled(x[k] - most, a.c);
-            total += x[k];
+            sum += x[k];
         }
         more[v - NV * BT] = x;
+        near += sum;
     }
+    double total = static_cast<double>(near);
     for (int v = (NV + lds_vecs) * BT + tid; v < nvec; v += BT) {
         const V x = reinterpret_cast<const V *>(zr)[v];
+        T sum = T(0);
 #pragma unroll
-        for (int k = 0; k < W; ++k) total += Num<T>::exp_scaled(x[k] - most, a.c);
+        for (int k = 0; k < W; ++k) sum += Num<T>::exp_scaled(x[k] - most, a.c);
+        total += static_cast<double>(sum);
     }
     last = tail < a.cols ? Num<T>::exp_scaled(last - most, a.c) : T(0);
-    total += last;
+    total += static_cast<double>(last);
     total = wave_sum(total);
-    if (tid % 64 == 0) red[2][wave] = total;
+    if (tid % 64 == 0) total_of[wave] = total;
     __syncthreads();
     const T tmost = join_waves<T, NW, true>(red[1]);
     if (tmost == Num<T>::neg_inf()) {  // (no slot counts; the same for the whole workgroup)
         empty_row<T, BT>(a, row);
         return;
     }
-    total = join_waves<T, NW, false>(red[2]);
-    const T wt = w * static_cast<T>(a.temperature), f = wt / total;
+    total = join_waves<double, NW, false>(total_of);
+    const T wt = w * static_cast<T>(a.temperature), f = wt / static_cast<T>(total);
     const auto put = [&](int v, V x) {
         if constexpr (NT) __builtin_nontemporal_store(x, &reinterpret_cast<V *>(gr)[v]);
         else reinterpret_cast<V *>(gr)[v] = x;
@@ -345,9 +354,9 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int l
     }
     if (tail < a.cols) gr[tail] = last * f;
     const T tsum_wave = slots_exp<T, BT>(a, slots, tmost);  // (now that the row's vectors have left the registers)
-    if (tid % 64 == 0) red[3][wave] = tsum_wave;
+    if (tid % 64 == 0) red[2][wave] = tsum_wave;
     __syncthreads();
-    const double loss = slots_loss<T, BT>(a, slots, join_waves<T, NW, false>(red[3]), most, total);
+    const double loss = slots_loss<T, BT>(a, slots, join_waves<T, NW, false>(red[2]), most, total);
     if (tid % 64 == 0) loss_of[wave] = loss;
     __syncthreads();  // the gradient's bulk comes first, the teacher's columns are written over it
     if (tid == 0) leave_loss(a, row, static_cast<double>(w) * join_waves<double, NW, false>(loss_of));
@@ -525,8 +534,8 @@ __global__ void __launch_bounds__(kPartThreads) distill_join_kernel(DistillArgs<
     constexpr int W = Num<T>::W, NW = kPartThreads / 64;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const Slots<T> slots(smem, a.top);
-    __shared__ T red[4][NW];
-    __shared__ double loss_of[NW];
+    __shared__ T red[3][NW];
+    __shared__ double total_of[NW], loss_of[NW];
     const int64_t row = blockIdx.y;
     const int tid = threadIdx.x, wave = tid / 64;
     const T *zr = a.z + row * a.z_row;
@@ -536,7 +545,8 @@ __global__ void __launch_bounds__(kPartThreads) distill_join_kernel(DistillArgs<
     const T w = a.weight ? a.weight[row] : a.uniform_weight;
     const bool mine = blockIdx.x == 0;  // the row's loss and its columns behind the last whole vector
     V x[kPartVecs];
-    T last = Num<T>::neg_inf(), most = Num<T>::neg_inf(), total = T(0), tmost = Num<T>::neg_inf(), tsum = T(0);
+    T last = Num<T>::neg_inf(), most = Num<T>::neg_inf(), tmost = Num<T>::neg_inf(), tsum = T(0);
+    double total = 0;  // of up to 2^18 parts: in 64 bits, as in distill_row_kernel
     if (w != T(0)) {  // (the same for the whole workgroup)
 #pragma unroll
         for (int i = 0; i < kPartVecs; ++i) {
@@ -555,19 +565,19 @@ __global__ void __launch_bounds__(kPartThreads) distill_join_kernel(DistillArgs<
         __syncthreads();
         most = join_waves<T, NW, true>(red[0]);
         tmost = join_waves<T, NW, true>(red[1]);
-        for (int i = tid; i < static_cast<int>(gridDim.x); i += kPartThreads) total += own[i].total * Num<T>::exp_scaled(own[i].most - most, a.c);
+        for (int i = tid; i < static_cast<int>(gridDim.x); i += kPartThreads) total += static_cast<double>(own[i].total * Num<T>::exp_scaled(own[i].most - most, a.c));
         total = wave_sum(total);
         tsum = slots_exp<T, kPartThreads>(a, slots, tmost);
         if (tid % 64 == 0) {
-            red[2][wave] = total;
-            red[3][wave] = tsum;
+            total_of[wave] = total;
+            red[2][wave] = tsum;
         }
         __syncthreads();
-        total = join_waves<T, NW, false>(red[2]);
-        tsum = join_waves<T, NW, false>(red[3]);
+        total = join_waves<double, NW, false>(total_of);
+        tsum = join_waves<T, NW, false>(red[2]);
     }
     const bool on = w != T(0) && tmost != Num<T>::neg_inf();
-    const T wt = w * static_cast<T>(a.temperature), f = wt / total;
+    const T wt = w * static_cast<T>(a.temperature), f = wt / static_cast<T>(total);
 #pragma unroll
     for (int i = 0; i < kPartVecs; ++i) {
         const int v = first + i * kPartThreads;
