@@ -383,6 +383,13 @@ ttamd_status ttamd_gated_linear_backward(int device, ttamd_dtype dtype, int acti
                                          void *grad_gate_bias, void *grad_up_bias, void *workspace, size_t workspace_bytes,
                                          void *stream);
 
+/* Name of the kernels that a gated_linear call with these arguments would run (tests and labels; nothing is launched, biases,
+ * results and activation make no difference): forward rows1 .. rows4, few16, few32, <rows>x<columns of both weights>
+ * (_halves), products; backward 64x64 or 128x128 with _x<n> / _w<n> for reductions cut into n, products.  "empty" for no
+ * rows, "invalid" for arguments that the call refuses.  The name is valid until the thread's next call. */
+const char *ttamd_gated_linear_variant(ttamd_dtype dtype, int64_t rows, int64_t inner, int64_t hidden, const ttamd_view2 *input,
+                                       const ttamd_view2 *gate_weight, const ttamd_view2 *up_weight, int backward);
+
 /* Distillation from a teacher's top logits, loss and gradient in one call.  With T the temperature and, for every row,
  *   p = softmax of teacher_logit / T over the row's valid slots,  q = softmax of input / T over all cols columns,
  *   loss_out [1] = sum over rows of row_weight * T^2 * sum_j p_j (log p_j - log q[teacher_index_j]),

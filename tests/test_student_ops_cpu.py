@@ -205,3 +205,27 @@ def test_python_argument_checks(tt):
     ):
         with pytest.raises(tt.TTException):
             call()
+
+
+def test_gated_variant_names(tt):
+    """The kernels by size and view, without a device."""
+    capi = tt._capi
+
+    def name(rows, inner, hidden, backward=0, code=capi.F32, order=(1, 1, 1), address=256):
+        views = []
+        for cols, lines, col in zip((inner, hidden, hidden), (rows, inner, inner), order):
+            v = capi.View2()
+            v.data, v.stride[0], v.stride[1] = address, cols if col == 1 else 1, 1 if col == 1 else lines
+            views.append(v)
+        return capi.lib.ttamd_gated_linear_variant(code, rows, inner, hidden, *(C.byref(v) for v in views), backward).decode()
+
+    assert [name(n, 1024, 4096) for n in (1, 2, 3, 4)] == ["gated_f32_rows%d" % n for n in (1, 2, 4, 4)]
+    assert name(16, 1024, 4096) == "gated_f32_few16" and name(32, 2048, 8192) == "gated_f32_few32"
+    assert name(1024, 784, 1024) == "gated_f32_64x128_halves" and name(4096, 1024, 4096) == "gated_f32_256x128"
+    assert name(777, 500, 1001, code=capi.F64) == "gated_f64_64x64"
+    assert name(16, 1024, 4096, order=(1, 0, 1)) == "gated_f32_products"
+    assert name(4096, 1024, 4096, 1).startswith("gated_backward_f32_128x128") and name(64, 64, 64, 1) == "gated_backward_f32_64x64"
+    assert name(300, 4, 1 << 20, 1, capi.F64) == "gated_backward_f64_products"
+    assert name(0, 4, 4) == "empty" and name(0, 4, 4, 1) == "empty"
+    assert name(1, 0, 4) == "invalid" and name(1, 4, 4, code=capi.I32) == "invalid" and name(1, 4, 4, address=257) == "invalid"
+    assert capi.lib.ttamd_gated_linear_variant(capi.F32, 1, 4, 4, None, None, None, 0) == b"invalid"

@@ -2,6 +2,9 @@
 loss -- against their formulas in 64 bits, at the sizes, views and masks where they can go wrong.
 
 Tolerances count roundings: u is half a step of the type (2^-24, 2^-53)."""
+import ctypes as C
+import fnmatch
+import re
 import zlib
 
 import numpy as np
@@ -400,6 +403,87 @@ def test_gated_linear_largest_grids(tt):
         assert np.array_equal(got[0], np.maximum(3 * w[0], 0) * (3 * w[1]))
     finally:
         tt._capi.lib.ttamd_empty_cache(0)  # (70 GB of workspace)
+
+
+def gated_variant(tt, tx, twg, twu, backward=False):
+    """The kernels that a call of these operands runs, without the prefix and the type."""
+    v = [t.view2() for t in (tx, twg, twu)]
+    name = tt._capi.lib.ttamd_gated_linear_variant(tx.dtype, *tx.shape, twg.shape[1], *(C.byref(a) for a in v), int(backward)).decode()
+    return re.sub(r"^gated(_backward)?_f(32|64)_", "", name)
+
+
+FORWARD_TILES = [(np.float32, "64x128", 269, 71, 71), (np.float32, "64x128", 260, 40, 72), (np.float32, "64x128_halves", 280, 253, 101),
+                 (np.float32, "64x128_halves", 1000, 784, 1012), (np.float32, "128x128", 5630, 71, 130), (np.float32, "128x128", 5748, 36, 132),
+                 (np.float32, "256x128", 1539, 100, 4588), (np.float32, "256x128", 5085, 50, 1429), (np.float64, "64x64", 258, 35, 74),
+                 (np.float64, "64x64", 265, 68, 68), (np.float64, "128x128", 333, 50, 4345), (np.float64, "128x128", 261, 36, 4964),
+                 (np.float64, "256x128", 721, 36, 4828), (np.float64, "256x128", 1227, 67, 2921)]
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype, tile, rows, inner, hidden", FORWARD_TILES)
+def test_gated_linear_forward_tiles(tt, dtype, tile, rows, inner, hidden, act):
+    """Every tile of the forward grid, sizes that are no multiples of it, whole vectors and not.  Inputs of 12 bits (f64: 29) and
+    weights of -1, 0, 1, all times powers of two: g and u are exact, and no type of fewer bits could hold what they are made of."""
+    bits = 11 if dtype is np.float32 else 28
+    T, u_ = tt.Tensor.from_numpy, U[dtype]
+    r = rng_of(rows, inner, hidden, act, "tiles")
+    x = (r.integers(-2 ** bits + 1, 2 ** bits, (rows, inner)) * 2.0 ** -bits).astype(dtype)
+    wg, wu = ((r.integers(-1, 2, (inner, hidden)) * 0.25).astype(dtype) for _ in range(2))
+    bg, bu = (r.integers(-9, 10, hidden).astype(dtype) * dtype(0.25) for _ in range(2))
+    tx, twg, twu = T(x), T(wg), T(wu)
+    assert gated_variant(tt, tx, twg, twu) == tile
+    g, u = gated_reference(x, wg, wu, bg, bu, act)
+    assert (np.abs(x).sum(1).max() * 0.25 + 2.25) * 2.0 ** (bits + 2) < 1 / u_  # (exact in the type, in any order)
+    h, sg, su = tt.gated_linear(tx, twg, twu, T(bg), T(bu), activation=act, out=(frame := framed(tt, (rows, hidden), dtype))[0], save=True)
+    assert np.array_equal(sg.to_numpy(), g) and np.array_equal(su.to_numpy(), u) and frame[1]()
+    value, _ = act_of(g, act)
+    # the activation's roundings and the product's; in f64 the reference's own as well
+    own = 2 if dtype is np.float64 else 1
+    assert np.all(np.abs(h.to_numpy() - value * u) <= own * (act_error(g, act, u_)[0] + 2 * u_ * np.abs(value)) * np.abs(u))
+    plain = tt.gated_linear(tx, twg, twu, T(bg), T(bu), activation=act).to_numpy()
+    assert np.array_equal(plain, h.to_numpy())
+
+
+BACKWARD_TILES = [(np.float32, "64x64", 138, 40, 68), (np.float32, "64x64_w*", 437, 36, 68), (np.float32, "64x64_x1", 140, 36, 248),
+                  (np.float32, "64x64_x1_w*", 434, 36, 116), (np.float32, "64x64_x2", 145, 34, 383), (np.float32, "64x64_x2_w*", 351, 36, 324),
+                  (np.float32, "128x128", 1766, 1948, 932), (np.float32, "128x128", 2022, 1923, 783), (np.float32, "128x128_w*", 1353, 1092, 68),
+                  (np.float32, "128x128_w*", 1492, 1126, 67), (np.float32, "128x128_x1", 797, 1884, 1184), (np.float32, "128x128_x1", 898, 1617, 1397),
+                  (np.float32, "128x128_x1_w*", 4295, 348, 1504), (np.float32, "128x128_x1_w*", 4465, 330, 1465),
+                  (np.float32, "128x128_x16", 335, 348, 4460), (np.float32, "128x128_x4", 199, 1483, 1706),
+                  (np.float32, "128x128_x4_w*", 4640, 72, 3088), (np.float32, "128x128_x4_w*", 4814, 67, 3201), (np.float64, "64x64", 138, 34, 74),
+                  (np.float64, "64x64_w*", 427, 36, 76), (np.float64, "64x64_x1", 151, 36, 224), (np.float64, "64x64_x1_w*", 438, 37, 118),
+                  (np.float64, "64x64_x2", 148, 33, 327), (np.float64, "64x64_x2_w*", 330, 36, 344)]
+
+
+@pytest.mark.parametrize("wide", ["operands", "products"])
+@pytest.mark.parametrize("dtype, tile, rows, inner, hidden", BACKWARD_TILES)
+def test_gated_linear_backward_tiles(tt, dtype, tile, rows, inner, hidden, wide):
+    """Every tile of the backward grid with whole and cut reductions, sizes that are no multiples of it, whole vectors and not.
+    Whole numbers under relu, of 12 bits (f64: 29) on one side of each product and -1, 0, 1 on the other: every sum is exact, and
+    no type of fewer bits could hold its terms."""
+    T = tt.Tensor.from_numpy
+    r = rng_of(rows, inner, hidden, wide)
+    most = 4095 if dtype is np.float32 else 2 ** 29 - 1
+    one = lambda *n: r.integers(-1, 2, n).astype(dtype)  # noqa: E731
+    many = lambda *n: r.integers(-most, most + 1, n).astype(dtype)  # noqa: E731
+    x, wg, wu = (many if wide == "operands" else one)(rows, inner), *((many if wide == "operands" else one)(inner, hidden) for _ in range(2))
+    g, u = ((one if wide == "operands" else many)(rows, hidden) for _ in range(2))
+    dh = one(rows, hidden)
+    tx, twg, twu = T(x), T(wg), T(wu)
+    assert fnmatch.fnmatch(gated_variant(tt, tx, twg, twu, True), tile) and ("_w" in tile) == ("_w" in gated_variant(tt, tx, twg, twu, True))
+    dg, du = (dh * u * (g >= 0)).astype(np.float64), (dh * np.maximum(g, 0)).astype(np.float64)
+    wide_x, wide_g, wide_u = (a.astype(np.float64) for a in (x, wg, wu))
+    want = (dg @ wide_g.T + du @ wide_u.T, wide_x.T @ dg, wide_x.T @ du, dg.sum(0), du.sum(0))
+    size = (np.abs(dg) @ np.abs(wide_g).T + np.abs(du) @ np.abs(wide_u).T, np.abs(wide_x).T @ np.abs(dg), np.abs(wide_x).T @ np.abs(du),
+            np.abs(dg).sum(0), np.abs(du).sum(0))
+    assert max(a.max() for a in size) < 1 / U[dtype]  # (exact in any order)
+    frames = [framed(tt, a.shape, dtype) for a in want]
+    got = tt.gated_linear_backward(T(dh), tx, twg, twu, T(g), T(u), activation="relu", out=tuple(f[0] for f in frames))
+    for name, a, b, f in zip(("dx", "dwg", "dwu", "dbg", "dbu"), got, want, frames):
+        assert np.array_equal(a.to_numpy().astype(np.float64), b), name
+        assert f[1](), name
+    none = tt.gated_linear_backward(T(dh), tx, twg, twu, T(g), T(u), activation="relu", bias_grad=False)
+    assert all(np.array_equal(a.to_numpy(), b) for a, b in zip(none[:3], want))
 
 
 def test_gated_linear_shapes(tt):

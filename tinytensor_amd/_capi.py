@@ -81,6 +81,7 @@ def _bind(lib: C.CDLL) -> None:
         "ttamd_gated_linear_workspace": (i, [i] + [C.c_int64] * 3 + [i, C.POINTER(sz)]),
         "ttamd_gated_linear_forward": (i, [i, i, i] + [C.c_int64] * 3 + [C.POINTER(View2)] * 3 + [vp] * 6 + [sz, vp]),
         "ttamd_gated_linear_backward": (i, [i, i, i] + [C.c_int64] * 3 + [vp] + [C.POINTER(View2)] * 3 + [vp] * 8 + [sz, vp]),
+        "ttamd_gated_linear_variant": (C.c_char_p, [i] + [C.c_int64] * 3 + [C.POINTER(View2)] * 3 + [i]),
         "ttamd_distill_loss_workspace": (i, [i] + [C.c_int64] * 3 + [C.POINTER(sz)]),
         "ttamd_distill_loss": (i, [i, i, i] + [C.c_int64] * 3 + [vp, C.c_int64, vp, vp, vp, C.c_double, vp, vp, vp, sz, vp]),
         "ttamd_random_fill_view": (i, [i, i, i, C.c_double, C.c_double, C.POINTER(C.c_uint64), i, C.POINTER(C.c_int64),

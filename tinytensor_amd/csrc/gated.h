@@ -81,7 +81,14 @@ struct GatedBackward {
     GatedSplit split;
     T *x_part, *w_part, *b_part;        // [2 x_splits][rows, inner], [w_splits][2][inner, hidden], [w_splits][2][hidden]
 };
+// The tile of the forward grid: bm rows of x against bn / 2 columns of both weights, in `halves` parts of the reduction.
+struct ForwardTile {
+    int bm, bn, halves;
+};
+ForwardTile pick_forward_tile(size_t item, int64_t rows, int64_t hidden, int64_t k);
+
 // A block of rows: k and w_cols are the true sizes, rows begin anywhere, hidden >= 2.  The estimate is its time in us.
+int few_rows_of(int64_t rows, int64_t hidden);  // rows of a workgroup: 16 or 32
 double few_rows_estimate(size_t item, int64_t rows, int64_t inner, int64_t hidden);
 template <typename T>
 ttamd_status launch_gated_few_rows(const GatedForward<T> &a, int device, hipStream_t st);

@@ -513,23 +513,16 @@ ttamd_status launch_rows(int act, const RowArgs<T> &a, int64_t rows, hipStream_t
     return TTAMD_OK;
 }
 
+// How the forward pass goes: the row kernel, blocks of rows, one grid of tiles, or two products and a launch behind them.
+enum class Way { rows, few, tiles, products };
 template <typename T>
-ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, void *out, void *gate, void *up) {
-    hipStream_t st = static_cast<hipStream_t>(p.stream);
-    const int64_t rows = p.rows, inner = p.inner, hidden = p.hidden;
-    const GatedSizes z = sizes_of(p.dtype, rows, inner, hidden, false);
-    Operand<T> x = operand_of<T>(p.x), wg = operand_of<T>(p.wg), wu = operand_of<T>(p.wu);
+Way forward_way(const GatedSizes &z, int64_t rows, int64_t inner, int64_t hidden, const Operand<T> &x, const Operand<T> &wg, const Operand<T> &wu) {
     const bool f32 = z.item == 4;
     const bool in_order = x.s1 == 1 && wg.s1 == 1 && wu.s1 == 1;
     const int64_t handful = f32 ? (hidden <= 4096 ? 4 : 1) : 2;
     // (a launch of 2^32 lanes, f64 from 2^26 - 15 columns on, is one too many)
     const bool in_a_launch = (hidden + kRowLanes * z.vec - 1) / (kRowLanes * z.vec) * kRowThreads < int64_t(1) << 32;
-    if (rows <= handful && wg.s1 == 1 && wu.s1 == 1 && hidden >= z.vec && in_a_launch) {
-        const RowArgs<T> a{x.data, wg.data, wu.data, static_cast<const T *>(gate_bias), static_cast<const T *>(up_bias), x.s0, x.s1, wg.s0, wu.s0,
-                           static_cast<T *>(out), static_cast<T *>(gate), static_cast<T *>(up), static_cast<int>(rows), static_cast<int>(inner), static_cast<int>(hidden)};
-        return launch_rows<T>(p.act, a, rows, st);
-    }
-    PrepareArgs<T> prep{};
+    if (rows <= handful && wg.s1 == 1 && wu.s1 == 1 && hidden >= z.vec && in_a_launch) return Way::rows;
     // One grid of both products (gated_tiles.hip), unless it would be few tiles of a long reduction, which the separate
     // products cut (f32, 64 x 128 tiles: 128 x 1024 x 2048, 64 tiles, 38 us against 28 in three launches; 256 x 1024 x 4096,
     // 256 tiles, 38 against 49; f64, 64 x 64 tiles: 200 x 2001 x 1003, 128 tiles, 98 against 77; 256 x 1024 x 4096, 512
@@ -544,14 +537,31 @@ ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, 
         const bool copies = !row_vectors(x, inner) || !row_vectors(wg, hidden) || !row_vectors(wu, hidden);
         const double others = tiled ? static_cast<double>((tiles + 255) / 256 * inner) * 0.034 + (copies ? 11 : 3)
                                     : 17 + 0.0035 * static_cast<double>(inner) + 4e-6 * static_cast<double>(rows * inner) * static_cast<double>(hidden) / (f32 ? 153 : 73);
-        if (few_rows_estimate(z.item, rows, inner, hidden) < others) {
-            const GatedForward<T> a{x.data, wg.data, wu.data, x.s0, wg.s0, wu.s0, static_cast<int>(rows), static_cast<int>(inner), static_cast<int>(hidden),
-                                    static_cast<int>(hidden), p.act, static_cast<const T *>(gate_bias), static_cast<const T *>(up_bias),
-                                    static_cast<T *>(out), static_cast<T *>(gate), static_cast<T *>(up)};
-            return launch_gated_few_rows<T>(a, p.device, st);
-        }
+        if (few_rows_estimate(z.item, rows, inner, hidden) < others) return Way::few;
     }
-    if (tiled) {
+    return tiled ? Way::tiles : Way::products;
+}
+
+template <typename T>
+ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, void *out, void *gate, void *up) {
+    hipStream_t st = static_cast<hipStream_t>(p.stream);
+    const int64_t rows = p.rows, inner = p.inner, hidden = p.hidden;
+    const GatedSizes z = sizes_of(p.dtype, rows, inner, hidden, false);
+    Operand<T> x = operand_of<T>(p.x), wg = operand_of<T>(p.wg), wu = operand_of<T>(p.wu);
+    const Way way = forward_way(z, rows, inner, hidden, x, wg, wu);
+    if (way == Way::rows) {
+        const RowArgs<T> a{x.data, wg.data, wu.data, static_cast<const T *>(gate_bias), static_cast<const T *>(up_bias), x.s0, x.s1, wg.s0, wu.s0,
+                           static_cast<T *>(out), static_cast<T *>(gate), static_cast<T *>(up), static_cast<int>(rows), static_cast<int>(inner), static_cast<int>(hidden)};
+        return launch_rows<T>(p.act, a, rows, st);
+    }
+    if (way == Way::few) {
+        const GatedForward<T> a{x.data, wg.data, wu.data, x.s0, wg.s0, wu.s0, static_cast<int>(rows), static_cast<int>(inner), static_cast<int>(hidden),
+                                static_cast<int>(hidden), p.act, static_cast<const T *>(gate_bias), static_cast<const T *>(up_bias),
+                                static_cast<T *>(out), static_cast<T *>(gate), static_cast<T *>(up)};
+        return launch_gated_few_rows<T>(a, p.device, st);
+    }
+    if (way == Way::tiles) {
+        PrepareArgs<T> prep{};
         const bool own = inner % z.vec == 0;  // (x's padding meets rows of zeros in the weights' copies)
         const auto far = [&](const Operand<T> &w) { return !own || !row_vectors(w, hidden) || !within_reach(z.item, inner, w.s0); };
         if (!row_vectors(x, inner) || !within_reach(z.item, kTileLines, x.s0)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
@@ -577,6 +587,13 @@ ttamd_status forward(const Pass &p, const void *gate_bias, const void *up_bias, 
     return launch_product<T>(p.act, g, u, out, rows * hidden, st);
 }
 
+// One grid of all three products (gated_tiles.hip) unless rows or weights are beyond its reach.
+bool backward_in_a_grid(const GatedSizes &z, int64_t rows) {
+    const int64_t piece = z.split.w_splits ? z.split.w_chunk : rows;  // rows under a tile of a weight's gradient
+    return rows > 0 && within_reach(z.item, piece, z.hidden_row) && within_reach(z.item, piece, z.inner_row) &&
+           within_reach(z.item, kTileLines, z.hidden_row) && within_reach(z.item, kTileLines, z.inner_row);
+}
+
 template <typename T>
 ttamd_status backward(const Pass &p, const void *grad_out, const void *gate, const void *up, void *dx, void *dwg, void *dwu, void *dbg, void *dbu) {
     hipStream_t st = static_cast<hipStream_t>(p.stream);
@@ -598,10 +615,8 @@ ttamd_status backward(const Pass &p, const void *grad_out, const void *gate, con
         prep.slope_rows = kFewSlopeRows;
         prep.slope_blocks = static_cast<int>((rows + kFewSlopeRows - 1) / kFewSlopeRows) * prep.slope_blocks_n;
     }
-    // One grid of all three products (gated_tiles.hip) unless rows or weights are beyond its reach.
-    const int64_t piece = z.split.w_splits ? z.split.w_chunk : rows;  // rows under a tile of a weight's gradient
-    if (rows > 0 && within_reach(z.item, piece, z.hidden_row) && within_reach(z.item, piece, z.inner_row) &&
-        within_reach(z.item, kTileLines, z.hidden_row) && within_reach(z.item, kTileLines, z.inner_row)) {
+    if (backward_in_a_grid(z, rows)) {
+        const int64_t piece = z.split.w_splits ? z.split.w_chunk : rows;
         const auto far = [&](const Operand<T> &w) { return !row_vectors(w, hidden) || !within_reach(z.item, kTileLines, w.s0); };
         if (!row_vectors(x, inner) || !within_reach(z.item, piece, x.s0)) prep.copy[0] = copy_job(x, rows, inner, rows, z.inner_row, p.ws + z.x);
         if (far(wg)) prep.copy[1] = copy_job(wg, inner, hidden, inner, z.hidden_row, p.ws + z.wg);
@@ -678,6 +693,40 @@ ttamd_status ttamd_gated_linear_workspace(ttamd_dtype dtype, int64_t rows, int64
     }
     *bytes = rows > 0 ? sizes_of(dtype, rows, inner, hidden, backward != 0).bytes : 0;
     return TTAMD_OK;
+}
+
+const char *ttamd_gated_linear_variant(ttamd_dtype dtype, int64_t rows, int64_t inner, int64_t hidden, const ttamd_view2 *input,
+                                       const ttamd_view2 *gate_weight, const ttamd_view2 *up_weight, int backward) {
+    const char *const what = "gated_linear_variant";
+    if (check_gated(what, dtype, rows, inner, hidden)) return "invalid";
+    const size_t item = dtype_size(dtype);
+    if (check_view(what, "input", input, item, false) || check_view(what, "gate weight", gate_weight, item, false) ||
+        check_view(what, "up weight", up_weight, item, false))
+        return "invalid";
+    if (rows == 0) return "empty";
+    const GatedSizes z = sizes_of(dtype, rows, inner, hidden, backward != 0);
+    static thread_local char name[64];
+    const char *const type = item == 4 ? "f32" : "f64";
+    if (backward) {
+        if (!backward_in_a_grid(z, rows)) return item == 4 ? "gated_backward_f32_products" : "gated_backward_f64_products";
+        char x[16] = "", w[16] = "";
+        if (z.split.x_splits) snprintf(x, sizeof(x), "_x%d", z.split.x_splits);
+        if (z.split.w_splits) snprintf(w, sizeof(w), "_w%d", z.split.w_splits);
+        snprintf(name, sizeof(name), "gated_backward_%s_%dx%d%s%s", type, z.split.tile, z.split.tile, x, w);
+        return name;
+    }
+    const auto way_of = [&]<typename T>() { return forward_way<T>(z, rows, inner, hidden, operand_of<T>(*input), operand_of<T>(*gate_weight), operand_of<T>(*up_weight)); };
+    switch (item == 4 ? way_of.template operator()<float>() : way_of.template operator()<double>()) {
+    case Way::rows: snprintf(name, sizeof(name), "gated_%s_rows%d", type, rows > 2 ? 4 : static_cast<int>(rows)); break;
+    case Way::few: snprintf(name, sizeof(name), "gated_%s_few%d", type, few_rows_of(rows, hidden)); break;
+    case Way::tiles: {
+        const ForwardTile t = pick_forward_tile(item, rows, hidden, z.inner_row);
+        snprintf(name, sizeof(name), "gated_%s_%dx%d%s", type, t.bm, t.bn, t.halves == 2 ? "_halves" : "");
+        break;
+    }
+    case Way::products: snprintf(name, sizeof(name), "gated_%s_products", type); break;
+    }
+    return name;
 }
 
 ttamd_status ttamd_gated_linear_forward(int device, ttamd_dtype dtype, int activation, int64_t rows, int64_t inner, int64_t hidden,

@@ -505,9 +505,9 @@ ttamd_status run_forward(const GatedForward<T> &a, int device, hipStream_t st) {
 
 // Whether two halves of a reduction have the same number of k tiles (they share the engine's barriers).
 template <typename T>
-bool halves_match(int k, int bk) {
+bool halves_match(int64_t k, int bk) {
     constexpr int VK = Mfma<T>::VK;
-    const int lower = ((k + 1) / 2 + VK - 1) / VK * VK;
+    const int64_t lower = ((k + 1) / 2 + VK - 1) / VK * VK;
     return k > lower && (lower + bk - 1) / bk == (k - lower + bk - 1) / bk;
 }
 
@@ -515,12 +515,12 @@ bool halves_match(int k, int bk) {
 
 // 16 rows a workgroup while each finds a CU of its own, else 32 (32 x 4000 x 512 f32 28 us against 50; 32 x 2048 x 8192 46
 // against 29).
-static int few_rows_blocks(int64_t rows, int64_t hidden) { return rows <= 16 || (rows + 15) / 16 * ((hidden + 31) / 32) <= 256 ? 1 : 2; }
+int few_rows_of(int64_t rows, int64_t hidden) { return rows <= 16 || (rows + 15) / 16 * ((hidden + 31) / 32) <= 256 ? 16 : 32; }
 
 double few_rows_estimate(size_t item, int64_t rows, int64_t inner, int64_t hidden) {
-    const int blocks = few_rows_blocks(rows, hidden);
-    const int64_t rounds = ((rows + 16 * blocks - 1) / (16 * blocks) * ((hidden + 31) / 32) + 255) / 256;
-    const double a_k = item == 4 ? (blocks == 1 ? 7.5e-3 : 13e-3) : (blocks == 1 ? 9e-3 : 17e-3);
+    const int block = few_rows_of(rows, hidden);
+    const int64_t rounds = ((rows + block - 1) / block * ((hidden + 31) / 32) + 255) / 256;
+    const double a_k = item == 4 ? (block == 16 ? 7.5e-3 : 13e-3) : (block == 16 ? 9e-3 : 17e-3);
     return static_cast<double>(rounds) * (a_k * static_cast<double>(inner) + 3);
 }
 
@@ -536,18 +536,15 @@ ttamd_status launch_gated_few_rows(const GatedForward<T> &a, int device, hipStre
     };
     using MI = std::conditional_t<sizeof(T) == 4, Mfma16, Mfma<T>>;
     static_assert(MI::MB == 16);
-    return few_rows_blocks(a.rows, a.hidden) == 1 ? run.template operator()<MI, 1>() : run.template operator()<MI, 2>();
+    return few_rows_of(a.rows, a.hidden) == 16 ? run.template operator()<MI, 1>() : run.template operator()<MI, 2>();
 }
 
 // The tile whose workgroups, dealt to 256 CUs, are done first: workgroups of the fullest CU x tile area / the share of the
 // peak that the tile reaches (measured at inner = 1024: f32 64 x 128 0.83, 128 x 128 0.84 alone on its CU and 0.90 from two
 // on, 256 x 128 0.90 and 0.925; f64 64 x 64 0.70 alone and 0.84, 128 x 128 0.89, 256 x 128 0.91).
-template <typename T>
-ttamd_status launch_gated_forward_tiles(const GatedForward<T> &a, int device, hipStream_t st) {
-    constexpr bool f32 = sizeof(T) == 4;
-    const auto per_cu = [&](int bm, int bn) {
-        return (static_cast<int64_t>((a.rows + bm - 1) / bm) * ((a.hidden + bn / 2 - 1) / (bn / 2)) + 255) / 256;
-    };
+ForwardTile pick_forward_tile(size_t item, int64_t rows, int64_t hidden, int64_t k) {
+    const bool f32 = item == 4;
+    const auto per_cu = [&](int bm, int bn) { return ((rows + bm - 1) / bm * ((hidden + bn / 2 - 1) / (bn / 2)) + 255) / 256; };
     const auto cost = [&](int bm, int bn, double alone, double shared) {
         const int64_t n = per_cu(bm, bn);
         return static_cast<double>(n) * bm * bn / (n == 1 ? alone : shared);
@@ -555,15 +552,22 @@ ttamd_status launch_gated_forward_tiles(const GatedForward<T> &a, int device, hi
     const double small = f32 ? cost(64, 128, 0.83, 0.83) : cost(64, 64, 0.70, 0.84);
     const double large = f32 ? cost(128, 128, 0.84, 0.90) : cost(128, 128, 0.89, 0.89);
     const double xl = f32 ? cost(256, 128, 0.90, 0.925) : cost(256, 128, 0.91, 0.91);
-    if constexpr (f32) {
-        if (xl < large && xl < small) return run_forward<float, 256, 128, 16, 2, 2, 1, 1>(a, device, st);
-        if (large < small) return run_forward<float, 128, 128, 16, 2, 2, 1, 1>(a, device, st);
-        // a workgroup alone on its CU: two halves of the reduction cover each other's waits (1024 x 784 x 1024: 31.2 -> 30.5 us)
-        if (per_cu(64, 128) == 1 && a.k >= 256 && halves_match<T>(a.k, 32)) return run_forward<float, 64, 128, 32, 2, 2, 2, 2>(a, device, st);
+    if (xl < large && xl < small) return {256, 128, 1};
+    if (large < small) return {128, 128, 1};
+    if (!f32) return {64, 64, 1};
+    // a workgroup alone on its CU: two halves of the reduction cover each other's waits (1024 x 784 x 1024: 31.2 -> 30.5 us)
+    return {64, 128, per_cu(64, 128) == 1 && k >= 256 && halves_match<float>(k, 32) ? 2 : 1};
+}
+
+template <typename T>
+ttamd_status launch_gated_forward_tiles(const GatedForward<T> &a, int device, hipStream_t st) {
+    const ForwardTile tile = pick_forward_tile(sizeof(T), a.rows, a.hidden, a.k);
+    if (tile.bm == 256) return run_forward<T, 256, 128, 16, 2, 2, 1, 1>(a, device, st);
+    if (tile.bm == 128) return run_forward<T, 128, 128, 16, 2, 2, 1, 1>(a, device, st);
+    if constexpr (sizeof(T) == 4) {
+        if (tile.halves == 2) return run_forward<float, 64, 128, 32, 2, 2, 2, 2>(a, device, st);
         return run_forward<float, 64, 128, 32, 2, 2, 2, 1>(a, device, st);
     } else {
-        if (xl < large && xl < small) return run_forward<double, 256, 128, 16, 2, 2, 1, 1>(a, device, st);
-        if (large < small) return run_forward<double, 128, 128, 16, 2, 2, 1, 1>(a, device, st);
         return run_forward<double, 64, 64, 16, 2, 2, 2, 1>(a, device, st);
     }
 }
