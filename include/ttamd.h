@@ -375,7 +375,8 @@ ttamd_status ttamd_gated_linear_forward(int device, ttamd_dtype dtype, int activ
  * dg = grad_out * u * act'(g), du = grad_out * act(g); grad_input [rows, inner] = dg . Wg^T + du . Wu^T;
  * grad_{gate,up}_weight [inner, hidden] = x^T . d{g,u}; grad_{gate,up}_bias [hidden] (each may be NULL) = column sums of
  * d{g,u}.  relu's derivative is 1 at 0, as TensorRelu::backward has it (autograd/unary_ops.cpp:568-573).  rows = 0: the
- * weights' and biases' gradients are zeros. */
+ * weights' and biases' gradients are zeros.  All sums are in the dtype, those over the rows too: as in a matrix product,
+ * their errors stay below a rounding (2^-24 or 2^-53) of the sum of the terms' magnitudes for each term. */
 ttamd_status ttamd_gated_linear_backward(int device, ttamd_dtype dtype, int activation, int64_t rows, int64_t inner,
                                          int64_t hidden, const void *grad_out, const ttamd_view2 *input,
                                          const ttamd_view2 *gate_weight, const ttamd_view2 *up_weight, const void *gate,
@@ -396,7 +397,7 @@ const char *ttamd_gated_linear_variant(ttamd_dtype dtype, int64_t rows, int64_t 
  *   grad_input_out [rows, cols] = d loss / d input = row_weight * T * (q - p at the teacher's columns).
  * input: rows of cols elements, input_row_stride >= cols apart; teacher_index (i32 / i64) and teacher_logit: dense
  * [rows, top], 1 <= top <= 1024.  A slot whose index lies outside the columns is padding; one whose logit is -inf has
- * p = 0; an index may come twice.  row_weight: dense [rows] or NULL (1 / rows each: the mean).  A row of weight 0, or
+ * p = 0; an index may come twice.  With top = 1 and T = 1 this is the cross-entropy with the index as the target.  row_weight: dense [rows] or NULL (1 / rows each: the mean).  A row of weight 0, or
  * without a slot that counts, adds nothing and has a gradient of zeros, whatever its logits are.  A row's sum of
  * exponentials is in the dtype over at most 128 terms one after another, then in 64 bits, as the loss is: its accuracy does not
  * depend on the number of columns. */

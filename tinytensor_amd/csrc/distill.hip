@@ -211,10 +211,13 @@ __device__ __forceinline__ void empty_row(const DistillArgs<T> &a, int64_t row) 
 
 // A workgroup a row.  The row is requested once and stays: NV vectors of it in every lane's registers, `lds_vecs` more in
 // the lane's own places in LDS, and only what is beyond both is read again for the sum and for the gradient (a row of
-// 131072 floats just fits: 24 vectors in registers, 8 in LDS).  Columns behind the row's last whole vector go one by one.
+// 131072 floats just fits: 24 vectors in registers, of which the kernel spills 13 registers, and 8 in LDS; of the f64 forms the one
+// of 24 vectors spills 42 registers, the one of 1024 lanes and 16 vectors 10).  Columns behind the row's last whole vector go one
+// by one.
 // NT: loads and stores that leave the caches alone, for matrices that would not stay in them anyway.
 // Traffic is the floor's, read once and written once: 2048 x 32000 f32 with 64 slots 94 us (5.6 TB/s; a copy of 2 GiB
-// reaches 4.9), 4096 x 131072 880 us (4.9 TB/s); as three reads and a write these took 199 and 1641 us.
+// reaches 4.9), 4096 x 131072 870 to 880 us (4.9 TB/s); as three reads and a write these took 199 and 1641 us.  Beyond the chip
+// the third read remains: 1024 x 100003 f64 470 us of a floor of 334, 1024 x 151936 f32 279 of 254.
 template <typename T, int BT, int NV, bool NT>
 __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int lds_vecs) {
     using V = typename Num<T>::vec_t;
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(BT) distill_row_kernel(DistillArgs<T> a, int l
     __syncthreads();
     most = join_waves<T, NW, true>(red[0]);
     // What is kept on the chip is added up in T, up to 128 exponentials a lane (vector by vector first, the 24-vector form would spill
-    // five registers more: 4096 x 131072 f32 880 us against 868); what is beyond in 64 bits, for a lane may have 2^18 vectors there and
+    // four registers more: 4096 x 131072 f32 880 us against 868); what is beyond in 64 bits, for a lane may have 2^18 vectors there and
     // a running sum in 32 would round that often (2^22 columns, some large, the others just too small to count beside them: 2e-4 of
     // the sum was lost).
     T near = T(0);
@@ -668,8 +671,8 @@ ttamd_status launch_some_rows(const DistillArgs<T> &a, int64_t rows, void *parts
         };
         // The smallest form that keeps the row: small workgroups share a CU and one's loads run under another's stores
         // (4096 x 8000 f32: 51 us with 256 x 8, 117 with 1024 x 8; 2048 x 64000: 214 with 1024 x 16, 294 with 256 x 32).
-        // 24 vectors a lane only where they keep a row that 16 and LDS would not: they spill (rows beyond that: 488 us with
-        // 16, 517 with 24 at 1024 x 100003 f64).
+        // 24 vectors a lane only where they keep a row that 16 and LDS would not: they spill (rows beyond that, 1024 x 100003 f64:
+        // 1.06 times as long with 24 as with 16).
         const auto pick = [&]<bool NT>() {
             if (nvec <= 256 * 4) return run(distill_row_kernel<T, 256, 4, NT>, 256, 4);
             if (nvec <= 256 * 8) return run(distill_row_kernel<T, 256, 8, NT>, 256, 8);

@@ -1,7 +1,7 @@
 // embedding.hip — rows of a table looked up by token, scaled, and the table's gradient (gfx950).
 //
 //   out[i] = scale * table[index[i]]            (an index outside the table: a row of zeros)
-//   dtable[v] = scale * sum of dy[i] over the positions i with index[i] = v, in the order of the positions
+//   dtable[v] = scale * sum of dy[i] over the positions i with index[i] = v, in groups of ordered positions
 // No counterpart in the reference; the layer stands in front of nn::Linear (nn/linear.cpp:42-50).
 //
 // Bound: HBM in both directions.  The gradient of a token is a sum over positions that lie anywhere, so the positions are
@@ -434,7 +434,8 @@ __device__ __forceinline__ void add_parts(const SumArgs<T> &a, int64_t c, int64_
 
 // The run that begins in chunk c and goes on: its parts are partial[2 c + 1] and partial[2 j] of the following chunks j
 // that begin with its token.  A wave joins a run of few parts, a workgroup one of many, whose waves add
-// contiguous shares, and the shares' sums are added in order.  The runs come in the order in which their chunks were listed,
+// contiguous shares, and the shares' sums are added in order.  (The f32 vector form keeps eight parts of four doubles in flight and
+// spills 20 registers.)  The runs come in the order in which their chunks were listed,
 // which changes from call to call and no result with it.
 template <typename T, int W>
 __global__ void __launch_bounds__(64 * kJoinWaves) embedding_join_kernel(SumArgs<T> a) {

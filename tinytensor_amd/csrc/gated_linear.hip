@@ -493,9 +493,10 @@ struct Pass {
     void *stream;
 };
 
-// Up to 4 rows (f32; 2 f64) in one launch: 1 x 2048 x 2048 f32 13.2 us against 18.3 on the matrix cores
-// (gated_few_kernel), 4 x 4000 x 512 27 against 33, f64 2 x 2048 x 2048 16.6 against 22.2; f32 of more columns only 1 row (1 x 2048 x 8192
-// 22.6 against 21.6, 4.9 TB/s; 4 x 2048 x 8192 28.9 against 22).
+// Up to 4 rows (f32; 2 f64) in one launch: 1 x 2048 x 2048 f32 13.2 us against 18.6 on the matrix cores (gated_few_kernel),
+// 4 x 4000 x 512 27 against 33, f64 2 x 2048 x 2048 16.7 against 23.2.  f32 of more than 4096 columns only 1 row: 4 x 2048 x 8192 28.7
+// against 21.8, while 1 row gains up to a fifth (1 x 2048 x 8200 36.5 against 44.6, 4096 x 12000 69 against 84) and loses up to
+// an eighth (2048 x 8192 22.4 against 21.5, 2048 x 16384 55 against 48).
 template <typename T>
 ttamd_status launch_rows(int act, const RowArgs<T> &a, int64_t rows, hipStream_t st) {
     constexpr int kCols = kRowLanes * VecOf<T>::W;

@@ -134,7 +134,7 @@ __device__ __forceinline__ void store_gated(Engine &eng, const GatedForward<T> &
     }
 }
 
-// BM rows of x against BN / 2 columns of both weights.  HALVES = 2: lanes 0-255 take the first half of the reduction, lanes
+// BM rows of x against BN / 2 columns of both weights (the tiles of 256 rows spill 2 registers in f32, 8 in f64).  HALVES = 2: lanes 0-255 take the first half of the reduction, lanes
 // 256-511 the second, each with buffers of its own (for grids of about a workgroup per CU, see gemm_mfma_dual_kernel); the
 // halves have the same number of k tiles.
 template <typename T, int BM, int BN, int BK, int WGM, int WGN, int PF, int HALVES>
@@ -179,7 +179,8 @@ gated_forward_kernel(GatedForward<T> a, int tiles_m, int tiles_n, int k_half) {
 // The backward pass's products as one grid of B x B tiles: first the tiles of dx = dg . Wg^T + du . Wu^T (two reductions one
 // after the other), then those of dWg = x^T . dg and dWu = x^T . du, whose first rows of tiles also add up the vectors
 // of dg / du that they stage: the bias gradients.  At least two workgroups share a CU, and one's first loads and stores run
-// under the other's products; the long reductions of dx go first and the weights' tiles fill up beside them.
+// under the other's products; the long reductions of dx go first and the weights' tiles fill up beside them.  The f32 kernel of
+// 128 x 128 tiles spills 48 registers, the accumulators set aside between dx's two reductions.
 template <typename T, int B>
 struct BackwardTile {
     static constexpr int BK = sizeof(T) == 4 && B == 64 ? 32 : 16;
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__((FewShape<T, MI, RB>::NW * 64)) gated_few_kern
                     for (int c = 0; c < CB; ++c) acc[m][r][c] = MI::mma(x[r][j], w[m][j][c], acc[m][r][c]);
     };
     // A wave's next group is requested once the last one has been multiplied; the other waves' loads fill the time.  (Two to
-    // four groups in flight a wave: 32 x 2048 x 8192 f32 42 us instead of 29.)
+    // four groups in flight a wave: 1.4 times as long at 32 x 2048 x 8192 f32.)
     const int groups = a.k / kGroup;
     if (wave < groups) {
         load(static_cast<int64_t>(wave) * kGroup);
@@ -513,8 +514,8 @@ bool halves_match(int64_t k, int bk) {
 
 }  // namespace
 
-// 16 rows a workgroup while each finds a CU of its own, else 32 (32 x 4000 x 512 f32 28 us against 50; 32 x 2048 x 8192 46
-// against 29).
+// 16 rows a workgroup while each finds a CU of its own, else 32 (32 x 4000 x 512 f32 35 us against 55 with 32; 32 x 2048 x 8192 42
+// with 16 against 32).
 int few_rows_of(int64_t rows, int64_t hidden) { return rows <= 16 || (rows + 15) / 16 * ((hidden + 31) / 32) <= 256 ? 16 : 32; }
 
 double few_rows_estimate(size_t item, int64_t rows, int64_t inner, int64_t hidden) {
