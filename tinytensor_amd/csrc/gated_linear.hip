@@ -61,7 +61,7 @@ struct CopyJob {
     const T *src;
     int64_t s0, s1, rows, cols, dst_rows, dst_row;
     T *dst;
-    int blocks;  // tiles of dst, copy_rows() x 64; 0: nothing to copy
+    int blocks;  // tiles of dst, copy_rows() x 64: little more than 2^30 for the 2^40 elements that check_gated allows; 0: nothing to copy
 };
 template <typename T>
 struct PrepareArgs {
